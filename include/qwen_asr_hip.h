@@ -471,6 +471,97 @@ int qwen_hip_causal_attention(float *out, const float *Q, const float *K, const 
 int qwen_hip_argmax_matvec_bf16(const float *x, const uint16_t *W_bf16,
                                 int in_dim, int out_dim, hipStream_t s);
 
+/* ------------------------------------------------------------------------
+ * Paged KV cache and token drawing: operators for a program that serves
+ * several streams at once.  No counterpart in the reference (one contiguous
+ * cache, one stream, greedy decoding).  Device pointers of the current device;
+ * every call only enqueues on s (no allocation, no synchronisation), so it can
+ * be captured into a graph; what a call needs besides is in the workspace that
+ * the caller passes.  A workspace is free again when the call's kernels have
+ * run: calls that may overlap (two streams, two graphs replayed at once) need
+ * one each; its contents do not matter.  rows == 0 launches nothing.
+ * ------------------------------------------------------------------------ */
+
+/* One layer's cache.  Position p of sequence s is slot p % page_size of page
+ * table[s][p / page_size]; pages may stand in any order, and sequences may
+ * share pages that neither writes.  A page id outside [0, n_pages) (-1) is no
+ * page: attention does not see its positions, append stores nothing there.
+ * Positions past table_stride * page_size (at most 2^30) are not there either. */
+typedef struct {
+    void *k, *v;            /* [n_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    const int *table;       /* [n_seqs][table_stride] */
+    int dtype;              /* QWEN_HIP_ST_F32 or QWEN_HIP_ST_BF16 */
+    int n_pages;
+    int page_size;          /* a power of two, 1 .. 2^24 */
+    int kv_heads;
+    int head_dim;           /* QWEN_HIP_HEAD_DIM */
+    int n_seqs;
+    int table_stride;       /* page ids per sequence */
+} qwen_hip_paged_kv;
+
+/* The rows of one call.  Sequence s owns rows row_start[s] .. row_start[s + 1] - 1
+ * (row_start not falling, within 0 .. rows); its last row sits at position
+ * kv_len[s] - 1, the others right before it.  Rows before row_start[0] or from
+ * row_start[n_seqs] on belong to no sequence: nothing reads or writes what
+ * stands at their place in the outputs.  row_start NULL: row s is sequence s's
+ * only one (rows == n_seqs). */
+typedef struct {
+    const int *row_start;   /* [n_seqs + 1] or NULL */
+    const int *kv_len;      /* [n_seqs]: cached positions with the call's rows (negative counts as 0) */
+    int rows;
+    int max_len;            /* about the longest kv_len, for the launch's shape only: results hold for
+                               any (0: the table's capacity) */
+} qwen_hip_paged_batch;
+
+/* New rows enter the cache: queries and keys get an RMS norm per head (q_norm,
+ * k_norm [head_dim], both NULL: none, as qwen_hip_rms_norm_per_head) and the
+ * NeoX rotation of their position (cos_vals, sin_vals [n_pos][head_dim], both
+ * NULL: none, as qwen_hip_apply_rope_neox with a table of positions); keys and
+ * values go to their pages, queries to q_out [rows][heads * head_dim].  q, k, v
+ * and q_out hold `dtype` (either of the two); rows of q are q_stride values
+ * apart, those of k and v kv_stride (at least a row, multiples of 16 bytes).
+ * q_out may be q (q_stride == heads * head_dim).  All arithmetic in fp32, rounded
+ * once to nearest even.  Pointers 16-byte aligned.  A row at a negative position
+ * or at one from n_pos on is left out altogether. */
+int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *q_out,
+                          const void *q, const void *k, const void *v, int dtype, long q_stride, long kv_stride,
+                          int heads, const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
+                          const float *sin_vals, int n_pos, hipStream_t s);
+
+/* Causal attention over the cache, q and out [rows][heads * head_dim] of
+ * `dtype` (out not q): a row sees the positions up to its own that are there;
+ * one that sees none gets 0.  heads is a multiple of kv_heads; `scale` positive,
+ * 1e-30 .. 1e30.  _decode takes one row per sequence (row_start NULL), _prefill
+ * packed rows (row_start given; sequences may have no rows, one, or all of their
+ * positions).  Softmax statistics and sums in fp32.  fp32 rows: products exact to
+ * 2^-24 on either cache type; bf16 rows: _prefill rounds the probabilities to
+ * bf16 before they meet V.  The workspace holds the partial results of a split
+ * over the positions. */
+size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);
+int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
+                                    const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
+                                    hipStream_t s);
+int qwen_hip_paged_attention_prefill(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
+                                     const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
+                                     hipStream_t s);
+
+/* One token per row of logits [rows][vocab] (rows row_stride entries apart), as
+ * given by the row's parameters (device arrays [rows], each may be NULL: off):
+ *   temperature  logits are divided by it; 0, negative or NaN: the largest logit
+ *   top_k        only the top_k largest (<= 0 or >= vocab: off; ties: lower index first)
+ *   top_p        of those, while the probability before an entry, in that order, is
+ *                below top_p (>= 1 or NaN: off; the first always stays)
+ *   min_p        of those, the ones with at least min_p times the largest probability
+ *                (<= 0 or NaN: off; above 1 as 1)
+ * and then the first index at which the probability of the entries up to it passes
+ * u[row] (a random number in [0, 1), clamped to it).  NaN logits never come out;
+ * a row without any entry above -infinity gives -1.  vocab up to 2^20, rows up to
+ * 2^16.  The same inputs give the same tokens. */
+size_t qwen_hip_sample_ws_bytes(int rows, int vocab);
+int qwen_hip_sample(int *tokens, const float *logits, long row_stride, int rows, int vocab,
+                    const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+                    const float *u, void *ws, size_t ws_bytes, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

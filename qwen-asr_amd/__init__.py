@@ -37,6 +37,17 @@ class LayerWeights(C.Structure):
                                           "q_norm", "k_norm", "input_norm", "post_attn_norm")]
 
 
+class PagedKV(C.Structure):
+    """qwen_hip_paged_kv: one layer's pages and the sequences' page table (device pointers)"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p)] + \
+        [(n, C.c_int) for n in ("dtype", "n_pages", "page_size", "kv_heads", "head_dim", "n_seqs", "table_stride")]
+
+
+class PagedBatch(C.Structure):
+    """qwen_hip_paged_batch: the rows of one call (device pointers)"""
+    _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("rows", C.c_int), ("max_len", C.c_int)]
+
+
 def build(jobs=8):
     """Compile the library in-tree (hipcc for gfx950 + gcc)."""
     subprocess.run(["make", "-s", "-C", HERE, f"-j{jobs}"], check=True)
@@ -120,6 +131,12 @@ SIGNATURES = [
     ("qwen_hip_linear_noalloc_max_bytes", C.c_size_t, []),
     ("qwen_hip_causal_attention", _i, [_vp] * 4 + [_i] * 5 + [_f, _i, _vp]),
     ("qwen_hip_argmax_matvec_bf16", _i, [_vp, _vp, _i, _i, _vp]),
+    ("qwen_hip_paged_append", _i, [_vp] * 6 + [_i, C.c_long, C.c_long, _i, _vp, _vp, _f, _vp, _vp, _i, _vp]),
+    ("qwen_hip_paged_attention_ws_bytes", C.c_size_t, [_vp, _vp, _i]),
+    ("qwen_hip_paged_attention_decode", _i, [_vp] * 4 + [_i, _i, _f, _vp, C.c_size_t, _vp]),
+    ("qwen_hip_paged_attention_prefill", _i, [_vp] * 4 + [_i, _i, _f, _vp, C.c_size_t, _vp]),
+    ("qwen_hip_sample_ws_bytes", C.c_size_t, [_i, _i]),
+    ("qwen_hip_sample", _i, [_vp, _vp, C.c_long, _i, _i] + [_vp] * 6 + [C.c_size_t, _vp]),
     ("qwen_synth_key", _u64, [_u64, _u64]),
     ("qwen_f32_to_bf16_rne", C.c_uint16, [_f]),
     ("qwen_synth_normal_bf16", None, [_vp, C.c_size_t, _u64, _u64, _d, _d, _i]),

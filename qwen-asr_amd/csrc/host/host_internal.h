@@ -34,4 +34,13 @@ void qk_set_err(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
         }                                                                       \
     } while (0)
 
+/* an argument that an entry point refuses */
+#define QK_REFUSE(...)                                                          \
+    do {                                                                        \
+        qk_set_err(__VA_ARGS__);                                                \
+        return QWEN_HIP_EINVAL;                                                 \
+    } while (0)
+
+static inline int qk_aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
+
 #endif

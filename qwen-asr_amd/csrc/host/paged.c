@@ -1,0 +1,153 @@
+/*
+ * paged.c - op-level ABI of the paged KV cache: appending rows, attention of
+ * single tokens and of packed prompts.  No counterpart in the reference, which
+ * keeps one contiguous cache for one stream (qwen_asr_decoder.c:122-160).
+ *
+ * Host checks cover everything the host can see (types, shapes, alignment,
+ * the workspace's size).  Lengths, row starts and page ids are device data:
+ * the kernels clamp them.  Nothing here allocates or synchronises.
+ */
+#include "host_internal.h"
+
+#include <float.h>
+#include <limits.h>
+#include <math.h>
+
+#define MAX_CAPACITY (1L << 30)   /* positions of one sequence */
+
+static int is_dtype(int t) { return t == QWEN_HIP_ST_F32 || t == QWEN_HIP_ST_BF16; }
+
+/* the cache and the batch, checked, in the kernels' form */
+static int paged_view(const char *op, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *b, int heads,
+                      int dtype, qk_paged *p) {
+    if (!kv || !b) QK_REFUSE("%s: no cache or no batch", op);
+    if (!is_dtype(kv->dtype) || !is_dtype(dtype))
+        QK_REFUSE("%s: types are QWEN_HIP_ST_F32 or QWEN_HIP_ST_BF16 (rows %d, cache %d)", op, dtype, kv->dtype);
+    if (kv->head_dim != QWEN_HIP_HEAD_DIM) QK_REFUSE("%s: head_dim %d (only %d)", op, kv->head_dim, QWEN_HIP_HEAD_DIM);
+    if (kv->page_size <= 0 || kv->page_size > (1 << 24) || (kv->page_size & (kv->page_size - 1)))
+        QK_REFUSE("%s: page_size %d is no power of two up to 2^24", op, kv->page_size);
+    if (kv->n_pages <= 0 || kv->kv_heads <= 0 || kv->n_seqs < 0 || kv->table_stride <= 0)
+        QK_REFUSE("%s: n_pages %d, kv_heads %d, n_seqs %d, table_stride %d", op, kv->n_pages, kv->kv_heads, kv->n_seqs,
+               kv->table_stride);
+    if (heads <= 0 || heads % kv->kv_heads) QK_REFUSE("%s: %d heads over %d kv heads", op, heads, kv->kv_heads);
+    if (b->rows < 0 || b->max_len < 0) QK_REFUSE("%s: rows %d, max_len %d", op, b->rows, b->max_len);
+    if ((long)b->rows * heads > INT_MAX / QWEN_HIP_HEAD_DIM) QK_REFUSE("%s: %d rows of %d heads", op, b->rows, heads);
+    if ((long)kv->n_seqs * kv->kv_heads > INT_MAX / 2) QK_REFUSE("%s: %d sequences of %d kv heads", op, kv->n_seqs, kv->kv_heads);
+    if (!b->row_start && b->rows != kv->n_seqs)
+        QK_REFUSE("%s: without row_start a sequence has one row (%d rows, %d sequences)", op, b->rows, kv->n_seqs);
+    int shift = 0;
+    while ((1 << shift) < kv->page_size) shift++;
+    const long cap = (long)kv->table_stride << shift;
+    *p = (qk_paged){.k = kv->k, .v = kv->v, .table = kv->table, .row_start = b->row_start, .kv_len = b->kv_len,
+                    .cache_bf16 = kv->dtype == QWEN_HIP_ST_BF16, .n_pages = kv->n_pages, .page_shift = shift,
+                    .kv_heads = kv->kv_heads, .n_seqs = kv->n_seqs, .table_stride = kv->table_stride,
+                    .rows = b->rows, .capacity = (int)(cap < MAX_CAPACITY ? cap : MAX_CAPACITY)};
+    return 0;
+}
+
+/* ... and the pointers that a call with rows reads */
+static int paged_pointers(const char *op, const qk_paged *p) {
+    if (!p->k || !p->v || !p->table || !p->kv_len) QK_REFUSE("%s: a pointer of the cache or the batch is NULL", op);
+    if (!qk_aligned16(p->k) || !qk_aligned16(p->v)) QK_REFUSE("%s: the pages are not 16-byte aligned", op);
+    return 0;
+}
+
+int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *q_out, const void *q,
+                          const void *k, const void *v, int dtype, long q_stride, long kv_stride, int heads,
+                          const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
+                          const float *sin_vals, int n_pos, hipStream_t s) {
+    static const char op[] = "paged_append";
+    qk_paged_append_args a = {0};
+    const int rc = paged_view(op, kv, batch, heads, dtype, &a.pg);
+    if (rc) return rc;
+    const int unit = dtype == QWEN_HIP_ST_F32 ? 4 : 8;
+    if (q_stride < (long)heads * QWEN_HIP_HEAD_DIM || kv_stride < (long)kv->kv_heads * QWEN_HIP_HEAD_DIM ||
+        q_stride % unit || kv_stride % unit)
+        QK_REFUSE("%s: row strides %ld, %ld (at least a row, multiples of 16 bytes)", op, q_stride, kv_stride);
+    if (!q_norm != !k_norm || !cos_vals != !sin_vals) QK_REFUSE("%s: one norm or one rotation table of two", op);
+    if (q_norm && !(eps >= 0.0f && eps <= FLT_MAX)) QK_REFUSE("%s: eps %g", op, (double)eps);
+    if (n_pos < 0) QK_REFUSE("%s: n_pos %d", op, n_pos);
+    if (batch->rows == 0) return 0;
+    if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
+    if (!q_out || !q || !k || !v) QK_REFUSE("%s: a pointer of the rows is NULL", op);
+    if (!qk_aligned16(q_out) || !qk_aligned16(q) || !qk_aligned16(k) || !qk_aligned16(v) || !qk_aligned16(q_norm) ||
+        !qk_aligned16(k_norm) || !qk_aligned16(cos_vals) || !qk_aligned16(sin_vals))
+        QK_REFUSE("%s: a pointer is not 16-byte aligned", op);
+    if (q_out == q && q_stride != (long)heads * QWEN_HIP_HEAD_DIM)
+        QK_REFUSE("%s: in place the queries' rows are %d values apart", op, heads * QWEN_HIP_HEAD_DIM);
+    a.q_out = q_out;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.act_bf16 = dtype == QWEN_HIP_ST_BF16;
+    a.heads = heads;
+    /* without a table no position is out of it */
+    a.n_pos = cos_vals ? n_pos : INT_MAX;
+    a.q_stride = q_stride;
+    a.kv_stride = kv_stride;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.cos_v = cos_vals;
+    a.sin_v = sin_vals;
+    a.eps = eps;
+    QK_TRY(qk_paged_append_launch(&a, s));
+    return 0;
+}
+
+/* splits of an attention call and the workspace it needs */
+static size_t attention_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk) {
+    if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;
+    if (p->row_start) qk_paged_prefill_plan(p->rows, p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
+    else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
+    if (*nsplit == 1) return 0;
+    return (size_t)p->rows * heads * *nsplit * (QWEN_HIP_HEAD_DIM + 2) * sizeof(float);
+}
+
+size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
+    qk_paged p;
+    int nsplit, chunk;
+    if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || p.rows == 0) return 0;
+    return attention_plan(&p, heads, batch->max_len, &nsplit, &chunk);
+}
+
+static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch,
+                     void *out, const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
+                     hipStream_t s) {
+    qk_paged_attn_args a = {0};
+    const int rc = paged_view(op, kv, batch, heads, dtype, &a.pg);
+    if (rc) return rc;
+    if (prefill && !batch->row_start) QK_REFUSE("%s: no row_start", op);
+    if (!prefill && batch->row_start) QK_REFUSE("%s: one row per sequence: row_start has to be NULL", op);
+    if (!(scale >= 1e-30f && scale <= 1e30f)) QK_REFUSE("%s: scale %g", op, (double)scale);
+    if (batch->rows == 0) return 0;
+    if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
+    if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
+    if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);
+    if (out == q) QK_REFUSE("%s: out cannot be q", op);
+    const size_t need = attention_plan(&a.pg, heads, batch->max_len, &a.nsplit, &a.chunk);
+    if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
+        QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);
+    a.out = out;
+    a.q = q;
+    a.act_bf16 = dtype == QWEN_HIP_ST_BF16;
+    a.heads = heads;
+    a.scale = scale;
+    a.part_o = (float *)ws;
+    a.part_ml = need ? a.part_o + (size_t)a.pg.rows * heads * a.nsplit * QWEN_HIP_HEAD_DIM : NULL;
+    if (prefill) QK_TRY(qk_paged_prefill_launch(&a, s));
+    else QK_TRY(qk_paged_decode_launch(&a, s));
+    if (need) QK_TRY(qk_paged_merge_launch(&a, s));
+    return 0;
+}
+
+int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
+                                    const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
+                                    hipStream_t s) {
+    return attention("paged_attention_decode", 0, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+}
+
+int qwen_hip_paged_attention_prefill(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
+                                     const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
+                                     hipStream_t s) {
+    return attention("paged_attention_prefill", 1, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+}

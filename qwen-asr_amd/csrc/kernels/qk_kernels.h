@@ -478,6 +478,63 @@ int qk_enc_ring_ok(const struct qwen_hip_encoder *e);
 /* whether forward_device reads a mel of this memory type and device where it is */
 int qk_enc_mel_in_place(int type, int mem_device, int device);
 
+/* ---- paged KV cache ---------------------------------------------------- */
+/* The cache's pages and the batch's rows as the kernels see them (device
+ * pointers; checked by the host, csrc/host/paged.c). */
+typedef struct {
+    void *k, *v;              /* [n_pages][kv_heads][1 << page_shift][128] */
+    const int *table;         /* [n_seqs][table_stride] page ids */
+    const int *row_start;     /* [n_seqs + 1], NULL: row i belongs to sequence i */
+    const int *kv_len;        /* [n_seqs] */
+    int cache_bf16, n_pages, page_shift, kv_heads, n_seqs, table_stride, rows;
+    int capacity;             /* min(table_stride << page_shift, INT_MAX) */
+} qk_paged;
+
+typedef struct {
+    qk_paged pg;
+    void *q_out;
+    const void *q, *k, *v;
+    int act_bf16, heads, n_pos;
+    long q_stride, kv_stride;
+    const float *q_norm, *k_norm, *cos_v, *sin_v;
+    float eps;
+} qk_paged_append_args;
+int qk_paged_append_launch(const qk_paged_append_args *a, hipStream_t s);
+
+/* Attention partials of split s of row r, head h: o[((r * heads + h) * nsplit + s) * 128 ..],
+ * unnormalised, and ml[2 * (..)] = (maximum in base 2, sum); a split without keys has the sum 0
+ * and no o. */
+typedef struct {
+    qk_paged pg;
+    void *out;
+    const void *q;
+    int act_bf16, heads;
+    float scale;
+    int nsplit, chunk;        /* keys per split, unless a sequence is longer than nsplit of them */
+    float *part_o, *part_ml;  /* nsplit > 1 */
+} qk_paged_attn_args;
+#define QK_PAGED_MAX_SPLIT 64
+/* splits and keys per split for sequences of up to max_len positions */
+void qk_paged_decode_plan(int n_seqs, int heads, int kv_heads, int max_len, int *nsplit, int *chunk);
+void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_heads, int max_len, int *nsplit, int *chunk);
+int qk_paged_decode_launch(const qk_paged_attn_args *a, hipStream_t s);
+int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s);
+/* joins the partials into out */
+int qk_paged_merge_launch(const qk_paged_attn_args *a, hipStream_t s);
+
+/* ---- drawing tokens ----------------------------------------------------- */
+typedef struct {
+    int *tokens;
+    const float *logits;
+    long row_stride;
+    int rows, vocab;
+    const float *temperature, *top_p, *min_p, *u;   /* [rows], NULL: off */
+    const int *top_k;
+    void *ws;
+} qk_sample_args;
+size_t qk_sample_ws_bytes(int rows, int vocab);
+int qk_sample_launch(const qk_sample_args *a, hipStream_t s);
+
 /* ---- elementwise (op-level ABI) --------------------------------------- */
 int qk_add_launch(float *a, const float *b, long n, hipStream_t s);
 int qk_rms_norm_launch(float *out, const float *x, const float *w, int S, int D,
