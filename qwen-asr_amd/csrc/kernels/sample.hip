@@ -13,14 +13,15 @@
 // held as integers, w_i 2^43 cut off (2^20 entries sum to less than 2^64), so sums do
 // not depend on the order of the atomics and every launch sees the same ones; what
 // is cut is below 2^-43 of the largest weight for each entry, against the 2^-24 of an
-// fp32 exponential.  a_i is computed in 64 bits, the exponential's fraction on the
-// hardware (v_exp_f32, 1 ulp).
+// fp32 exponential.  y_i = a_i log2(e) is held as the sum of two fp32 numbers (the
+// difference and the product with their rounding errors), so the weight's only
+// errors are those of v_exp_f32 (1 ulp) and of its argument's fraction (2^-25).
 //
 // Four launches over blocks of the row, each reading the row once (from the
 // caches after the first time):
 //   sample_max    largest and smallest finite logit of each block's share
-//   sample_hist   count and weight of SM_BINS classes of a, evenly over the row's range
-//                 (at most 32: the last class holds what weighs 0)
+//   sample_hist   count (for top-k) and weight (for top-p) of SM_BINS classes of y, evenly
+//                 over the row's range (at most 32 log2(e): the last class weighs 0)
 //   sample_pick   from the classes' running sums: which are kept whole, and which hold
 //                 a threshold.  Entries of the latter go to a short list, the former
 //                 are summed per 1024 entries
@@ -28,8 +29,6 @@
 //                 thresholds, and walks the sums down to the one entry
 // A row whose threshold classes hold more than SM_CAND entries (nearly equal
 // logits) takes a radix selection over the row in the last launch instead.
-// Bound by launch latency for few rows; for many by reading the row and the
-// 64-bit arithmetic on each entry.
 #include "common.h"
 #include "qk_kernels.h"
 #include "qwen_asr_hip.h"
@@ -43,24 +42,26 @@
 #define SM_MAX_BLOCKS 256
 #define SM_ONE (1ull << 43)
 
+struct SmPar {
+    float M, c, c_lo;             // largest logit; log2(e) / T in two parts
+    float scale;                  // classes per unit of y
+    float lim, lim_lo;            // largest y that min-p keeps, in two parts
+    float top_p;                  // >= 1: off
+    int k;                        // 0: off
+    int none;                     // no entry at all
+};
+
 struct SmRow {                    // one row's part of the workspace
     unsigned long long weight[SM_BINS];
     unsigned count[SM_BINS];
     float max[SM_MAX_BLOCKS], min[SM_MAX_BLOCKS];
-    unsigned n_cand, slow, pad[2];
-    int lo, hi, bk, pad1;         // classes below lo are kept whole; lo .. hi and bk hold the thresholds
+    SmPar par;
+    unsigned n_cand, pad[2];
+    int lo, hi, bk;               // classes below lo are kept whole; lo .. hi and bk hold the thresholds
     unsigned count_k;             // entries before class bk
-    unsigned pad2;
-    unsigned long long weight_k, weight_lo, weight_all;   // before bk, before lo, of the row
-    unsigned cand[SM_CAND];
+    unsigned long long weight_k, weight_lo, weight_all, pad2;   // before bk, before lo, of the row
+    unsigned long long cand[SM_CAND];                           // the logit's bits, the index
     unsigned long long sub[SM_MAX_SUBS];
-};
-
-struct SmPar {
-    double M, inv_t, scale, lim;  // largest logit; 1 / T; classes per unit of a; largest a that min-p keeps
-    float top_p;                  // >= 1: off
-    int k;                        // 0: off
-    bool none;                    // no entry at all
 };
 
 // the value as it counts: what is no number never does, -0 is 0
@@ -76,27 +77,40 @@ __device__ __forceinline__ unsigned long long sm_comp(float l, int i) {
     return (unsigned long long)sm_key(l) << 32 | (0xffffffffu - (unsigned)i);
 }
 
-__device__ __forceinline__ double sm_a(const SmPar &p, float l) {
-    if ((double)l == p.M) return 0.0;
-    const double a = (p.M - (double)l) * p.inv_t;
-    return a < 1e30 ? a : 1e30;                  // also where it is none (0 times infinity)
+struct SmY {
+    float y, lo;                  // y + lo
+    int bin;                      // not falling with y
+};
+
+// Any l: what is -infinity or no number gets the last class, which weighs nothing.
+__device__ __forceinline__ SmY sm_y(const SmPar &p, float l) {
+    // M - l and its rounding error
+    const float d0 = p.M - l, bb = d0 - p.M, e0 = (p.M - (d0 - bb)) - (l + bb);
+    const bool top = l == p.M;                   // also inf - inf
+    const float d = top ? 0.0f : d0, e = top ? 0.0f : e0;
+    SmY r;
+    r.y = d * p.c;
+    r.lo = fmaf(e, p.c, fmaf(d, p.c_lo, fmaf(d, p.c, -r.y)));
+    r.bin = (int)fminf(r.y * p.scale, (float)(SM_BINS - 1));
+    return r;
 }
 
-__device__ __forceinline__ int sm_bin(const SmPar &p, double a) {
-    const double b = a * p.scale;
-    return b < (double)(SM_BINS - 1) ? (int)b : SM_BINS - 1;
+__device__ __forceinline__ bool sm_likely(const SmPar &p, const SmY &v) {
+    return (v.y - p.lim) + (v.lo - p.lim_lo) <= 0.0f;
 }
 
-__device__ __forceinline__ unsigned long long sm_weight(double a) {
-    if (!(a < 32.0)) return 0;
-    const double y = a * 1.4426950408889634074;
-    const int n = (int)(y + 0.5);
-    const float e = __builtin_amdgcn_exp2f((float)((double)n - y));      // 2^(-1/2) .. 2^(1/2)
-    return ((unsigned long long)(unsigned)(e * 16777216.0f) << 19) >> n;
+__device__ __forceinline__ unsigned long long sm_weight(const SmY &v) {
+    const float n = rintf(v.y);
+    const float e = __builtin_amdgcn_exp2f(-((v.y - n) + v.lo));         // 2^(-1/2) .. 2^(1/2)
+    const unsigned m = v.bin == SM_BINS - 1 ? 0u : (unsigned)(e * 16777216.0f);
+    return ((unsigned long long)m << 19) >> ((int)n & 63);
 }
 
 __device__ __forceinline__ SmPar sm_par(const qk_sample_args &a, const SmRow &w, int row, int nb) {
     __shared__ float smx, smn;
+    const float T = a.temperature ? a.temperature[row] : 1.0f, tp = a.top_p ? a.top_p[row] : 1.0f,
+                mp = a.min_p ? a.min_p[row] : 0.0f;
+    int k = a.top_k ? a.top_k[row] : 0;
     if (threadIdx.x < 64) {
         float mx = -INFINITY, mn = INFINITY;
         for (int i = threadIdx.x; i < nb; i += 64) {
@@ -114,40 +128,53 @@ __device__ __forceinline__ SmPar sm_par(const qk_sample_args &a, const SmRow &w,
     SmPar p;
     p.M = smx;
     p.none = smx == -INFINITY;
-    const float T = a.temperature ? a.temperature[row] : 1.0f;
     const bool greedy = !(T > 0.0f);
-    p.inv_t = greedy ? 1.0 : 1.0 / (double)T;
-    int k = a.top_k ? a.top_k[row] : 0;
+    const double c = fmin((greedy ? 1.0 : 1.0 / (double)T) * 1.4426950408889634074, 1e30);
+    p.c = (float)c;
+    p.c_lo = (float)(c - (double)p.c);
     if (greedy) k = 1;
     p.k = k <= 0 || k >= a.vocab ? 0 : k;
-    const float tp = a.top_p ? a.top_p[row] : 1.0f;
     p.top_p = tp != tp ? 1.0f : fmaxf(tp, 0.0f);
-    const float mp = a.min_p ? a.min_p[row] : 0.0f;
-    p.lim = mp > 0.0f ? -log((double)fminf(mp, 1.0f)) : 1e300;
-    double range = (p.M - (double)smn) * p.inv_t;
-    range = range < 32.0 ? range * (1.0 + 1e-9) : 32.0;       // also where it is none
-    p.scale = (double)(SM_BINS - 1) / fmax(range, 1e-300);
-    if (!(p.scale < 1e300)) p.scale = 1e300;
-    __syncthreads();                             // the shared pair may be written again
+    p.lim = INFINITY;
+    p.lim_lo = 0.0f;
+    if (mp > 0.0f) {
+        const double lim = -log2((double)fminf(mp, 1.0f));
+        p.lim = (float)lim;
+        p.lim_lo = (float)(lim - (double)p.lim);
+    }
+    const float range = (p.M - smn) * p.c * 1.000001f;       // the lowest entry is not in the last class
+    p.scale = fminf((float)(SM_BINS - 1) / (range < 46.166242f ? range : 46.166242f), 1e30f);
     return p;
 }
 
-// exclusive sum over the block of one value per thread, and the sum of all
-template <int NT, typename V>
-__device__ __forceinline__ V sm_scan(V v, V &total) {
-    constexpr int NW = NT / 64;
-    __shared__ V ws[NW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    V x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
+// inclusive sum over the wave: rows of 16 by shifts, then the rows' ends passed on
+__device__ __forceinline__ unsigned long long sm_wave_scan(unsigned long long v) {
+#define SM_STEP(CTRL, ROWS)                                                                                 \
+    {                                                                                                       \
+        const unsigned l = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, false);      \
+        const unsigned h = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, false); \
+        v += (unsigned long long)h << 32 | l;                                                               \
     }
+    SM_STEP(0x111, 0xF) SM_STEP(0x112, 0xF) SM_STEP(0x114, 0xF) SM_STEP(0x118, 0xF)      // row_shr 1, 2, 4, 8
+    SM_STEP(0x142, 0xA) SM_STEP(0x143, 0xC)                                              // row_bcast 15, 31
+#undef SM_STEP
+    return v;
+}
+
+// ... of the whole wave, in its last lane
+__device__ __forceinline__ unsigned long long sm_wave_sum(unsigned long long v) { return sm_wave_scan(v); }
+
+// exclusive sum over the block of one value per thread, and the sum of all
+template <int NT>
+__device__ __forceinline__ unsigned long long sm_scan(unsigned long long v, unsigned long long &total) {
+    constexpr int NW = NT / 64;
+    __shared__ unsigned long long ws[NW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned long long x = sm_wave_scan(v);
     __syncthreads();
     if (lane == 63) ws[wave] = x;
     __syncthreads();
-    V base = 0, all = 0;
+    unsigned long long base = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < NW; i++) {
         if (i < wave) base += ws[i];
@@ -155,12 +182,6 @@ __device__ __forceinline__ V sm_scan(V v, V &total) {
     }
     total = all;
     return base + x - v;
-}
-
-__device__ __forceinline__ unsigned long long sm_wave_sum(unsigned long long v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
 }
 
 __global__ __launch_bounds__(256) void sample_max(qk_sample_args a, int nb) {
@@ -172,7 +193,7 @@ __global__ __launch_bounds__(256) void sample_max(qk_sample_args a, int nb) {
         w.weight[i] = 0;
         w.count[i] = 0;
     }
-    if (b == 0 && threadIdx.x == 0) w.n_cand = w.slow = 0;
+    if (b == 0 && threadIdx.x == 0) w.n_cand = 0;
     float mx = -INFINITY, mn = INFINITY;
 #pragma unroll 8
     for (int i = b * 256 + threadIdx.x; i < a.vocab; i += nb * 256) {
@@ -194,34 +215,44 @@ __global__ __launch_bounds__(256) void sample_max(qk_sample_args a, int nb) {
     }
 }
 
-__global__ __launch_bounds__(256) void sample_hist(qk_sample_args a, int nb) {
-    const int row = blockIdx.x / nb, b = blockIdx.x % nb;
+// Blocks of 1024 threads: each adds its classes to the row's with one atomic a
+// class, so few large blocks.  The counts are left out without top-k, the weights
+// without top-p.
+__global__ __launch_bounds__(1024) void sample_hist(qk_sample_args a, int nb, int nh) {
+    const int row = blockIdx.x / nh, b = blockIdx.x % nh;
     SmRow &w = ((SmRow *)a.ws)[row];
-    const SmPar p = sm_par(a, w, row, nb);
-    if (p.none || (p.k == 0 && p.top_p >= 1.0f)) return;     // nothing asks for the order
     __shared__ unsigned long long hw[SM_BINS];
     __shared__ unsigned hc[SM_BINS];
-    for (int i = threadIdx.x; i < SM_BINS; i += 256) {
+    for (int i = threadIdx.x; i < SM_BINS; i += 1024) {
         hw[i] = 0;
         hc[i] = 0;
     }
-    __syncthreads();
+    const SmPar p = sm_par(a, w, row, nb);                   // its barrier orders the clearing, too
+    if (b == 0 && threadIdx.x == 0) w.par = p;
+    const bool counts = p.k > 0, weights = p.top_p < 1.0f;
+    if (p.none || !(counts || weights)) return;              // nothing asks for the order
     const float *x = a.logits + (size_t)row * a.row_stride;
-#pragma unroll 4
-    for (int i = b * 256 + threadIdx.x; i < a.vocab; i += nb * 256) {
-        const float l = sm_clean(x[i]);
-        if (l == -INFINITY) continue;
-        const double d = sm_a(p, l);
-        const int c = sm_bin(p, d);
-        atomicAdd(&hw[c], sm_weight(d));
-        atomicAdd(&hc[c], 1u);
+    constexpr int U = 4;
+    for (int i0 = b * 1024 + threadIdx.x; i0 < a.vocab; i0 += nh * 1024 * U) {
+        float l[U];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const long i = i0 + (long)j * nh * 1024;
+            l[j] = i < a.vocab ? x[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const SmY v = sm_y(p, l[j]);
+            if (v.bin == SM_BINS - 1) continue;
+            if (weights) atomicAdd(&hw[v.bin], sm_weight(v));
+            if (counts) atomicAdd(&hc[v.bin], 1u);
+        }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < SM_BINS; i += 256)
-        if (hc[i]) {
-            atomicAdd(&w.weight[i], hw[i]);
-            atomicAdd(&w.count[i], hc[i]);
-        }
+    for (int i = threadIdx.x; i < SM_BINS; i += 1024) {
+        if (hw[i]) atomicAdd(&w.weight[i], hw[i]);
+        if (hc[i]) atomicAdd(&w.count[i], hc[i]);
+    }
 }
 
 struct SmCut {
@@ -230,90 +261,107 @@ struct SmCut {
     unsigned long long weight_k, weight_lo, weight_all;
 };
 
-// which classes hold the thresholds (256 threads)
-__device__ SmCut sm_cut(const SmPar &p, const SmRow &w) {
-    constexpr int PER = SM_BINS / 256;
-    SmCut c = {SM_BINS, -1, -1, 0, 0, 0, 0};
-    if (p.k == 0 && p.top_p >= 1.0f) return c;
+// which classes hold the thresholds (256 threads; n, v: this thread's SM_PER classes)
+#define SM_PER (SM_BINS / 256)
+__device__ __forceinline__ SmCut sm_cut(const SmPar &p, const unsigned (&n)[SM_PER],
+                                        const unsigned long long (&v)[SM_PER]) {
     __shared__ SmCut sc;
-    __shared__ int s_lo, s_hi;
-    __shared__ unsigned long long s_end_k;
-    unsigned n[PER], nt = 0, n_all;
-    unsigned long long v[PER], vt = 0, v_all;
+    __shared__ unsigned long long s_end_k, ws[4][2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool by_k = p.k > 0, by_p = p.top_p < 1.0f;
+    unsigned nt = 0;
+    unsigned long long vt = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        n[i] = w.count[threadIdx.x * PER + i];
-        v[i] = w.weight[threadIdx.x * PER + i];
+    for (int i = 0; i < SM_PER; i++) {
         nt += n[i];
         vt += v[i];
     }
-    const unsigned n0 = sm_scan<256>(nt, n_all);
-    const unsigned long long v0 = sm_scan<256>(vt, v_all);
-    if (threadIdx.x == 0) {
-        sc = c;
-        sc.weight_all = v_all;
-        s_lo = s_hi = SM_BINS - 1;
+    const unsigned long long ns = sm_wave_scan(nt), vs = sm_wave_scan(vt);
+    if (lane == 63) {
+        ws[wave][0] = ns;
+        ws[wave][1] = vs;
     }
+    if (threadIdx.x == 0) sc = {SM_BINS, -1, -1, 0, 0, 0, 0};
     __syncthreads();
-    // top-k ends in class bk; the last class weighs nothing, so an end there is none
-    if (p.k > 0) {
-        unsigned at = n0;
-        unsigned long long vat = v0;
+    unsigned long long n0 = ns - nt, v0 = vs - vt, v_all = 0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int b = threadIdx.x * PER + i;
+    for (int i = 0; i < 4; i++) {
+        n0 += i < wave ? ws[i][0] : 0;
+        v0 += i < wave ? ws[i][1] : 0;
+        v_all += ws[i][1];
+    }
+    if (by_k) {
+        // top-k ends in class bk; the last class weighs nothing, so an end there is none
+        unsigned long long at = n0, vat = v0;
+#pragma unroll
+        for (int i = 0; i < SM_PER; i++) {
+            const int b = threadIdx.x * SM_PER + i;
             if (b < SM_BINS - 1 && at < (unsigned)p.k && at + n[i] >= (unsigned)p.k) {
                 sc.bk = b;
-                sc.count_k = at;
+                sc.count_k = (unsigned)at;
                 sc.weight_k = vat;
                 s_end_k = vat + v[i];
+                if (!by_p) {
+                    sc.lo = sc.hi = b;
+                    sc.weight_lo = vat;
+                }
             }
             at += n[i];
             vat += v[i];
         }
+        __syncthreads();
     }
-    __syncthreads();
-    const int bk = sc.bk;
-    if (p.top_p < 1.0f) {
+    if (by_p) {
         // the weight that top-p is a share of lies between these; so does its end
-        const double wl = bk >= 0 ? (double)sc.weight_k : (double)v_all, wh = bk >= 0 ? (double)s_end_k : (double)v_all;
+        const int bk = by_k ? sc.bk : -1;
+        const double wl = (double)(bk >= 0 ? sc.weight_k : v_all), wh = (double)(bk >= 0 ? s_end_k : v_all);
         const double tl = (double)p.top_p * wl, th = (double)p.top_p * wh;
         unsigned long long vat = v0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int b = threadIdx.x * PER + i;
+        for (int i = 0; i < SM_PER; i++) {
+            const int b = threadIdx.x * SM_PER + i;
             const double x0 = (double)vat, x1 = (double)(vat + v[i]);
-            if (x1 >= tl && (x0 < tl || b == 0)) s_lo = b;
-            if (x1 >= th && (x0 < th || b == 0)) s_hi = b;
+            if (x1 >= tl && (x0 < tl || b == 0)) {
+                sc.lo = b;
+                sc.weight_lo = vat;
+            }
+            if (x1 >= th && (x0 < th || b == 0)) sc.hi = b;
             vat += v[i];
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            sc.lo = s_lo;
-            sc.hi = s_hi;
-        }
-    } else if (threadIdx.x == 0) {
-        sc.lo = bk >= 0 ? bk : SM_BINS;
-        sc.hi = bk;
     }
-    __syncthreads();
-    const int lo = sc.lo;
-    unsigned long long vat = v0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        if (threadIdx.x * PER + i == lo) sc.weight_lo = vat;
-        vat += v[i];
-    }
-    __syncthreads();
-    return sc;
+    SmCut c = sc;
+    c.weight_all = v_all;
+    return c;
 }
 
 __global__ __launch_bounds__(256) void sample_pick(qk_sample_args a, int nb) {
     const int row = blockIdx.x / nb, b = blockIdx.x % nb, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     SmRow &w = ((SmRow *)a.ws)[row];
-    const SmPar p = sm_par(a, w, row, nb);
+    const float *x = a.logits + (size_t)row * a.row_stride;
+    const int subs = (a.vocab + SM_SUB - 1) / SM_SUB;
+    constexpr int PL = SM_SUB / 64;
+    float l[PL];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < PL; j++) {
+            const int i = s * SM_SUB + 64 * j + lane;
+            l[j] = i < a.vocab ? x[i] : -INFINITY;
+        }
+    };
+    // what does not wait for the thresholds: the first entries, the classes
+    int s = b * 4 + wave;
+    if (s < subs) load(s);
+    unsigned cn[SM_PER];
+    unsigned long long cw[SM_PER];
+#pragma unroll
+    for (int i = 0; i < SM_PER; i++) {
+        cn[i] = w.count[threadIdx.x * SM_PER + i];
+        cw[i] = w.weight[threadIdx.x * SM_PER + i];
+    }
+    const SmPar p = w.par;
     if (p.none) return;
-    const SmCut c = sm_cut(p, w);
+    const SmCut c = sm_cut(p, cn, cw);
     if (b == 0 && threadIdx.x == 0) {
         w.lo = c.lo;
         w.hi = c.hi;
@@ -323,27 +371,43 @@ __global__ __launch_bounds__(256) void sample_pick(qk_sample_args a, int nb) {
         w.weight_lo = c.weight_lo;
         w.weight_all = c.weight_all;
     }
-    const float *x = a.logits + (size_t)row * a.row_stride;
-    const int subs = (a.vocab + SM_SUB - 1) / SM_SUB;
-    for (int s = b * 4 + wave; s < subs; s += nb * 4) {
-        unsigned long long sum = 0;
-#pragma unroll 4
-        for (int j = 0; j < SM_SUB / 64; j++) {
-            const int i = s * SM_SUB + 64 * j + lane;
-            const float l = i < a.vocab ? sm_clean(x[i]) : -INFINITY;
-            if (l == -INFINITY) continue;
-            const double d = sm_a(p, l);
-            const int cl = sm_bin(p, d);
-            if (cl < c.lo) {
-                if (d <= p.lim) sum += sm_weight(d);
-            } else if (cl <= c.hi || cl == c.bk) {
-                const unsigned at = atomicAdd(&w.n_cand, 1u);
-                if (at < SM_CAND) w.cand[at] = (unsigned)i;
+    // the block's list, then one place in the row's for it all
+    __shared__ unsigned long long list[SM_CAND];
+    __shared__ unsigned n, at;
+    if (threadIdx.x == 0) n = 0;
+    __syncthreads();
+    auto entries = [&](auto min_p) {
+        for (; s < subs; s += nb * 4) {
+            float now[PL];
+#pragma unroll
+            for (int j = 0; j < PL; j++) now[j] = l[j];
+            if (s + nb * 4 < subs) load(s + nb * 4);
+            // With branches: an entry that is not kept costs no weight, which saves more
+            // than 16 unbroken chains overlap (64 rows of 151936: 20.3 us against 25.7).
+            unsigned long long sum = 0;
+#pragma unroll
+            for (int j = 0; j < PL; j++) {
+                const SmY v = sm_y(p, now[j]);
+                if (v.bin < c.lo) {
+                    if (!min_p() || sm_likely(p, v)) sum += sm_weight(v);
+                } else if (v.bin <= c.hi || v.bin == c.bk) {
+                    const unsigned i = atomicAdd(&n, 1u);
+                    if (i < SM_CAND)
+                        list[i] = (unsigned long long)__float_as_uint(now[j]) << 32 | (unsigned)(s * SM_SUB + 64 * j + lane);
+                }
             }
+            sum = sm_wave_sum(sum);
+            if (lane == 63) w.sub[s] = sum;
         }
-        sum = sm_wave_sum(sum);
-        if (lane == 0) w.sub[s] = sum;
-    }
+    };
+    if (p.lim < INFINITY) entries([] { return true; });
+    else entries([] { return false; });
+    __syncthreads();
+    if (n == 0) return;
+    if (threadIdx.x == 0) at = atomicAdd(&w.n_cand, n);
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < n && i < SM_CAND; i += 256)
+        if (at + i < SM_CAND) w.cand[at + i] = list[i];
 }
 
 // The entry at which a running sum over the order reaches `target`, by counting
@@ -371,7 +435,7 @@ __device__ unsigned long long sm_select(const SmPar &p, const float *x, int voca
             const unsigned long long cp = sm_comp(l, i);
             if (cp < least || (shift < 56 && (cp >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
             const int d = (int)(cp >> shift) & 255;
-            atomicAdd(&hw[d], sm_weight(sm_a(p, l)));
+            atomicAdd(&hw[d], sm_weight(sm_y(p, l)));
             atomicAdd(&hc[d], 1u);
         }
         __syncthreads();
@@ -403,114 +467,120 @@ __device__ unsigned long long sm_select(const SmPar &p, const float *x, int voca
         __syncthreads();
     }
     const int i = (int)(0xffffffffu - (unsigned)prefix);
-    upto = before + sm_weight(sm_a(p, sm_clean(x[i])));
+    upto = before + sm_weight(sm_y(p, sm_clean(x[i])));
     return prefix;
 }
 
-__global__ __launch_bounds__(1024) void sample_draw(qk_sample_args a, int nb) {
+__global__ __launch_bounds__(1024) void sample_draw(qk_sample_args a) {
     const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     SmRow &w = ((SmRow *)a.ws)[row];
-    const SmPar p = sm_par(a, w, row, nb);
+    // [0, n) in list order, padded; by rank; sums before each rank
+    __shared__ __attribute__((aligned(16))) unsigned long long comp[SM_CAND], before[SM_CAND + 1], sub[SM_MAX_SUBS];
+    __shared__ unsigned rank[SM_CAND];
+    __shared__ int found;
+    __shared__ unsigned long long base;
+    const int subs = (a.vocab + SM_SUB - 1) / SM_SUB;
+    const int lo = w.lo, hi = w.hi, bk = w.bk;
+    const unsigned n = w.n_cand;
+    const unsigned long long entry = t < (int)min(n, (unsigned)SM_CAND) ? w.cand[t] : 0;
+    const unsigned long long sub_t = t < subs ? w.sub[t] : 0;
+    float u = a.u[row];
+    const SmPar p = w.par;
     if (p.none) {
         if (t == 0) a.tokens[row] = -1;
         return;
     }
     const float *x = a.logits + (size_t)row * a.row_stride;
-    __shared__ unsigned long long comp[SM_CAND], wt[SM_CAND], sub[SM_MAX_SUBS];
-    __shared__ int found;
-    const int subs = (a.vocab + SM_SUB - 1) / SM_SUB;
-    const int lo = w.lo, hi = w.hi, bk = w.bk;
-    const unsigned n = w.n_cand;
     const bool slow = n > SM_CAND;               // block-uniform
     unsigned long long least = 0, all;
     unsigned long long mine = 0;                 // this thread's listed entry's weight, if it is kept
-    int index = -1;
-    if (!slow) {
-        sub[t] = t < subs ? w.sub[t] : 0;
-        float l = 0.0f;
-        double d = 0.0;
-        int cl = SM_BINS;
-        if (t < (int)n) {
-            index = (int)w.cand[t];
-            l = sm_clean(x[index]);
-            d = sm_a(p, l);
-            cl = sm_bin(p, d);
-            comp[t] = sm_comp(l, index);
-            wt[t] = sm_weight(d);
+    const int index = (int)(unsigned)entry;
+    sub[t] = sub_t;
+    if (!slow && n > 0) {
+        const float l = sm_clean(__uint_as_float((unsigned)(entry >> 32)));
+        const SmY v = sm_y(p, l);
+        const unsigned long long weight = sm_weight(v);
+        bool keep = t < (int)n;
+        // nothing real is 0: the padding is before nothing
+        comp[t] = keep ? sm_comp(l, index) : 0;
+        rank[t] = 0;
+        before[t] = 0;
+        __syncthreads();
+        // the rank of each: groups of waves compare it with a part of the list each
+        const int padded = (int)(n + 63) & ~63, parts = 1024 / padded, part = t / padded, i = t % padded;
+        if (part < parts) {
+            const unsigned long long me = comp[i];
+            const int len = (padded / 2 + parts - 1) / parts * 2, j0 = part * len, j1 = min(j0 + len, padded);
+            unsigned r = 0;
+#pragma unroll 4
+            for (int j = j0; j < j1; j += 2) {
+                const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&comp[j]);
+                r += (o.x > me) + (o.y > me);
+            }
+            if (r) atomicAdd(&rank[i], r);
         }
         __syncthreads();
-        unsigned before_n = 0;
-        unsigned long long before_w = 0;
-        if (t < (int)n) {
-            const unsigned long long me = comp[t];
-            for (unsigned j = 0; j < n; j++)
-                if (comp[j] > me) {
-                    before_n++;
-                    before_w += wt[j];
-                }
-        }
-        bool keep = t < (int)n;
+        const unsigned my = rank[t];
+        if (keep) before[my] = weight;
+        __syncthreads();
+        const unsigned long long sorted = before[t];
+        const unsigned long long ahead_w = sm_scan<1024>(sorted, all);
+        before[t] = ahead_w;
+        if (t == 0) before[SM_CAND] = all;
         unsigned long long whole = w.weight_all;
+        const unsigned ahead = (unsigned)__syncthreads_count(keep && v.bin < bk);    // listed entries of earlier classes
         if (bk >= 0) {
-            unsigned ahead;
-            (void)sm_scan<1024>((unsigned)(keep && cl < bk), ahead);     // listed entries of earlier classes
-            if (cl == bk) keep = keep && w.count_k + (before_n - ahead) < (unsigned)p.k;
-            unsigned long long in_k;
-            (void)sm_scan<1024>(keep && cl == bk ? wt[t] : 0ull, in_k);
-            whole = w.weight_k + in_k;
+            const unsigned left = (unsigned)p.k - w.count_k;         // entries that class bk gives to the top k
+            if (v.bin == bk) keep = keep && my - ahead < left;
+            whole = w.weight_k + (before[min(ahead + left, n)] - before[ahead]);
         }
         if (p.top_p < 1.0f) {
-            const unsigned long long before = w.weight_lo + before_w;
-            keep = keep && cl <= hi && ((double)before < (double)p.top_p * (double)whole || before == 0);
+            const unsigned long long sum = w.weight_lo + before[my];
+            keep = keep && v.bin <= hi && ((double)sum < (double)p.top_p * (double)whole || sum == 0);
         }
-        if (keep && d <= p.lim) {
-            mine = wt[t];
+        if (keep && sm_likely(p, v)) {
+            mine = weight;
             atomicAdd(&sub[index / SM_SUB], mine);
         }
         __syncthreads();
-    } else {
+    } else if (slow) {
         unsigned long long upto = 0;
         if (p.k > 0) least = sm_select(p, x, a.vocab, 0, false, (double)p.k, upto);
         if (p.top_p < 1.0f)
             least = sm_select(p, x, a.vocab, least, true, (double)p.top_p * (p.k > 0 ? (double)upto : (double)w.weight_all), upto);
-        for (int s = wave; s < SM_MAX_SUBS; s += 16) {
+        for (int s = wave; s < subs; s += 16) {
             unsigned long long sum = 0;
-            if (s < subs)
-                for (int j = 0; j < SM_SUB / 64; j++) {
-                    const int i = s * SM_SUB + 64 * j + lane;
-                    const float l = i < a.vocab ? sm_clean(x[i]) : -INFINITY;
-                    if (l == -INFINITY || sm_comp(l, i) < least) continue;
-                    const double d = sm_a(p, l);
-                    if (d <= p.lim) sum += sm_weight(d);
-                }
+            for (int j = 0; j < SM_SUB / 64; j++) {
+                const int i = s * SM_SUB + 64 * j + lane;
+                const float l = i < a.vocab ? sm_clean(x[i]) : -INFINITY;
+                if (l == -INFINITY || sm_comp(l, i) < least) continue;
+                const SmY v = sm_y(p, l);
+                if (sm_likely(p, v)) sum += sm_weight(v);
+            }
             sum = sm_wave_sum(sum);
-            if (lane == 0) sub[s] = sum;
+            if (lane == 63) sub[s] = sum;
         }
         __syncthreads();
     }
-    float u = a.u[row];
     u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
     // the 1024 entries, then the entry, at which the sum passes u times all of it
     const unsigned long long s0 = sm_scan<1024>(sub[t], all);
     const double target = (double)u * (double)all;
-    if ((double)s0 <= target && (double)(s0 + sub[t]) > target) found = t;
-    __syncthreads();
-    const int s = found;
-    __shared__ unsigned long long base;
-    if (t == s) base = s0;
-    __syncthreads();
+    if ((double)s0 <= target && (double)(s0 + sub[t]) > target) {
+        found = t;
+        base = s0;
+    }
     comp[t] = 0;
     __syncthreads();
+    const int s = found;
     if (mine && index / SM_SUB == s) comp[index % SM_SUB] = mine;
+    const int i = s * SM_SUB + t;
+    const float l = i < a.vocab ? sm_clean(x[i]) : -INFINITY;
     __syncthreads();
     unsigned long long v = comp[t];
-    const int i = s * SM_SUB + t;
-    if (i < a.vocab) {
-        const float l = sm_clean(x[i]);
-        if (l > -INFINITY) {
-            const double d = sm_a(p, l);
-            if (d <= p.lim && (slow ? sm_comp(l, i) >= least : sm_bin(p, d) < lo)) v = sm_weight(d);
-        }
+    if (l > -INFINITY) {
+        const SmY y = sm_y(p, l);
+        if ((slow ? sm_comp(l, i) >= least : y.bin < lo) && sm_likely(p, y)) v = sm_weight(y);
     }
     unsigned long long in_sub;
     const unsigned long long v0 = base + sm_scan<1024>(v, in_sub);
@@ -520,17 +590,20 @@ __global__ __launch_bounds__(1024) void sample_draw(qk_sample_args a, int nb) {
 extern "C" size_t qk_sample_ws_bytes(int rows, int vocab) { return (size_t)rows * sizeof(SmRow); }
 
 extern "C" int qk_sample_launch(const qk_sample_args *a, hipStream_t s) {
-    // four partial sums a block at least, and about 1024 blocks
+    // A wave of sample_pick takes a partial sum at a time and 4096 waves are there at
+    // once: as many turns as that takes, and blocks of four waves for so many turns.
     const int subs = (a->vocab + SM_SUB - 1) / SM_SUB;
-    int nb = (subs + 3) / 4;
-    const int most = a->rows >= 1024 ? 1 : 1024 / a->rows;
-    if (nb > most) nb = most;
+    const long turns = ((long)subs * a->rows + 4095) / 4096;
+    int nb = (int)((subs + 4 * turns - 1) / (4 * turns));
     if (nb > SM_MAX_BLOCKS) nb = SM_MAX_BLOCKS;
-    if ((long)a->rows * nb > 0x7fffffffL) return QWEN_HIP_EINVAL;
     const unsigned blocks = (unsigned)(a->rows * nb);
+    // 4096 entries a block at least, and about 512 blocks
+    int nh = (a->vocab + 4095) / 4096;
+    const int most_h = a->rows >= 512 ? 1 : 512 / a->rows;
+    if (nh > most_h) nh = most_h;
     sample_max<<<blocks, 256, 0, s>>>(*a, nb);
-    sample_hist<<<blocks, 256, 0, s>>>(*a, nb);
+    sample_hist<<<(unsigned)(a->rows * nh), 1024, 0, s>>>(*a, nb, nh);
     sample_pick<<<blocks, 256, 0, s>>>(*a, nb);
-    sample_draw<<<a->rows, 1024, 0, s>>>(*a, nb);
+    sample_draw<<<a->rows, 1024, 0, s>>>(*a);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }
