@@ -28,9 +28,8 @@
 //                    of step j is key 16 j + 8 (i / 4) + 4 hl + i % 4; A = V^T read
 //                    from the row-major V tile by transposing LDS reads (16
 //                    lanes take 4 keys x 16 dims and get 4 keys of one dim each).
-// LDS rows are 256 bytes, 16-byte chunk c of row r in slot c ^ 2 (r & 7): eight
-// rows of a fragment read, and the four rows of a transposing read, meet
-// different banks.
+// LDS rows are 256 bytes, their 16-byte chunks in an order by row (swz) that
+// keeps both kinds of reads free of bank conflicts.
 //
 // bf16 pages go straight to LDS (two buffers); fp32 pages pass through
 // registers, split on the way (one buffer a block, two blocks a CU).
@@ -39,17 +38,18 @@
 // partials paged_merge joins.
 //
 // Masked keys: a masked score is -inf before the maximum, but 0 times what the
-// cache holds is no number where that is infinite or none.  Rows past the split's
-// keys or without a page are read as zeros.  A V row that some rows of a tile see
-// and others do not shows in the sums, which stay no number once they are: a
-// block that ends with one runs again with every V element looked at, the ones
-// that are not finite counted per row that sees them (nothing for the others).
+// cache holds is no number where that is infinite or none.  Such a V
+// element shows in the sums, which stay no number once they are: a block that
+// ends with one runs again with every V element looked at, the ones that are not
+// finite counted per row that sees them (nothing for the others).
 #include "paged.h"
+#include "ring.h"
+
+#include <limits.h>
 
 typedef float pp_f32x16 __attribute__((ext_vector_type(16)));
 typedef short pp_i16x4 __attribute__((ext_vector_type(4)));
 
-#define PP_ROWS 128               // flattened rows per block
 #define PP_KT 32                  // keys per tile
 #define PP_PLANE (PP_KT * 256)    // bytes of one term of a K or V tile
 
@@ -57,11 +57,21 @@ __device__ __forceinline__ pp_f32x16 pp_mfma(bf16x8 a, bf16x8 b, pp_f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// what a masked or missing key's row is read from
-__device__ __attribute__((aligned(256))) unsigned pp_zero_row[PG_HD];
-
-__device__ __forceinline__ void pp_lds_load16(const unsigned char *g, unsigned char *l0) {
-    __builtin_amdgcn_global_load_lds(g, l0, 16, 0, 0);
+// 16 bytes a lane from global memory straight into LDS (lane l at byte 16 l of the
+// 1 KB at l0): base + off, base the same for the wave.  Written out because the
+// compiler lets every transposing LDS read wait for all such loads on their way,
+// also those to the other buffer; the walk's barriers wait for them instead.
+// They write no register but m0, which the compiler sets anew before each use, and
+// its own counts of loads only become stricter by ones that it does not see.
+__device__ __forceinline__ void pp_lds_load16(const unsigned char *base, unsigned off, unsigned char *l0) {
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)l0;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(off), "s"(base), "s"(at) : "memory");
+}
+// ... from an address of each lane's own
+__device__ __forceinline__ void pp_lds_load16(const unsigned char *p, unsigned char *l0) {
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)l0;
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p), "s"(at) : "memory");
 }
 
 // the three terms of two values, each pair in one word (a low)
@@ -90,29 +100,46 @@ __device__ __forceinline__ void pp_terms8(const float *x, bf16x8 (&t)[NT]) {
     }
 }
 
-// c += sum of the term pairs (i, j), i + j <= 2, small ones first
+// The term pairs (i, j), i + j <= 2, of a product of NA by NB terms, small ones first
+template <int NA, int NB>
+struct PpPairs {
+    static constexpr int N = NA * NB == 9 ? 6 : NA * NB;
+    struct List {
+        int a[N], b[N];
+    };
+    static constexpr List make() {
+        List l = {};
+        int n = 0;
+        for (int sum = 2; sum >= 0; sum--)
+            for (int i = NA - 1; i >= 0; i--)
+                for (int j = NB - 1; j >= 0; j--)
+                    if (i + j == sum) {
+                        l.a[n] = i;
+                        l.b[n++] = j;
+                    }
+        return l;
+    }
+};
+
 template <int NA, int NB>
 __device__ __forceinline__ pp_f32x16 pp_products(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], pp_f32x16 c) {
+    constexpr auto L = PpPairs<NA, NB>::make();
 #pragma unroll
-    for (int sum = (NA == 3 || NB == 3) ? 2 : 0; sum >= 0; sum--)
-#pragma unroll
-        for (int i = NA - 1; i >= 0; i--)
-#pragma unroll
-            for (int j = NB - 1; j >= 0; j--)
-                if (i + j == sum) c = pp_mfma(a[i], b[j], c);
+    for (int n = 0; n < PpPairs<NA, NB>::N; n++) c = pp_mfma(a[L.a[n]], b[L.b[n]], c);
     return c;
 }
 
 // 8 elements of V^T (dims by lane, the lane's 8 keys of step j): two transposing reads
-__device__ __forceinline__ bf16x8 pp_vfrag(const unsigned char *p) {
+__device__ __forceinline__ bf16x8 pp_vfrag(const unsigned char *p, const unsigned char *p8) {
     typedef __attribute__((address_space(3))) pp_i16x4 *lds_p;
     const pp_i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p);
-    const pp_i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 8 * 256));
+    const pp_i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p8);
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // The lanes' words with every element that is infinite or no number replaced by
-// 0; cls gets 1, 64 or 4096 in the places of +inf, -inf and no number.
+// 0 (lower terms of an infinite value are none); cls gets 1, 64 or 4096 in the
+// places of +inf, -inf and no number.
 __device__ __forceinline__ bf16x8 pp_finite(bf16x8 v, bf16x8 &cls) {
     uint4 w = __builtin_bit_cast(uint4, v), k = make_uint4(0u, 0u, 0u, 0u);
     uint32_t *pw = &w.x, *pk = &k.x;
@@ -130,332 +157,579 @@ __device__ __forceinline__ bf16x8 pp_finite(bf16x8 v, bf16x8 &cls) {
     return __builtin_bit_cast(bf16x8, w);
 }
 
+template <bool B>
+struct PpBool {
+    static constexpr bool value = B;
+};
+
 template <typename T>
 struct PpTerms {
     static constexpr int N = sizeof(T) == 4 ? 3 : 1;
 };
 
+// RB blocks of 32 rows a wave, WR waves over the rows, KG groups of such waves over the
+// keys (tiles in turn, joined in LDS).
 template <typename T, typename C>
-__global__ __launch_bounds__(256, PpTerms<T>::N == 3 ? 1 : 2) void paged_prefill(qk_paged_attn_args a) {
+struct PpShape {
+    static constexpr int RB = 1, WR = 4 / RB, KG = 2;
+    static constexpr int ROWS = 32 * RB * WR, THREADS = 64 * WR * KG, OCC = 1;
+};
+
+// The tile of block `b`: sequence and first flattened row (a whole wave asks).  Longest
+// first over up to 64 sequences: a tile's level is its last position in steps of 128 keys,
+// and tiles go out by falling level, so the ones that take longest start first (8 prompts
+// of 101 .. 1515 rows: see the table of measurements below).  For more sequences, by
+// sequence from the last: tiles of sequence s take the slots from start_s G / ROWS + s on
+// (ceil(n G / ROWS) of them never pass the next sequence's first).
+template <int ROWS>
+__device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int slots, int &s, int &f0) {
+    const int lane = threadIdx.x & 63;
+    auto begin = [&](int i) { return min(max(pg.row_start[i], 0), pg.rows); };
+    if (pg.n_seqs > 64) {
+        const int slot = slots - 1 - b;
+        auto first_slot = [&](int i) { return begin(i) * G / ROWS + i; };
+        s = __builtin_amdgcn_readfirstlane(pg_search<64>(pg.n_seqs, slot, first_slot));
+        if (s < 0) return false;
+        f0 = (slot - first_slot(s)) * ROWS;
+        return f0 >= 0;
+    }
+    if (pg.n_seqs == 1) {
+        s = 0;
+        f0 = ((max(begin(1) - begin(0), 0) * G + ROWS - 1) / ROWS - 1 - b) * ROWS;
+        return f0 >= 0;
+    }
+    const bool on = lane < pg.n_seqs;
+    const int n = on ? max(begin(lane + 1) - begin(lane), 0) : 0;
+    const int tiles = (n * G + ROWS - 1) / ROWS, off = on ? min(max(pg_len(pg, lane) - n, 0), pg.capacity) : 0;
+    // tiles of this lane's sequence at level t or above; counts fit a float exactly
+    auto first_at = [&](int t) {
+        const long want = ((long)t * 128 - off) * G;
+        return (int)min(max((want + ROWS - 1) / ROWS - 1, 0L), (long)tiles);
+    };
+    auto sum_at = [&](int t) { return (int)wave_sum((float)(tiles - first_at(t))); };
+    if (b >= sum_at(0)) return false;
+    int lo = 0, hi = (int)wave_max(on && n > 0 ? (float)((off + n + ROWS) / 128 + 2) : 0.0f);
+    while (hi - lo > 1) {                        // sum_at(lo) > b >= sum_at(hi)
+        const int mid = (lo + hi) >> 1;
+        if (sum_at(mid) > b) lo = mid;
+        else hi = mid;
+    }
+    const int left = b - sum_at(lo + 1), from = first_at(lo), mine = first_at(lo + 1) - from;
+    int upto = mine;                             // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += o;
+    }
+    const unsigned long long past = __ballot(upto > left);
+    s = __builtin_amdgcn_readfirstlane(past ? __builtin_ctzll(past) : 0);
+    const int tile = from + left - (upto - mine);
+    f0 = __builtin_amdgcn_readfirstlane(__shfl(tile, s, 64)) * ROWS;
+    return past != 0 && f0 >= 0;
+}
+
+// SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions)
+template <typename T, typename C, bool SMALL>
+__global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) void paged_prefill(qk_paged_attn_args a,
+                                                                                                int slots) {
     constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N;
+    constexpr int RB = PpShape<T, C>::RB, WR = PpShape<T, C>::WR, KG = PpShape<T, C>::KG, ROWS = PpShape<T, C>::ROWS;
     constexpr bool DIRECT = NK == 1;
     constexpr int NBUF = DIRECT ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[NBUF][2][NK][PP_PLANE];
-    __shared__ __attribute__((aligned(4))) unsigned char seen_lds[NBUF][4];   // keys of a tile that are there, a bit each
+    constexpr int STAGE = 2 * NK * PP_PLANE;              // bytes of one K and V tile
+    constexpr int JOIN = (KG - 1) * WR * RB * (16384 + 512);
+    constexpr int BYTES = KG * NBUF * STAGE > JOIN ? KG * NBUF * STAGE : JOIN;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds_all[BYTES];
 
     const qk_paged &pg = a.pg;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = wid % WR, kg = wid / WR;
     const int ql = lane & 31, hl = lane >> 5;
-    const int G = a.heads / pg.kv_heads;
-    const int slots = pg.rows * G / PP_ROWS + pg.n_seqs;      // rows * heads fits an int
-    const int slot = slots - 1 - (int)(blockIdx.x / pg.kv_heads), kvh = blockIdx.x % pg.kv_heads;
-    // Tiles of sequence s take the slots from start_s G / 128 + s on: ceil(n G / 128)
-    // never passes the next sequence's first.
-    auto begin = [&](int s) { return min(max(pg.row_start[s], 0), pg.rows); };
-    auto first_slot = [&](int s) { return begin(s) * G / PP_ROWS + s; };
-    const int s = __builtin_amdgcn_readfirstlane(pg_search<64>(pg.n_seqs, slot, first_slot));
-    if (s < 0) return;
-    const int r0 = begin(s), n = max(begin(s + 1) - r0, 0);
-    const int f0 = (slot - first_slot(s)) * PP_ROWS, frows = n * G;
-    if (f0 >= frows) return;                              // block-uniform, as all above
+    const int G = a.heads / pg.kv_heads, kvh = blockIdx.x % pg.kv_heads;
+    int s, f0;
+    if (!pp_tile<ROWS>(pg, G, (int)(blockIdx.x / pg.kv_heads), slots, s, f0)) return;     // block-uniform, as the next
+    const int r0 = min(max(pg.row_start[s], 0), pg.rows), n = max(min(max(pg.row_start[s + 1], 0), pg.rows) - r0, 0);
+    const int frows = n * G;
+    if (f0 >= frows) return;
     const int len = pg_len(pg, s);
-    const int off0 = len - n;                      // position of the sequence's first new row (< 0: sees nothing)
-    const int lastf = min(f0 + PP_ROWS, frows) - 1;
+    const int off0 = len - n;                             // position of the sequence's first new row (< 0: sees nothing)
+    const int lastf = min(f0 + ROWS, frows) - 1;
     const int kend = min(max(off0 + lastf / G + 1, 0), pg.capacity);
     const int need = (int)(((long)kend + a.nsplit - 1) / a.nsplit);
     const int chunk = max(a.chunk, (need + PP_KT - 1) / PP_KT * PP_KT), split = blockIdx.y;
     const int k0s = (int)min((long)split * chunk, (long)kend), k1 = (int)min((long)k0s + chunk, (long)kend);
 
-    // this lane's row
-    const int f = f0 + 32 * wave + ql;
-    const bool on = f < frows;
-    const int qi = on ? f / G : 0, head = kvh * G + (on ? f % G : 0);
-    const size_t orow = (size_t)(r0 + qi) * a.heads + head;
-    const int pos = on ? off0 + qi : -1;
+    // this lane's rows
+    int head[RB], qrow[RB], pos[RB];
+    bool on[RB];
+#pragma unroll
+    for (int x = 0; x < RB; x++) {
+        const int f = f0 + 32 * (RB * wave + x) + ql;
+        on[x] = f < frows;
+        const int qi = on[x] ? f / G : 0;
+        head[x] = kvh * G + (on[x] ? f % G : 0);
+        qrow[x] = r0 + qi;
+        pos[x] = on[x] ? off0 + qi : -1;
+    }
+    auto orow = [&](int x) { return (size_t)qrow[x] * a.heads + head[x]; };
     if (k0s >= k1 && a.nsplit > 1) {
-        if (on && hl == 0) {
-            float *ml = a.part_ml + 2 * (orow * a.nsplit + split);
-            ml[0] = -INFINITY;
-            ml[1] = 0.0f;
-        }
+#pragma unroll
+        for (int x = 0; x < RB; x++)
+            if (on[x] && hl == 0 && kg == 0) {
+                float *ml = a.part_ml + 2 * (orow(x) * a.nsplit + split);
+                ml[0] = -INFINITY;
+                ml[1] = 0.0f;
+            }
         return;
     }
     // the wave's first and last positions (rows do not fall with f)
-    const int fw = f0 + 32 * wave;
+    const int fw = f0 + 32 * RB * wave;
     const bool wave_on = fw < frows;
-    const int pos_lo = off0 + fw / G, pos_hi = off0 + min(fw + 31, frows - 1) / G;
+    const int pos_lo = off0 + fw / G, pos_hi = off0 + min(fw + 32 * RB - 1, frows - 1) / G;
 
-    // queries: dims 16 t + 8 hl .. + 7; fp32 ones take the scale along
-    bf16x8 q[8][NQ];
-#pragma unroll
-    for (int t = 0; t < 8; t++) {
-        const T *qp = (const T *)a.q + orow * PG_HD + 16 * t + 8 * hl;
-        if constexpr (NQ == 1) {
-            q[t][0] = *reinterpret_cast<const bf16x8 *>(qp);
-        } else {
-            const float4 x0 = pg_load4(qp), x1 = pg_load4(qp + 4);
-            const float fs = a.scale * PG_LOG2E;
-            const float x[8] = {x0.x * fs, x0.y * fs, x0.z * fs, x0.w * fs, x1.x * fs, x1.y * fs, x1.z * fs, x1.w * fs};
-            pp_terms8<NQ>(x, q[t]);
-        }
-    }
+    bf16x8 q[RB][8][NQ];
     const float sc = NQ == 1 ? a.scale * PG_LOG2E : 1.0f;
+    pp_f32x16 o[RB][4];
+    float m[RB], l[RB];
 
-    pp_f32x16 o[4];
-    float m, l;
-
-    // ---- staging: the wave's 8 rows of a tile; a lane's rows RPL of them -------------
-    constexpr int RPL = DIRECT ? 2 : 4;
-    const int srow0 = DIRECT ? lane >> 4 : lane >> 5;     // row 8 wave + RSTEP i + srow0
-    constexpr int RSTEP = DIRECT ? 4 : 2;
-    int pid[RPL];
-    auto ids = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < RPL; i++) {
-            const int key = k0 + 8 * wave + RSTEP * i + srow0;
-            pid[i] = key < k1 ? pg_page(pg, s, key) : -1;
-        }
+    // ---- staging: the group's waves take SROWS rows of its tile each; a lane's rows RPL of them ----
+    constexpr int SROWS = PP_KT / WR, RSTEP = DIRECT ? 4 : 2, RPL = SROWS / RSTEP;
+    constexpr int ROWB = PG_HD * sizeof(C);
+    const int srow0 = DIRECT ? lane >> 4 : lane >> 5;     // row SROWS wave + RSTEP i + srow0
+    unsigned char *const lds = lds_all + kg * NBUF * STAGE;
+    auto plane = [&](int buf, int v, int t) { return lds + buf * STAGE + (v * NK + t) * PP_PLANE; };
+    // The slot of row r's chunk 0: 16 rows of a K fragment read meet the 16 16-byte slots of
+    // the banks' 256 bytes, and so do the 64-byte pieces of four rows of a transposing read.
+    auto swz = [](int r) { return 4 * (r & 3) + ((r >> 2) & 3); };
+    const int smask = (1 << pg.page_shift) - 1;
+    const int *const table = pg.table + (size_t)s * pg.table_stride;
+    auto tile_k0 = [&](int t) { return k0s + PP_KT * (KG * t + kg); };
+    // Where the wave's rows of tile t lie.  Pages of at least SROWS positions hold them in one page
+    // (the tiles start at multiples of 32): one offset from the pages' start, without vector
+    // arithmetic.  Rows past the split's end are read at its last key (any row does: their scores
+    // are masked), rows without a page from the first page's start.
+    const size_t pstride = ((size_t)pg.kv_heads << pg.page_shift) * ROWB;
+    const unsigned char *const pages[2] = {(const unsigned char *)pg.k + ((size_t)kvh << pg.page_shift) * ROWB,
+                                           (const unsigned char *)pg.v + ((size_t)kvh << pg.page_shift) * ROWB};
+    auto locate = [&](int t, int i0) {
+        const int at = min(tile_k0(t) + SROWS * wave, k1 - 1);
+        return ((unsigned)i0 < (unsigned)pg.n_pages ? i0 : 0) * pstride + (unsigned)(at & smask) * ROWB;
     };
-    auto seen_byte = [&]() {
-        unsigned b = 0;
-#pragma unroll
-        for (int i = 0; i < RPL; i++) {
-            const unsigned long long v = __ballot(pid[i] >= 0);
-#pragma unroll
-            for (int j = 0; j < RSTEP; j++) b |= (unsigned)(v >> (64 / RSTEP * j) & 1) << (RSTEP * i + j);
-        }
-        return b;
+    // Page ids come 64 tiles at a time, a lane each: one that was loaded every turn would be
+    // waited for behind the tiles' loads.  Where that does not do (smaller pages; a page missing
+    // in the split's range, so that a tile's keys have to be asked one by one) every tile asks
+    // for its 32 keys' pages and waits.
+    int missing = 0;
+    for (int p = (k0s >> pg.page_shift) + (int)threadIdx.x; p <= (k1 - 1) >> pg.page_shift; p += PpShape<T, C>::THREADS)
+        missing |= (unsigned)table[p] >= (unsigned)pg.n_pages;
+    const bool fast = !__syncthreads_or(missing) && !SMALL;
+    int idv = 0, idv_at = INT_MIN / 2;                    // pages of tiles idv_at + lane
+    struct Where {
+        size_t off;
+        int id;                                           // of key lane % 32, where the tile asked for them
+        unsigned seen;                                    // keys that are there, a bit each
     };
-    float4 stk[DIRECT ? 1 : 4], stv[DIRECT ? 1 : 4];
-    unsigned st_seen = 0;
-    // bf16: K and V rows to buffer buf; fp32: to registers
-    auto fetch = [&](int k0, int buf) {
-#pragma unroll
-        for (int i = 0; i < RPL; i++) {
-            const int r = 8 * wave + RSTEP * i + srow0;
-            const size_t off = pid[i] >= 0 ? pg_offset(pg, pid[i], kvh, k0 + r) : 0;
-            if constexpr (DIRECT) {
-                const int byte = 16 * ((lane & 15) ^ (2 * (r & 7)));
-                const unsigned char *z = (const unsigned char *)pp_zero_row;
-                const unsigned char *kr = pid[i] >= 0 ? (const unsigned char *)((const C *)pg.k + off) : z;
-                const unsigned char *vr = pid[i] >= 0 ? (const unsigned char *)((const C *)pg.v + off) : z;
-                pp_lds_load16(kr + byte, &lds[buf][0][0][256 * (8 * wave + RSTEP * i)]);
-                pp_lds_load16(vr + byte, &lds[buf][1][0][256 * (8 * wave + RSTEP * i)]);
-            } else {
-                const float *kr = pid[i] >= 0 ? (const float *)pg.k + off : (const float *)pp_zero_row;
-                const float *vr = pid[i] >= 0 ? (const float *)pg.v + off : (const float *)pp_zero_row;
-                stk[i] = pg_load4(kr + 4 * ql);
-                stv[i] = pg_load4(vr + 4 * ql);
+    auto where = [&](int t) {
+        Where w;
+        const int left = k1 - tile_k0(t);
+        w.seen = left >= PP_KT ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+        if (fast) {
+            if (t - idv_at >= 64) {
+                idv_at = t;
+                idv = table[min(min(tile_k0(0), k1 - 1) + (long)KG * PP_KT * (t + lane) + SROWS * wave, (long)k1 - 1) >> pg.page_shift];
             }
-        }
-        const unsigned b = seen_byte();
-        if constexpr (DIRECT) {
-            if (lane == 0) seen_lds[buf][wave] = (unsigned char)b;
+            w.id = 0;
+            w.off = locate(t, __builtin_amdgcn_readlane(idv, t - idv_at));
         } else {
-            st_seen = b;
+            w.id = table[min(tile_k0(t) + ql, k1 - 1) >> pg.page_shift];
+            w.seen &= (unsigned)__ballot((unsigned)w.id < (unsigned)pg.n_pages);
+            w.off = locate(t, __builtin_amdgcn_readlane(w.id, SROWS * wave));
         }
+        return w;
     };
-    // fp32: the terms of the staged rows to LDS
-    auto put = [&]() {
-        if constexpr (!DIRECT) {
-#pragma unroll
-            for (int i = 0; i < RPL; i++) {
-                const int r = 8 * wave + RSTEP * i + srow0;
-                const int at = 256 * r + 16 * ((ql >> 1) ^ (2 * (r & 7))) + 8 * (ql & 1);
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const float4 v = x ? stv[i] : stk[i];
-                    uint32_t w0[3], w1[3];
-                    pp_split2(v.x, v.y, w0);
-                    pp_split2(v.z, v.w, w1);
-                    // the terms below an infinite one (or none) are 0, not inf - inf
-                    const float z = fmaf(v.x, 0.0f, fmaf(v.y, 0.0f, fmaf(v.z, 0.0f, v.w * 0.0f)));
-                    if (z != 0.0f) {
-                        auto fix = [](uint32_t hw, uint32_t w) {
-                            const uint32_t lo = (hw & 0x7f80u) == 0x7f80u ? 0u : 0xffffu;
-                            const uint32_t hi = (hw & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
-                            return w & (lo | hi);
-                        };
-#pragma unroll
-                        for (int t = 1; t < 3; t++) {
-                            w0[t] = fix(w0[0], w0[t]);
-                            w1[t] = fix(w1[0], w1[t]);
-                        }
-                    }
-#pragma unroll
-                    for (int t = 0; t < 3; t++)
-                        *reinterpret_cast<uint2 *>(&lds[0][x][t][at]) = make_uint2(w0[t], w1[t]);
-                }
-            }
-            if (lane == 0) seen_lds[0][wave] = (unsigned char)st_seen;
-        }
-    };
-
-    // ---- fragment addresses ----------------------------------------------------------
-    const int ksw = 2 * (ql & 7);                         // K row ql: chunk 2 t + hl in slot (2 t + hl) ^ ksw
-    const int vrow = 4 * hl + ((lane & 15) >> 2);         // V row of this lane's transposing reads (mod 8)
-    const int vchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vbyte = 256 * vrow + 8 * (lane & 1);
-    auto vaddr = [&](int buf, int t, int d, int j) {
-        return &lds[buf][1][t][vbyte + 16 * ((4 * d + vchunk) ^ (2 * (vrow & 7))) + 16 * 256 * j];
-    };
-
-    bool guarded = false;
-    for (;;) {
-#pragma unroll
-    for (int d = 0; d < 4; d++) o[d] = (pp_f32x16){};
-    m = -INFINITY;
-    l = 0.0f;
-    ids(k0s);
-    fetch(k0s, 0);
-    ids(k0s + PP_KT);
-    int buf = 0;
-    for (int k0 = k0s; k0 < k1; k0 += PP_KT) {
-        if constexpr (DIRECT) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);           // this wave's rows are in LDS
-            __syncthreads();                              // everyone's are, and the other buffer is read
-            if (k0 + PP_KT < k1) {
-                fetch(k0 + PP_KT, buf ^ 1);
-                ids(k0 + 2 * PP_KT);
-            }
+    // this lane's row i of tile t at its wave's offset: of_wave(base, bytes); or at its own
+    auto row_of = [&](int t, const Where &w, int v, int i, auto of_wave, auto of_lane) {
+        const int key0 = tile_k0(t) + SROWS * wave, r = RSTEP * i + srow0;
+        if constexpr (!SMALL) {
+            of_wave(pages[v] + w.off, (unsigned)min(r, max(k1 - 1 - key0, 0)) * ROWB);
         } else {
-            __syncthreads();                              // the last tile is read
-            put();
-            __syncthreads();
-            if (k0 + PP_KT < k1) {
-                fetch(k0 + PP_KT, 0);
-                ids(k0 + 2 * PP_KT);
+            const int at = min(key0 + r, k1 - 1), i1 = __shfl(w.id, SROWS * wave + r, 64);
+            of_lane(pages[v] + ((unsigned)i1 < (unsigned)pg.n_pages ? i1 : 0) * pstride + (unsigned)(at & smask) * ROWB);
+        }
+    };
+    // bf16: straight to the K (v 0) or V (v 1) rows of buffer buf
+    auto fetch_row = [&](int t, const Where &w, int v, int buf, int i) {
+        const unsigned chunk = 16u * ((lane & 15) ^ swz(SROWS * wave + RSTEP * i + srow0));
+        unsigned char *const to = plane(buf, v, 0) + 256 * (SROWS * wave + RSTEP * i);
+        row_of(t, w, v, i, [&](const unsigned char *p, unsigned at) { pp_lds_load16(p, at + chunk, to); },
+               [&](const unsigned char *row) { pp_lds_load16(row + chunk, to); });
+    };
+    auto fetch = [&](int t, const Where &w, int v, int buf) {
+#pragma unroll
+        for (int i = 0; i < RPL; i++) fetch_row(t, w, v, buf, i);
+    };
+    // fp32: to registers, and from there split into terms
+    auto load = [&](int t, const Where &w, int v, float4 (&st)[RPL]) {
+#pragma unroll
+        for (int i = 0; i < RPL; i++)
+            row_of(t, w, v, i,
+                   [&](const unsigned char *p, unsigned at) { st[i] = pg_load4((const float *)(p + (at + 16 * ql))); },
+                   [&](const unsigned char *row) { st[i] = pg_load4((const float *)(row + 16 * ql)); });
+    };
+    auto put = [&](int v, const float4 (&st)[RPL]) {
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            const int r = SROWS * wave + RSTEP * i + srow0;
+            const int at = 256 * r + 16 * ((ql >> 1) ^ swz(r)) + 8 * (ql & 1);
+            uint32_t w0[3], w1[3];
+            pp_split2(st[i].x, st[i].y, w0);
+            pp_split2(st[i].z, st[i].w, w1);
+            // terms below an infinite one come out as none: see pp_finite
+#pragma unroll
+            for (int t = 0; t < NK; t++) *reinterpret_cast<uint2 *>(plane(0, v, t) + at) = make_uint2(w0[t], w1[t]);
+        }
+    };
+
+    // ---- fragment addresses: what depends on the lane once, the rest as bits over it ----
+    const unsigned klane = 256 * ql + 16 * (hl ^ swz(ql));            // K row ql, chunk 2 t + hl: ^ 32 t
+    // V^T rows 32 d + 16 (lane / 16 % 2) + lane % 16, keys 16 j + 4 hl .. + 3 and + 8: the rows that
+    // this lane addresses, chunk 4 d + ..: ^ 64 d
+    const int vrow = 4 * hl + ((lane & 15) >> 2), vchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const unsigned vlane = 256 * vrow + 8 * (lane & 1) + 16 * (vchunk ^ swz(vrow)),
+                   vlane8 = 256 * (vrow + 8) + 8 * (lane & 1) + 16 * (vchunk ^ swz(vrow + 8));
+    auto kfrag = [&](int buf, int y, int t) {
+        return *reinterpret_cast<const bf16x8 *>(plane(buf, 0, y) + (klane ^ (32 * t)));
+    };
+    auto vfrag = [&](int buf, int y, int d, int j) {
+        const unsigned char *p = plane(buf, 1, y) + 16 * 256 * j;
+        return pp_vfrag(p + (vlane ^ (64 * d)), p + (vlane8 ^ (64 * d)));
+    };
+
+    // Barriers by hand: behind __syncthreads() the compiler has every LDS read wait for loads
+    // that are still on their way to LDS.  `landed`: this wave's are there but for the last turn's
+    // 2 RPL.
+    auto barrier = [&](bool landed) {
+        if (landed) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * RPL));
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    const int nt = (k1 - k0s + KG * PP_KT - 1) / (KG * PP_KT);       // tiles of a group
+    pp_f32x16 st[RB];
+    bf16x8 pt[RB][2][NQ];
+    [[maybe_unused]] bf16x8 one[RB][2];
+
+    // S^T of the tile in K buffer buf
+    auto scores = [&](int buf) {
+#pragma unroll
+        for (int x = 0; x < RB; x++) st[x] = (pp_f32x16){};
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            bf16x8 kf[NK];
+#pragma unroll
+            for (int y = 0; y < NK; y++) kf[y] = kfrag(buf, y, t);
+#pragma unroll
+            for (int x = 0; x < RB; x++) st[x] = pp_products<NK, NQ>(kf, q[x][t], st[x]);
+        }
+    };
+    // The matrix part of a turn: V of one tile and K of the next, product by product in turn (the
+    // scores are one chain of sums), fragments read AHEAD steps before their products.
+    auto matrix = [&](int vbuf, int kbuf) {
+        constexpr int PAIRS = PpPairs<NK, NQ>::N, AHEAD = PAIRS == 1 ? 3 : 1, RING = AHEAD + 1;
+        constexpr auto L = PpPairs<NK, NQ>::make();
+        bf16x8 kf[RING][NK], vf[RING][NK];
+        auto read = [&](int u) {
+#pragma unroll
+            for (int y = 0; y < NK; y++) {
+                kf[u % RING][y] = kfrag(kbuf, y, u);
+                vf[u % RING][y] = vfrag(vbuf, y, u & 3, u >> 2);
+            }
+        };
+#pragma unroll
+        for (int x = 0; x < RB; x++) st[x] = (pp_f32x16){};
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) read(u);
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            if (u + AHEAD < 8) read(u + AHEAD);
+#pragma unroll
+            for (int n = 0; n < PAIRS; n++)
+#pragma unroll
+                for (int x = 0; x < RB; x++) {
+                    st[x] = pp_mfma(kf[u % RING][L.a[n]], q[x][u][L.b[n]], st[x]);
+                    o[x][u & 3] = pp_mfma(vf[u % RING][L.a[n]], pt[x][u >> 2][L.b[n]], o[x][u & 3]);
+                }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 3 * NK * AHEAD, 0);
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            if (u + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 3 * NK, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * RB * PAIRS, 0);
+        }
+    };
+    // The probabilities of the tile at k0.  The maximum that they are taken against follows the
+    // running one only once a row has passed it by 2^8: p stays below that, no sum is the worse
+    // for it, and most tiles leave the accumulators alone.
+    auto softmax = [&](int k0, unsigned seen, auto guarded) {
+        if (seen != 0xffffffffu || k0 + PP_KT - 1 > pos_lo) {                  // wave-uniform
+#pragma unroll
+            for (int x = 0; x < RB; x++) {
+                const int last = pos[x] - k0;
+                const unsigned bits = (last >= 31 ? seen : last < 0 ? 0u : seen & ((2u << last) - 1)) >> (4 * hl);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if ((int)(bits << (31 - 8 * (r / 4) - r % 4)) >= 0) st[x][r] = -INFINITY;
             }
         }
-        if (wave_on && k0 <= pos_hi) {
-            pp_f32x16 st = {};
 #pragma unroll
-            for (int t = 0; t < 8; t++) {
-                bf16x8 kf[NK];
+        for (int x = 0; x < RB; x++) {
+            float mx = st[x][0];
 #pragma unroll
-                for (int x = 0; x < NK; x++)
-                    kf[x] = *reinterpret_cast<const bf16x8 *>(&lds[buf][0][x][256 * ql + 16 * ((2 * t + hl) ^ ksw)]);
-                st = pp_products<NK, NQ>(kf, q[t], st);
-            }
-            const unsigned seen = *reinterpret_cast<const unsigned *>(seen_lds[buf]);
-            const bool open = seen == 0xffffffffu && k0 + PP_KT - 1 <= pos_lo;    // wave-uniform
-            if (!open) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int key = 8 * (r / 4) + 4 * hl + r % 4;
-                    if (!((seen >> key) & 1) || k0 + key > pos) st[r] = -INFINITY;
-                }
-            }
-            float mx = st[0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[r]);
+            for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[x][r]);
             float other = mx;
             swap32(mx, other);
-            const float mn = fmaxf(m, fmaxf(mx, other) * sc), ref = pg_ref(mn);
-            const float corr = __builtin_amdgcn_exp2f(m - ref);
-            m = mn;
+            mx = fmaxf(mx, other) * sc;
+            if (__any(mx > m[x] + 8.0f)) {
+                const float mn = fmaxf(m[x], mx), corr = __builtin_amdgcn_exp2f(m[x] - pg_ref(mn));
+                m[x] = mn;
+                l[x] *= corr;
+#pragma unroll
+                for (int d = 0; d < 4; d++) o[x][d] *= corr;
+            }
+            const float ref = pg_ref(m[x]);
             float p[16], sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                p[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sc, -ref));
+                p[r] = __builtin_amdgcn_exp2f(fmaf(st[x][r], sc, -ref));
                 sum += p[r];
             }
-            l = fmaf(l, corr, sum);
-            if (!__all(corr == 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < 4; d++) o[d] *= corr;
-            }
-            bf16x8 pt[2][NQ];
-            pp_terms8<NQ>(p, pt[0]);
-            pp_terms8<NQ>(p + 8, pt[1]);
-            if (!guarded) {
-#pragma unroll
-                for (int d = 0; d < 4; d++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        bf16x8 vf[NK];
-#pragma unroll
-                        for (int x = 0; x < NK; x++) vf[x] = pp_vfrag(vaddr(buf, x, d, j));
-                        o[d] = pp_products<NK, NQ>(vf, pt[j], o[d]);
-                    }
-            } else {
-                // finite values as ever, and how many infinite ones (and ones that are no
-                // number) each row sees, counted on the matrix cores: + 1, 64 or 4096
-                // each, at most 32 of them
-                bf16x8 one[2];
+            l[x] += sum;
+            pp_terms8<NQ>(p, pt[x][0]);
+            pp_terms8<NQ>(p + 8, pt[x][1]);
+            if constexpr (decltype(guarded)::value) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    float x[8];
+                    float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = p[8 * j + i] > 0.0f ? 1.0f : 0.0f;
+                    for (int i = 0; i < 8; i++) v[i] = p[8 * j + i] > 0.0f ? 1.0f : 0.0f;
                     bf16x8 t[1];
-                    pp_terms8<1>(x, t);
-                    one[j] = t[0];
-                }
-#pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    pp_f32x16 cnt = {};
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        bf16x8 vf[NK], cls;
-#pragma unroll
-                        for (int x = NK - 1; x >= 0; x--) vf[x] = pp_finite(pp_vfrag(vaddr(buf, x, d, j)), cls);
-                        o[d] = pp_products<NK, NQ>(vf, pt[j], o[d]);
-                        cnt = pp_mfma(cls, one[j], cnt);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int k = (int)cnt[r], pi = k & 63, ni = k >> 6 & 63;
-                        if (k >= 4096 || (pi && ni)) o[d][r] = NAN;
-                        else if (k) o[d][r] += pi ? INFINITY : -INFINITY;
-                    }
+                    pp_terms8<1>(v, t);
+                    one[x][j] = t[0];
                 }
             }
         }
-        if constexpr (DIRECT) buf ^= 1;
-    }
-    if (guarded) break;
+    };
+    // O^T += V^T P^T with V buffer buf, where values may be infinite or none: finite ones as ever,
+    // and how many others each row sees, counted on the matrix cores: + 1, 64 or 4096 each, at
+    // most 32 of them
+    auto values_guarded = [&](int buf) {
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+            for (int x = 0; x < RB; x++) {
+                pp_f32x16 cnt = {};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    bf16x8 vf[NK], cls;
+#pragma unroll
+                    for (int y = NK - 1; y >= 0; y--) vf[y] = pp_finite(vfrag(buf, y, d, j), cls);
+                    o[x][d] = pp_products<NK, NQ>(vf, pt[x][j], o[x][d]);
+                    cnt = pp_mfma(cls, one[x][j], cnt);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int k = (int)cnt[r], pi = k & 63, ni = k >> 6 & 63;
+                    if (k >= 4096 || (pi && ni)) o[x][d][r] = NAN;
+                    else if (k) o[x][d][r] += pi ? INFINITY : -INFINITY;
+                }
+            }
+    };
+
+    // What a walk begins with: its first tiles on their way.
+    Where next_v = {}, next_k = {};                       // of the tile whose V is fetched next, whose K was last
+    unsigned seen1 = 0, seen2 = 0;                        // of the next softmax's tile, and of the one behind it
+    float4 kr[DIRECT ? 2 : RPL], vr[DIRECT ? 2 : RPL];
+    auto prime = [&]() {
+        idv_at = INT_MIN / 2;
+        next_v = where(0);
+        next_k = where(1);
+        seen1 = next_v.seen;
+        seen2 = next_k.seen;
+        if constexpr (DIRECT) {
+            fetch(0, next_v, 0, 0);
+            fetch(1, next_k, 0, 1);
+            fetch(0, next_v, 1, 0);
+        } else {
+            load(0, next_v, 0, kr);
+        }
+    };
+    // The group's tiles.  Turn i is a matrix part (V of tile i, K of tile i + 1) and a vector part
+    // (softmax of tile i + 1, staging), a barrier behind each; the second group is a barrier
+    // behind the first, so that on every SIMD one wave's matrix part meets another's vector
+    // part.  Waves in step would leave the matrix cores idle in their vector parts.
+    auto walk = [&](auto guarded) {
+#pragma unroll
+        for (int x = 0; x < RB; x++) {
+#pragma unroll
+            for (int d = 0; d < 4; d++) o[x][d] = (pp_f32x16){};
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+        }
+        if (nt == 0) return;                              // block-uniform
+        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        else put(0, kr);
+        barrier(false);
+        if (KG == 2 && kg == 1) barrier(false);
+        for (int i = -1; i < nt; i++) {
+            if (wave_on) {
+                // past the last tile the scores are of its last key again, and not used
+                const int vbuf = DIRECT ? i & 1 : 0, kbuf = DIRECT ? (i + 1) & 1 : 0;
+                if constexpr (decltype(guarded)::value) {
+                    if (i >= 0) values_guarded(vbuf);
+                    scores(kbuf);
+                } else {
+                    if (i >= 0) matrix(vbuf, kbuf);
+                    else scores(kbuf);
+                }
+            }
+            barrier(false);
+            const unsigned seen = seen1;
+            seen1 = seen2;
+            if constexpr (DIRECT) {
+                // over K of tile i + 1 and V of tile i, which are read
+                next_v = next_k;
+                next_k = where(i + 3);
+                seen2 = next_k.seen;
+                fetch(i + 3, next_k, 0, (i + 1) & 1);
+                fetch(i + 2, next_v, 1, i & 1);
+                if (wave_on && i + 1 < nt) softmax(tile_k0(i + 1), seen, guarded);
+            } else {
+                if (i >= 0) {
+                    next_v = next_k;
+                    next_k = where(i + 2);
+                    seen1 = next_k.seen;
+                }
+                load(i + 2, next_k, 0, kr);
+                load(i + 1, next_v, 1, vr);
+                if (wave_on && i + 1 < nt) softmax(tile_k0(i + 1), seen, guarded);
+                put(0, kr);
+                put(1, vr);
+            }
+            barrier(DIRECT);
+        }
+        if (KG == 2 && kg == 0) barrier(false);
+        // nothing may land later: the tiles' memory is used again, and then another block's
+        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    };
+    if (nt > 0) prime();                                  // block-uniform
+
+    // queries: dims 16 t + 8 hl .. + 7; fp32 ones take the scale along
+#pragma unroll
+    for (int x = 0; x < RB; x++)
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            const T *qp = (const T *)a.q + orow(x) * PG_HD + 16 * t + 8 * hl;
+            if constexpr (NQ == 1) {
+                q[x][t][0] = *reinterpret_cast<const bf16x8 *>(qp);
+            } else {
+                const float4 x0 = pg_load4(qp), x1 = pg_load4(qp + 4);
+                const float fs = a.scale * PG_LOG2E;
+                const float v[8] = {x0.x * fs, x0.y * fs, x0.z * fs, x0.w * fs, x1.x * fs, x1.y * fs, x1.z * fs, x1.w * fs};
+                pp_terms8<NQ>(v, q[x][t]);
+            }
+        }
+    walk(PpBool<false>());
     float z = 0.0f;
 #pragma unroll
-    for (int d = 0; d < 4; d++)
+    for (int x = 0; x < RB; x++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) z = fmaf(o[d][r], 0.0f, z);
-    if (!__syncthreads_or(z != 0.0f)) break;              // 0 times what is infinite or no number is none
-    guarded = true;
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) z = fmaf(o[x][d][r], 0.0f, z);
+    // 0 times what is infinite or no number is none
+    if (__syncthreads_or(z != 0.0f)) {
+        if (nt > 0) prime();
+        walk(PpBool<true>());
+        if constexpr (KG > 1) __syncthreads();
     }
-    if (!wave_on) return;
 
-    float lo_ = l, hi_ = l;
-    swap32(lo_, hi_);
-    const float L = lo_ + hi_;
-    if (!on) return;
-    if (a.nsplit == 1) {
-        // 0 only where no key was seen: the largest p is 1
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        T *dst = (T *)a.out + orow * PG_HD + 4 * hl;
+    float L[RB];
 #pragma unroll
-        for (int d = 0; d < 4; d++)
+    for (int x = 0; x < RB; x++) {
+        float u = l[x], v = l[x];
+        swap32(u, v);
+        L[x] = u + v;
+    }
+    if constexpr (KG == 2) {
+        // the second group's sums over the buffers that were last read before the barrier
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                pg_store4(dst + 32 * d + 2 * r, make_float4(o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv));
-    } else {
-        const size_t at = orow * a.nsplit + split;
-        float *dst = a.part_o + at * PG_HD + 4 * hl;
+        for (int x = 0; x < RB; x++) {
+            float4 *po = reinterpret_cast<float4 *>(lds_all + (wave * RB + x) * 16384) + lane;
+            float2 *pm = reinterpret_cast<float2 *>(lds_all + WR * RB * 16384 + (wave * RB + x) * 512) + lane;
+            if (kg == 1) {
 #pragma unroll
-        for (int d = 0; d < 4; d++)
+                for (int i = 0; i < 16; i++) {
+                    const int d = i / 4, r = 4 * (i % 4);
+                    po[64 * i] = make_float4(o[x][d][r], o[x][d][r + 1], o[x][d][r + 2], o[x][d][r + 3]);
+                }
+                *pm = make_float2(m[x], L[x]);
+            }
+        }
+        __syncthreads();
+        if (kg == 1) return;
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<float4 *>(dst + 32 * d + 2 * r) = make_float4(o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
-        if (hl == 0) {
-            a.part_ml[2 * at] = m;
-            a.part_ml[2 * at + 1] = L;
+        for (int x = 0; x < RB; x++) {
+            const float4 *po = reinterpret_cast<const float4 *>(lds_all + (wave * RB + x) * 16384) + lane;
+            const float2 ml = *(reinterpret_cast<const float2 *>(lds_all + WR * RB * 16384 + (wave * RB + x) * 512) + lane);
+            const float mn = fmaxf(m[x], ml.x), ref = pg_ref(mn);
+            const float c0 = __builtin_amdgcn_exp2f(m[x] - ref), c1 = __builtin_amdgcn_exp2f(ml.x - ref);
+            m[x] = mn;
+            L[x] = fmaf(L[x], c0, ml.y * c1);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int d = i / 4, r = 4 * (i % 4);
+                const float4 v = po[64 * i];
+                o[x][d][r] = fmaf(v.x, c1, o[x][d][r] * c0);
+                o[x][d][r + 1] = fmaf(v.y, c1, o[x][d][r + 1] * c0);
+                o[x][d][r + 2] = fmaf(v.z, c1, o[x][d][r + 2] * c0);
+                o[x][d][r + 3] = fmaf(v.w, c1, o[x][d][r + 3] * c0);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < RB; x++) {
+        if (!on[x]) continue;
+        if (a.nsplit == 1) {
+            // 0 only where no key was seen: the largest p is 1
+            const float inv = L[x] == 0.0f ? 0.0f : 1.0f / L[x];
+            T *dst = (T *)a.out + orow(x) * PG_HD + 4 * hl;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    pg_store4(dst + 32 * d + 2 * r, make_float4(o[x][d][r] * inv, o[x][d][r + 1] * inv,
+                                                                o[x][d][r + 2] * inv, o[x][d][r + 3] * inv));
+        } else {
+            const size_t at = orow(x) * a.nsplit + split;
+            float *dst = a.part_o + at * PG_HD + 4 * hl;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<float4 *>(dst + 32 * d + 2 * r) =
+                        make_float4(o[x][d][r], o[x][d][r + 1], o[x][d][r + 2], o[x][d][r + 3]);
+            if (hl == 0) {
+                a.part_ml[2 * at] = m[x];
+                a.part_ml[2 * at + 1] = L[x];
+            }
         }
     }
 }
 
+#define PP_PLAN_ROWS 128          // rows of the plan's tiles
+
 extern "C" void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_heads, int max_len, int *nsplit,
                                       int *chunk) {
-    const long tiles = (long)rows * (heads / kv_heads) / PP_ROWS + n_seqs;
+    const long tiles = (long)rows * (heads / kv_heads) / PP_PLAN_ROWS + n_seqs;
     const long blocks = tiles * kv_heads;
     long n = (512 + blocks - 1) / blocks;
     if (n > QK_PAGED_MAX_SPLIT) n = QK_PAGED_MAX_SPLIT;
@@ -467,16 +741,18 @@ extern "C" void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_he
     *chunk = (int)c;
 }
 
-extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
-    const long slots = (long)a->pg.rows * (a->heads / a->pg.kv_heads) / PP_ROWS + a->pg.n_seqs;
+template <typename T, typename C>
+static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
+    using S = PpShape<T, C>;
+    const long slots = (long)a->pg.rows * (a->heads / a->pg.kv_heads) / S::ROWS + a->pg.n_seqs;
     if (slots * a->pg.kv_heads > 0x7fffffffL) return QWEN_HIP_EINVAL;
     const dim3 grid((unsigned)(slots * a->pg.kv_heads), (unsigned)a->nsplit);
-    if (a->act_bf16) {
-        if (a->pg.cache_bf16) paged_prefill<uint16_t, uint16_t><<<grid, 256, 0, s>>>(*a);
-        else paged_prefill<uint16_t, float><<<grid, 256, 0, s>>>(*a);
-    } else {
-        if (a->pg.cache_bf16) paged_prefill<float, uint16_t><<<grid, 256, 0, s>>>(*a);
-        else paged_prefill<float, float><<<grid, 256, 0, s>>>(*a);
-    }
+    if ((1 << a->pg.page_shift) < PP_KT / S::WR) paged_prefill<T, C, true><<<grid, S::THREADS, 0, s>>>(*a, (int)slots);
+    else paged_prefill<T, C, false><<<grid, S::THREADS, 0, s>>>(*a, (int)slots);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
+}
+
+extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
+    if (a->act_bf16) return a->pg.cache_bf16 ? prefill_launch<uint16_t, uint16_t>(a, s) : prefill_launch<uint16_t, float>(a, s);
+    return a->pg.cache_bf16 ? prefill_launch<float, uint16_t>(a, s) : prefill_launch<float, float>(a, s);
 }
