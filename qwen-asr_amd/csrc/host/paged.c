@@ -29,6 +29,9 @@ static int paged_view(const char *op, const qwen_hip_paged_kv *kv, const qwen_hi
     if (kv->n_pages <= 0 || kv->kv_heads <= 0 || kv->n_seqs < 0 || kv->table_stride <= 0)
         QK_REFUSE("%s: n_pages %d, kv_heads %d, n_seqs %d, table_stride %d", op, kv->n_pages, kv->kv_heads, kv->n_seqs,
                kv->table_stride);
+    /* 2^31 rows of 128 values are more than any memory holds */
+    if ((double)kv->n_pages * kv->kv_heads * kv->page_size > (double)INT_MAX)
+        QK_REFUSE("%s: %d pages of %d positions and %d kv heads", op, kv->n_pages, kv->page_size, kv->kv_heads);
     if (heads <= 0 || heads % kv->kv_heads) QK_REFUSE("%s: %d heads over %d kv heads", op, heads, kv->kv_heads);
     if (b->rows < 0 || b->max_len < 0) QK_REFUSE("%s: rows %d, max_len %d", op, b->rows, b->max_len);
     if ((long)b->rows * heads > INT_MAX / QWEN_HIP_HEAD_DIM) QK_REFUSE("%s: %d rows of %d heads", op, b->rows, heads);

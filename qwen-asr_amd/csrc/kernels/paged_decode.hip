@@ -8,68 +8,80 @@
 // Bound by the bytes of K and V: every K and V row is read once for all query
 // heads that share it (up to 8 in one block; more take another block's pass).
 //
-// Block (sequence x kv head x up to 8 heads, split): four waves take the
-// split's keys in turns of 4 U.  Sixteen lanes own one key (8 dims a lane: 16 or
-// 32 bytes, whole rows contiguous within a page), with statistics of their own,
-// joined at the end: over the wave's four groups by row swaps, over the waves in
-// LDS.  Loads of a turn (U keys' K and V a lane) are all in flight before the
-// first product.
+// Block (sequence x kv head x up to 8 heads, split): four waves take the split's
+// keys in turns.  L lanes own one key (128 / L dims a lane, in 8-dim chunks L
+// apart, so that the lanes of a load read whole lines), each such group with
+// statistics of its own, joined at the end: over the wave by halving exchanges,
+// over the waves in LDS.  Fewer lanes a key mean fewer steps of the sum over them
+// and fewer lanes that compute the same exponential, but more registers for
+// queries and outputs: 8 lanes for one or two heads (4 lanes: 68 us against 49 at
+// the second size below), 16 for four and eight.  Loads of a turn (U keys' K and V
+// a group) are all in flight before the first product, the page ids of the next
+// turn before those.
+//
+// Measured, kernel and join, 8 kv heads, bf16 cache (a device copy moves 4.8 TB/s):
+//   64 sequences of 31 to 4097 positions, bf16 rows, 2 heads each: 49 us, 4.5 TB/s
+//   3 sequences of 20011 to 32769, fp32 rows, 4 heads each: 67 us, 4.9 TB/s
+// One short sequence is the time of two launches (11 us).
 #include "paged.h"
 
-struct PdRow8 {
-    float x[8];
-};
-__device__ __forceinline__ PdRow8 pd_widen(uint4 w) {
-    return {{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y), bf16_lo(w.z), bf16_hi(w.z), bf16_lo(w.w),
-             bf16_hi(w.w)}};
+// 8 values of a cached row as they lie in memory, widened at their use.  NT: rows that are
+// read once pass by the caches (64 streams, 224 MB of pages: 56 us without, 49 with).
+typedef uint32_t pd_u32x4 __attribute__((ext_vector_type(4)));
+template <bool NT>
+__device__ __forceinline__ pd_u32x4 pd_load16(const void *p) {
+    const pd_u32x4 *q = (const pd_u32x4 *)p;
+    if constexpr (NT) return __builtin_nontemporal_load(q);
+    else return *q;
 }
-
-// 8 values of a cached row as they lie in memory, widened at their use
 template <typename C>
-struct PdRaw;
-template <>
-struct PdRaw<uint16_t> {
-    uint4 w;
-    __device__ __forceinline__ void load(const uint16_t *p) { w = *reinterpret_cast<const uint4 *>(p); }
-    __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ PdRow8 get() const { return pd_widen(w); }
-};
-template <>
-struct PdRaw<float> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const float *p) {
-        a = *reinterpret_cast<const float4 *>(p);
-        b = *reinterpret_cast<const float4 *>(p + 4);
+struct PdRaw {
+    static constexpr int N = sizeof(C) / 2;
+    pd_u32x4 w[N];
+    template <bool NT>
+    __device__ __forceinline__ void load(const C *p) {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = pd_load16<NT>((const pd_u32x4 *)p + i);
     }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ __forceinline__ PdRow8 get() const { return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = (pd_u32x4){0u, 0u, 0u, 0u};
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if constexpr (N == 2) x[i] = __uint_as_float(w[i / 4][i % 4]);
+            else x[i] = i % 2 ? bf16_hi(w[0][i / 2]) : bf16_lo(w[0][i / 2]);
+        }
+    }
 };
+
+// Sums over the lanes that differ in the bits 32, 16, .., L of v[N], halving the values that
+// a lane carries at each step: the lane ends with N L / 64 of them, from `base` on.
+template <int N, int M, int L, int FULL>
+__device__ __forceinline__ void pd_gather(float (&v)[FULL], int lane, int &base) {
+    if constexpr (M >= L) {
+        transpose_step<FULL, M>(v, N, lane);
+        if (lane & M) base += N / 2;
+        pd_gather<N / 2, M / 2, L, FULL>(v, lane, base);
+    }
+}
 
 __device__ __forceinline__ int pd_chunk(int len, int chunk, int nsplit) {
     const int need = (int)(((long)len + nsplit - 1) / nsplit);
     return max(chunk, (need + 63) & ~63);
 }
 
-template <typename T, typename C, int GT, int U>
+template <typename T, typename C, int GT, int L, int U, bool NT>
 __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gchunks) {
+    constexpr int D = PG_HD / L, NC = D / 8, KEYS = 64 / L;      // dims and chunks a lane, keys a wave at once
     const qk_paged &pg = a.pg;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, grp = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % L, grp = lane / L;
     const int G = a.heads / pg.kv_heads;
     const int kvh = blockIdx.x / gchunks % pg.kv_heads, s = blockIdx.x / gchunks / pg.kv_heads;
     const int g0 = blockIdx.x % gchunks * GT, gn = min(GT, G - g0);
     const int h0 = kvh * G + g0, split = blockIdx.y;
     const size_t qrow = (size_t)s * a.heads + h0;
-
-    // this lane's 8 dims of each head's query, times scale * log2(e)
-    float q[GT][8];
-#pragma unroll
-    for (int g = 0; g < GT; g++) {
-        const T *qp = (const T *)a.q + (qrow + min(g, gn - 1)) * PG_HD + 8 * c;
-        const float4 x = pg_load4(qp), y = pg_load4(qp + 4);
-        const float f = a.scale * PG_LOG2E;
-        q[g][0] = x.x * f; q[g][1] = x.y * f; q[g][2] = x.z * f; q[g][3] = x.w * f;
-        q[g][4] = y.x * f; q[g][5] = y.y * f; q[g][6] = y.z * f; q[g][7] = y.w * f;
-    }
     const int len = min(pg_len(pg, s), pg.capacity);
     const int chunk = pd_chunk(len, a.chunk, a.nsplit);
     const long first = (long)split * chunk;
@@ -84,64 +96,103 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
     }
     const int k0 = (int)first, k1 = (int)min((long)len, first + chunk);
 
-    float m[GT], l[GT], o[GT][8];
+    // rows of a kv head: page id * rstride + slot (the host has seen that they fit an int)
+    const int *const table = pg.table + (size_t)s * pg.table_stride;
+    const int rstride = pg.kv_heads << pg.page_shift, smask = (1 << pg.page_shift) - 1;
+    const C *kp = (const C *)pg.k + ((size_t)kvh << pg.page_shift) * PG_HD + 8 * c;
+    const C *vp = (const C *)pg.v + ((size_t)kvh << pg.page_shift) * PG_HD + 8 * c;
+    constexpr int TURN = KEYS * U;                    // keys of one wave's turn
+    int pid[U];
+    auto ids = [&](int kb) {
+#pragma unroll
+        for (int u = 0; u < U; u++) pid[u] = k1 > k0 ? table[min(kb + KEYS * u + grp, k1 - 1) >> pg.page_shift] : -1;
+    };
+    ids(k0 + wave * TURN);
+
+    // this lane's dims of each head's query, times scale * log2(e)
+    float q[GT][D];
+#pragma unroll
+    for (int g = 0; g < GT; g++) {
+        const T *qp = (const T *)a.q + (qrow + min(g, gn - 1)) * PG_HD + 8 * c;
+        const float f = a.scale * PG_LOG2E;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const float4 x = pg_load4(qp + 8 * L * i), y = pg_load4(qp + 8 * L * i + 4);
+            float *o = &q[g][8 * i];
+            o[0] = x.x * f; o[1] = x.y * f; o[2] = x.z * f; o[3] = x.w * f;
+            o[4] = y.x * f; o[5] = y.y * f; o[6] = y.z * f; o[7] = y.w * f;
+        }
+    }
+    float m[GT], l[GT], o[GT * D];
 #pragma unroll
     for (int g = 0; g < GT; g++) {
         m[g] = -INFINITY;
         l[g] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[g][i] = 0.0f;
     }
-    const C *kp = (const C *)pg.k, *vp = (const C *)pg.v;
-    constexpr int TURN = 4 * U;                       // keys of one wave's turn
-    int pid[U];
-    auto ids = [&](int kb) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int key = kb + 4 * u + grp;
-            pid[u] = key < k1 ? pg_page(pg, s, key) : -1;
-        }
-    };
-    ids(k0 + wave * TURN);
+    for (int i = 0; i < GT * D; i++) o[i] = 0.0f;
+
     for (int kb = k0 + wave * TURN; kb < k1; kb += 4 * TURN) {
-        PdRaw<C> kr[U], vr[U];
+        PdRaw<C> kr[U][NC], vr[U][NC];
         bool on[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            on[u] = pid[u] >= 0;
-            if (on[u]) {
-                const size_t off = pg_offset(pg, pid[u], kvh, kb + 4 * u + grp) + 8 * c;
-                kr[u].load(kp + off);
-                vr[u].load(vp + off);
-            } else {
-                kr[u].zero();
-                vr[u].zero();
+            // a key past the end, or without a page, is read where it does no harm and weighs nothing
+            const int key = kb + KEYS * u + grp;
+            const bool page = (unsigned)pid[u] < (unsigned)pg.n_pages;
+            on[u] = page && key < k1;
+            const size_t row = (unsigned)((page ? pid[u] : 0) * rstride + (min(key, k1 - 1) & smask));
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                kr[u][i].template load<NT>(kp + row * PG_HD + 8 * L * i);
+                vr[u][i].template load<NT>(vp + row * PG_HD + 8 * L * i);
             }
         }
-        ids(kb + 4 * TURN);                           // the next turn's pages
+        if (kb + 4 * TURN < k1) ids(kb + 4 * TURN);   // the next turn's pages
         float sc[U][GT];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const PdRow8 k8 = kr[u].get();
+#pragma unroll
+            for (int g = 0; g < GT; g++) sc[u][g] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                float x[8];
+                kr[u][i].get(x);
+#pragma unroll
+                for (int g = 0; g < GT; g++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) sc[u][g] = fmaf(q[g][8 * i + e], x[e], sc[u][g]);
+            }
 #pragma unroll
             for (int g = 0; g < GT; g++) {
-                float d = q[g][0] * k8.x[0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) d = fmaf(q[g][i], k8.x[i], d);
-                d = group_sum<16>(d);
+                const float d = group_sum<L>(sc[u][g]);
                 sc[u][g] = on[u] ? d : -INFINITY;
+            }
+        }
+        // the maximum, followed once a key has passed it by 2^8: weights stay below that, no sum is the
+        // worse for it, and most turns leave the outputs alone
+        bool passed = false;
+        float mx[GT];
+#pragma unroll
+        for (int g = 0; g < GT; g++) {
+            mx[g] = sc[0][g];
+#pragma unroll
+            for (int u = 1; u < U; u++) mx[g] = fmaxf(mx[g], sc[u][g]);
+            passed = passed || mx[g] > m[g] + 8.0f;
+        }
+        if (__any(passed)) {
+#pragma unroll
+            for (int g = 0; g < GT; g++) {
+                const float mn = fmaxf(m[g], mx[g]), corr = __builtin_amdgcn_exp2f(m[g] - pg_ref(mn));
+                m[g] = mn;
+                l[g] *= corr;
+#pragma unroll
+                for (int i = 0; i < D; i++) o[g * D + i] *= corr;
             }
         }
 #pragma unroll
         for (int g = 0; g < GT; g++) {
-            float mn = m[g];
-#pragma unroll
-            for (int u = 0; u < U; u++) mn = fmaxf(mn, sc[u][g]);
-            const float ref = pg_ref(mn), corr = __builtin_amdgcn_exp2f(m[g] - ref);
-            m[g] = mn;
-            l[g] *= corr;
-#pragma unroll
-            for (int i = 0; i < 8; i++) o[g][i] *= corr;
+            const float ref = pg_ref(m[g]);
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 sc[u][g] = __builtin_amdgcn_exp2f(sc[u][g] - ref);
@@ -149,76 +200,89 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const PdRow8 v8 = vr[u].get();
+        for (int u = 0; u < U; u++)
+            if (!__all(on[u])) {                      // the last turn: nothing may come of 0 times what is there
 #pragma unroll
-            for (int g = 0; g < GT; g++)
+                for (int i = 0; i < NC; i++)
+                    if (!on[u]) vr[u][i].zero();
+            }
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[g][i] = fmaf(sc[u][g], v8.x[i], o[g][i]);
-        }
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                float x[8];
+                vr[u][i].get(x);
+#pragma unroll
+                for (int g = 0; g < GT; g++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) o[g * D + 8 * i + e] = fmaf(sc[u][g], x[e], o[g * D + 8 * i + e]);
+            }
     }
 
-    // the wave's four groups, then the four waves
+    // the wave's groups, then the four waves
     __shared__ __attribute__((aligned(16))) float so[4][GT][PG_HD];
     __shared__ float sm[4][GT], sl[4][GT];
 #pragma unroll
     for (int g = 0; g < GT; g++) {
-        const float M = xor_max16_32(m[g]), f = __builtin_amdgcn_exp2f(m[g] - pg_ref(M));
-        const float L = xor_sum16_32(l[g] * f);
-        float t[8];
+        const float M = wave_max(m[g]), f = __builtin_amdgcn_exp2f(m[g] - pg_ref(M));
+        const float S = wave_sum(l[g] * f) * (1.0f / L);          // L lanes hold the same
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = xor_sum16_32(o[g][i] * f);
-        if (grp == 0) {
-            *reinterpret_cast<float4 *>(&so[wave][g][8 * c]) = make_float4(t[0], t[1], t[2], t[3]);
-            *reinterpret_cast<float4 *>(&so[wave][g][8 * c + 4]) = make_float4(t[4], t[5], t[6], t[7]);
-        }
+        for (int i = 0; i < D; i++) o[g * D + i] *= f;
         if (lane == 0) {
             sm[wave][g] = M;
-            sl[wave][g] = L;
+            sl[wave][g] = S;
         }
+    }
+    int base = 0;
+    pd_gather<GT * D, 32, L>(o, lane, base);
+#pragma unroll
+    for (int i = 0; i < GT * D * L / 64; i++) {
+        const int n = base + i, g = n / D, e = n % D;             // dim: chunk e / 8 of this lane's
+        so[wave][g][8 * c + 8 * L * (e / 8) + e % 8] = o[i];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < gn * (PG_HD / 4); i += 256) {
         const int g = i / (PG_HD / 4), d = 4 * (i % (PG_HD / 4));
         const float M = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g])), ref = pg_ref(M);
-        float L = 0.0f;
+        float sum = 0.0f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float f = __builtin_amdgcn_exp2f(sm[w][g] - ref);
             const float4 x = *reinterpret_cast<const float4 *>(&so[w][g][d]);
-            L = fmaf(sl[w][g], f, L);
+            sum = fmaf(sl[w][g], f, sum);
             v.x = fmaf(x.x, f, v.x);
             v.y = fmaf(x.y, f, v.y);
             v.z = fmaf(x.z, f, v.z);
             v.w = fmaf(x.w, f, v.w);
         }
         if (a.nsplit == 1) {
-            // L is 0 only where no key was seen (the largest p is 1); a sum that is no number stays one
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            // 0 only where no key was seen (the largest p is at least 2^-8); a sum that is no number stays one
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             pg_store4((T *)a.out + (qrow + g) * PG_HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         } else {
             const size_t at = (qrow + g) * a.nsplit + split;
             *reinterpret_cast<float4 *>(a.part_o + at * PG_HD + d) = v;
             if (d == 0) {
                 a.part_ml[2 * at] = M;
-                a.part_ml[2 * at + 1] = L;
+                a.part_ml[2 * at + 1] = sum;
             }
         }
     }
 }
 
 // ---------------------------------------------------------------------------
-// The join: a wave per (row, head), two dims a lane.  Lane i holds split i's
+// The join: W waves per (row, head), two dims a lane.  Lane i holds split i's
 // maximum and sum, so one load and one wave maximum give every weight; splits
-// with the sum 0 have no partial output and are skipped.  Rows before the first
-// or behind the last sequence have no partials and are left as they are.
+// with the sum 0 have no partial output and are skipped.  A wave takes every W-th
+// split, 16 loads in flight.  Rows before the first or behind the last sequence have
+// no partials and are left as they are.
 // ---------------------------------------------------------------------------
-template <typename T>
+template <typename T, int W>
 __global__ __launch_bounds__(256) void paged_merge(qk_paged_attn_args a) {
     const qk_paged &pg = a.pg;
-    const int lane = threadIdx.x & 63;
-    const long u = 4L * blockIdx.x + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long u = W == 1 ? 4L * blockIdx.x + wave : (long)blockIdx.x;
     if (u >= (long)pg.rows * a.heads) return;
     if (pg.row_start) {
         const int row = (int)(u / a.heads);
@@ -238,21 +302,34 @@ __global__ __launch_bounds__(256) void paged_merge(qk_paged_attn_args a) {
     const float L = wave_sum(l * f);
     const unsigned long long some = __ballot(l != 0.0f);
     float x = 0.0f, y = 0.0f;
-    const int last = 63 - __clzll((long long)some | 1);
-    // four loads in flight; a split without keys reads the last one that has some
-    for (int i0 = 0; i0 <= last; i0 += 4) {
-        float2 v[4];
+    const int last = 63 - __clzll((long long)some | 1), first = W == 1 ? 0 : wave;
+    // a split without keys reads the last one that has some, with no weight
+    constexpr int F = W == 1 ? 8 : 16;
+    for (int i0 = first; some && i0 <= last; i0 += F * W) {
+        float2 v[F];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int i = (some >> min(i0 + j, 63)) & 1 ? i0 + j : last;
-            v[j] = some ? *reinterpret_cast<const float2 *>(a.part_o + (at + i) * PG_HD + 2 * lane) : make_float2(0.f, 0.f);
+        for (int j = 0; j < F; j++) {
+            const int i = i0 + W * j <= last && (some >> (i0 + W * j)) & 1 ? i0 + W * j : last;
+            v[j] = *reinterpret_cast<const float2 *>(a.part_o + (at + i) * PG_HD + 2 * lane);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (i0 + j > last || !((some >> (i0 + j)) & 1)) continue;
-            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i0 + j));
+        for (int j = 0; j < F; j++) {
+            if (i0 + W * j > last || !((some >> (i0 + W * j)) & 1)) continue;
+            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i0 + W * j));
             x = fmaf(v[j].x, w, x);
             y = fmaf(v[j].y, w, y);
+        }
+    }
+    if constexpr (W > 1) {
+        __shared__ float2 part[W][64];
+        part[wave][lane] = make_float2(x, y);
+        __syncthreads();
+        if (wave > 0) return;
+        x = y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            x += part[i][lane].x;
+            y += part[i][lane].y;
         }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -262,10 +339,17 @@ __global__ __launch_bounds__(256) void paged_merge(qk_paged_attn_args a) {
 }
 
 extern "C" int qk_paged_merge_launch(const qk_paged_attn_args *a, hipStream_t s) {
-    const long blocks = ((long)a->pg.rows * a->heads + 3) / 4;
-    if (blocks > 0x7fffffffL) return QWEN_HIP_EINVAL;
-    if (a->act_bf16) paged_merge<uint16_t><<<(unsigned)blocks, 256, 0, s>>>(*a);
-    else paged_merge<float><<<(unsigned)blocks, 256, 0, s>>>(*a);
+    const long units = (long)a->pg.rows * a->heads;
+    // few rows with many splits: a block each
+    const bool wide = a->nsplit > 16 && units <= 4096;
+    const unsigned blocks = (unsigned)(wide ? units : (units + 3) / 4);
+    if (a->act_bf16) {
+        if (wide) paged_merge<uint16_t, 4><<<blocks, 256, 0, s>>>(*a);
+        else paged_merge<uint16_t, 1><<<blocks, 256, 0, s>>>(*a);
+    } else {
+        if (wide) paged_merge<float, 4><<<blocks, 256, 0, s>>>(*a);
+        else paged_merge<float, 1><<<blocks, 256, 0, s>>>(*a);
+    }
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }
 
@@ -288,11 +372,11 @@ template <typename T, typename C>
 static void decode_dispatch(const qk_paged_attn_args *a, hipStream_t s) {
     const int G = a->heads / a->pg.kv_heads, gt = decode_gt(G), gc = (G + gt - 1) / gt;
     const dim3 grid((unsigned)(a->pg.rows * a->pg.kv_heads * gc), (unsigned)a->nsplit);
-    constexpr int U = 4;
-    if (gt == 1) paged_decode<T, C, 1, U><<<grid, 256, 0, s>>>(*a, gc);
-    else if (gt == 2) paged_decode<T, C, 2, U><<<grid, 256, 0, s>>>(*a, gc);
-    else if (gt == 4) paged_decode<T, C, 4, U><<<grid, 256, 0, s>>>(*a, gc);
-    else paged_decode<T, C, 8, U><<<grid, 256, 0, s>>>(*a, gc);
+    if (gt == 1) paged_decode<T, C, 1, 8, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+    else if (gt == 2) paged_decode<T, C, 2, 8, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+    else if (gt == 4) paged_decode<T, C, 4, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+    else if (gc == 1) paged_decode<T, C, 8, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+    else paged_decode<T, C, 8, 16, 4, false><<<grid, 256, 0, s>>>(*a, gc);      // every block of heads reads the rows
 }
 
 extern "C" int qk_paged_decode_launch(const qk_paged_attn_args *a, hipStream_t s) {

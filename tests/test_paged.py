@@ -38,7 +38,7 @@ def attend(qa, which, kvd={}, bd={}, **k):
 
 
 BAD_KV = [dict(dtype=1), dict(dtype=-1), dict(head_dim=64), dict(page_size=0), dict(page_size=24),
-          dict(page_size=1 << 25), dict(n_pages=0), dict(kv_heads=0), dict(kv_heads=3), dict(n_seqs=-1),
+          dict(page_size=1 << 25), dict(n_pages=0), dict(kv_heads=0), dict(kv_heads=3), dict(n_seqs=-1), dict(n_pages=2 ** 31 - 1),
           dict(table_stride=0), dict(k=None), dict(v=None), dict(table=None), dict(k=P + 8), dict(v=P + 2)]
 BAD_BATCH = [dict(rows=-1), dict(max_len=-1), dict(kv_len=None), dict(rows=2 ** 31 - 1)]
 
