@@ -534,8 +534,9 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
  * 1e-30 .. 1e30.  _decode takes one row per sequence (row_start NULL), _prefill
  * packed rows (row_start given; sequences may have no rows, one, or all of their
  * positions).  Softmax statistics and sums in fp32.  fp32 rows: products exact to
- * 2^-24 on either cache type; bf16 rows: _prefill rounds the probabilities to
- * bf16 before they meet V.  A key with an infinite element makes the rows that see
+ * 2^-24 on either cache type; bf16 rows: _prefill, and _decode of more than four
+ * heads a kv head on a bf16 cache, round the probabilities to bf16 before they
+ * meet V.  A key with an infinite element makes the rows that see
  * it undefined (NaN); what a row does not see never reaches it.  The workspace
  * holds the partial results of a split over the positions. */
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);

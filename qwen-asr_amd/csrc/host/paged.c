@@ -97,10 +97,23 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
     return 0;
 }
 
+/*
+ * Whether single tokens run on the matrix cores, as prompts of one row do: where many heads share
+ * a bf16 cache's rows, the vector units are what bounds the other kernel.  Microseconds, vector
+ * kernel against matrix kernel, 24 sequences of 500 to 6001 positions, 8 kv heads:
+ *   bf16 rows, 4 heads a kv head: 59, 66; 8: 104, 73; 16: 139, 74
+ *   fp32 rows (split into three terms), 8: 104, 101; 16: 139, 123
+ * 24 sequences of 131 to 530, bf16, 5 heads: 26, 25; 16: 40, 26.  fp32 pages take the matrix
+ * kernel longer throughout (8 heads: 138, 234).
+ */
+static int tokens_by_matrix(int act_bf16, int cache_bf16, int group) {
+    return cache_bf16 && group > (act_bf16 ? 4 : 8);
+}
+
 /* splits of an attention call and the workspace it needs */
-static size_t attention_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk) {
+static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int *nsplit, int *chunk) {
     if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;
-    if (p->row_start) qk_paged_prefill_plan(p->rows, p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
+    if (matrix) qk_paged_prefill_plan(p->rows, p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
     else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
     if (*nsplit == 1) return 0;
     return (size_t)p->rows * heads * *nsplit * (QWEN_HIP_HEAD_DIM + 2) * sizeof(float);
@@ -110,7 +123,15 @@ size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen
     qk_paged p;
     int nsplit, chunk;
     if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || p.rows == 0) return 0;
-    return attention_plan(&p, heads, batch->max_len, &nsplit, &chunk);
+    const int group = heads / p.kv_heads;
+    size_t need = 0;
+    /* of either type of rows */
+    for (int bf16 = 0; bf16 <= 1; bf16++) {
+        const int matrix = p.row_start || tokens_by_matrix(bf16, p.cache_bf16, group);
+        const size_t n = attention_plan(&p, matrix, heads, batch->max_len, &nsplit, &chunk);
+        need = n > need ? n : need;
+    }
+    return need;
 }
 
 static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch,
@@ -127,7 +148,8 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
     if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);
     if (out == q) QK_REFUSE("%s: out cannot be q", op);
-    const size_t need = attention_plan(&a.pg, heads, batch->max_len, &a.nsplit, &a.chunk);
+    const int matrix = prefill || tokens_by_matrix(dtype == QWEN_HIP_ST_BF16, a.pg.cache_bf16, heads / a.pg.kv_heads);
+    const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, &a.nsplit, &a.chunk);
     if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);
     a.out = out;
@@ -137,7 +159,7 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
     a.scale = scale;
     a.part_o = (float *)ws;
     a.part_ml = need ? a.part_o + (size_t)a.pg.rows * heads * a.nsplit * QWEN_HIP_HEAD_DIM : NULL;
-    if (prefill) QK_TRY(qk_paged_prefill_launch(&a, s));
+    if (matrix) QK_TRY(qk_paged_prefill_launch(&a, s));
     else QK_TRY(qk_paged_decode_launch(&a, s));
     if (need) QK_TRY(qk_paged_merge_launch(&a, s));
     return 0;

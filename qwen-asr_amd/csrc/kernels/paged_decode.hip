@@ -6,7 +6,8 @@
 //
 // in one pass over the keys with a running m; a sequence without any gets 0.
 // Bound by the bytes of K and V: every K and V row is read once for all query
-// heads that share it (up to 8 in one block; more take another block's pass).
+// heads that share it (up to 8 in one block; more take another block's pass).  Many
+// heads on a bf16 cache run on the matrix cores instead (csrc/host/paged.c).
 //
 // Block (sequence x kv head x up to 8 heads, split): four waves take the split's
 // keys in turns.  L lanes own one key (128 / L dims a lane, in 8-dim chunks L

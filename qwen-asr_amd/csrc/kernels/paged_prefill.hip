@@ -175,6 +175,11 @@ struct PpShape {
     static constexpr int ROWS = 32 * RB * WR, THREADS = 64 * WR * KG, OCC = 1;
 };
 
+// First row of sequence i (i = n_seqs: the end of the last); without row_start each has one
+__device__ __forceinline__ int pp_begin(const qk_paged &pg, int i) {
+    return pg.row_start ? min(max(pg.row_start[i], 0), pg.rows) : i;
+}
+
 // The tile of block `b`: sequence and first flattened row (a whole wave asks).  Longest
 // first over up to 64 sequences: a tile's level is its last position in steps of 128 keys,
 // and tiles go out by falling level, so the ones that take longest start first (8 prompts
@@ -184,7 +189,7 @@ struct PpShape {
 template <int ROWS>
 __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int slots, int &s, int &f0) {
     const int lane = threadIdx.x & 63;
-    auto begin = [&](int i) { return min(max(pg.row_start[i], 0), pg.rows); };
+    auto begin = [&](int i) { return pp_begin(pg, i); };
     if (pg.n_seqs > 64) {
         const int slot = slots - 1 - b;
         auto first_slot = [&](int i) { return begin(i) * G / ROWS + i; };
@@ -248,7 +253,7 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     const int G = a.heads / pg.kv_heads, kvh = blockIdx.x % pg.kv_heads;
     int s, f0;
     if (!pp_tile<ROWS>(pg, G, (int)(blockIdx.x / pg.kv_heads), slots, s, f0)) return;     // block-uniform, as the next
-    const int r0 = min(max(pg.row_start[s], 0), pg.rows), n = max(min(max(pg.row_start[s + 1], 0), pg.rows) - r0, 0);
+    const int r0 = pp_begin(pg, s), n = max(pp_begin(pg, s + 1) - r0, 0);
     const int frows = n * G;
     if (f0 >= frows) return;
     const int len = pg_len(pg, s);

@@ -92,8 +92,10 @@ class Paged:
         scaling is off by at most g(136) sum |q_d k_d| scale (the products that a split into
         three bf16 terms drops add 4 2^-24 of it: in the 136), the exponential and its argument
         by 4 2^-24 (1 + |s|) of the weight, the sums over n keys by g(n + 8) of their absolute
-        terms each.  bf16 rows of a prefill round each weight by 2^-8.  The result is rounded
-        once more to its type."""
+        terms each.  bf16 rows of a prefill round each weight by 2^-8, and so do single tokens of more
+        than four heads a kv head on a bf16 cache, which run as prompts of one row (all weights of
+        an output are rounded, and nothing else is: sum |dw_j v_j| <= 2^-8 sum w_j |v_j|).  The
+        result is rounded once more to its type."""
         out = torch.full((self.rows, self.heads, HD), 7.0, dtype=torch.float64)
         tol = torch.full_like(out, -1.0)
         e = 2.0 ** -24
@@ -118,7 +120,7 @@ class Paged:
                     n = kk.shape[0]
                     off = 136 * e * (kk.abs() @ q.abs() * scale) + 4 * e * (1 + sc.abs())
                     rel = 2 * off.max() + 2 * (n + 8) * e
-                    if self.act == "bf16" and self.row_start is not None:
+                    if self.act == "bf16" and (self.row_start is not None or self.cache == "bf16" and self.group > 4):
                         rel = rel + 2.0 ** -8
                     out[row, h] = o
                     tol[row, h] = 1.1 * (rel * (w @ vv.abs()) + HALF[self.act] * o.abs()) + 1e-37

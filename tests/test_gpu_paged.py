@@ -358,3 +358,41 @@ def test_same_bits_every_time(qa, gpu):
         first = p.attention(qa, SCALE)
         for _ in range(3):
             assert T.equal(first, p.attention(qa, SCALE))
+
+
+# ---------------------------------------------------------------------------
+# single tokens of many heads a kv head on a bf16 cache: the matrix cores' kernel
+# ---------------------------------------------------------------------------
+MANY = [("bf16", 8), ("f32", 12)]
+
+
+@pytest.mark.parametrize("page", [1, 4, 64, 512])
+@pytest.mark.parametrize("act,group", MANY)
+def test_many_heads_pages(qa, gpu, act, group, page):
+    p = Paged(60, LENS, group=group, kv_heads=1, page=page, act=act, cache="bf16").gpu(qa)
+    check(p.attention(qa, SCALE), *p.reference(SCALE))
+
+
+@pytest.mark.parametrize("act,group", MANY)
+def test_many_heads_many_sequences(qa, gpu, act, group):
+    lens = [(5 * i) % 40 for i in range(150)]
+    p = Paged(61, lens, group=group, kv_heads=2, page=16, act=act, cache="bf16").gpu(qa)
+    check(p.attention(qa, SCALE), *p.reference(SCALE))
+
+
+@pytest.mark.parametrize("act,group", MANY)
+def test_many_heads_missing_pages_and_infinite_values(qa, gpu, act, group):
+    p = Paged(62, [300, 100, 64, 70], group=group, kv_heads=2, page=16, act=act, cache="bf16")
+    p.table[0, :10] = -1
+    p.table[1, 3] = p.n_pages
+    p.table[2, :] = -2 ** 31
+    p.v[p.page_of(3, 20), 0, 20 % 16, 5] = math.inf
+    p.v[p.page_of(3, 60), 1, 60 % 16, 9] = math.nan
+    check(p.gpu(qa).attention(qa, SCALE), *p.reference(SCALE))
+
+
+@pytest.mark.parametrize("act,group", MANY)
+def test_many_heads_any_max_len(qa, gpu, act, group):
+    p = Paged(63, [1, 900, 130, 0], group=group, kv_heads=1, page=32, act=act, cache="bf16").gpu(qa)
+    for max_len in (0, 1, 100, 2 ** 31 - 1):
+        check(p.attention(qa, SCALE, max_len=max_len), *p.reference(SCALE))
