@@ -31,11 +31,23 @@
 // LDS rows are 256 bytes, their 16-byte chunks in an order by row (swz) that
 // keeps both kinds of reads free of bank conflicts.
 //
-// bf16 pages go straight to LDS (two buffers); fp32 pages pass through
-// registers, split on the way (one buffer a block, two blocks a CU).
+// A block is eight waves: two groups of four, every other tile of keys each, joined
+// in LDS at the end.  The second group runs half a turn behind the first, so that on
+// every SIMD one wave's products meet another's softmax.  bf16 pages go straight
+// to LDS (two buffers a group); fp32 pages pass through registers, split on the way.
 //
 // Blocks go out longest first; few rows split the keys over blocks, whose
 // partials paged_merge joins.
+//
+// Measured (8 kv heads, 2 heads each; the card's large bf16 product: 1290 TFLOP/s):
+//   one prompt of 8191 rows, bf16: 311 us, the causal half's products at 880 TFLOP/s; bound by
+//     what a turn of 64 keys reads from LDS and the softmax beside the products (tiles
+//     staged through registers: 1.24 times the time; 64 rows a wave, one wave a SIMD: 2.1;
+//     three buffers, loads among the products: 1.20)
+//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 79 us;
+//     bound by the products, and by what a block does before and behind them
+//     (about 11 us of its 31: tile search, first tiles, join)
+//   31 new rows behind 993, all fp32: 22 us, a chain of first loads and the join's launch
 //
 // Masked keys: a masked score is -inf before the maximum, but 0 times what the
 // cache holds is no number where that is infinite or none.  Such a V
@@ -167,45 +179,55 @@ struct PpTerms {
     static constexpr int N = sizeof(T) == 4 ? 3 : 1;
 };
 
-// RB blocks of 32 rows a wave, WR waves over the rows, KG groups of such waves over the
-// keys (tiles in turn, joined in LDS).
-template <typename T, typename C>
-struct PpShape {
-    static constexpr int RB = 1, WR = 4 / RB, KG = 2;
-    static constexpr int ROWS = 32 * RB * WR, THREADS = 64 * WR * KG, OCC = 1;
-};
+// A block: WR waves over the rows, 32 each, and KG groups of such waves over the keys (tiles in turn,
+// joined in LDS).
+#define PP_WR 4
+#define PP_KG 2
+#define PP_ROWS (32 * PP_WR)
+#define PP_THREADS (64 * PP_WR * PP_KG)
 
 // First row of sequence i (i = n_seqs: the end of the last); without row_start each has one
 __device__ __forceinline__ int pp_begin(const qk_paged &pg, int i) {
     return pg.row_start ? min(max(pg.row_start[i], 0), pg.rows) : i;
 }
 
-// The tile of block `b`: sequence and first flattened row (a whole wave asks).  Longest
-// first over up to 64 sequences: a tile's level is its last position in steps of 128 keys,
-// and tiles go out by falling level, so the ones that take longest start first (8 prompts
-// of 101 .. 1515 rows: see the table of measurements below).  For more sequences, by
-// sequence from the last: tiles of sequence s take the slots from start_s G / ROWS + s on
-// (ceil(n G / ROWS) of them never pass the next sequence's first).
+// The tile of block `b`: its sequence s with rows r0 .. r0 + n - 1 and len cached positions, and
+// its first flattened row f0 (a whole wave asks).  Longest first over up to 64 sequences: a tile's
+// level is its last position in steps of 128 keys, and tiles go out by falling level, so the ones
+// that take longest start first.  For more sequences, by sequence from the last: tiles of
+// sequence s take the slots from start_s G / ROWS + s on (ceil(n G / ROWS) of them never pass the
+// next sequence's first).
+struct PpTile {
+    int s, f0, r0, n, len;
+};
 template <int ROWS>
-__device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int slots, int &s, int &f0) {
+__device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int slots, PpTile &o) {
     const int lane = threadIdx.x & 63;
     auto begin = [&](int i) { return pp_begin(pg, i); };
+    auto take = [&](int s) {
+        o.s = s;
+        o.r0 = begin(s);
+        o.n = max(begin(s + 1) - o.r0, 0);
+        o.len = pg_len(pg, s);
+    };
     if (pg.n_seqs > 64) {
         const int slot = slots - 1 - b;
         auto first_slot = [&](int i) { return begin(i) * G / ROWS + i; };
-        s = __builtin_amdgcn_readfirstlane(pg_search<64>(pg.n_seqs, slot, first_slot));
+        const int s = __builtin_amdgcn_readfirstlane(pg_search<64>(pg.n_seqs, slot, first_slot));
         if (s < 0) return false;
-        f0 = (slot - first_slot(s)) * ROWS;
-        return f0 >= 0;
+        take(s);
+        o.f0 = (slot - (o.r0 * G / ROWS + s)) * ROWS;
+        return o.f0 >= 0;
     }
     if (pg.n_seqs == 1) {
-        s = 0;
-        f0 = ((max(begin(1) - begin(0), 0) * G + ROWS - 1) / ROWS - 1 - b) * ROWS;
-        return f0 >= 0;
+        take(0);
+        o.f0 = ((o.n * G + ROWS - 1) / ROWS - 1 - b) * ROWS;
+        return o.f0 >= 0;
     }
+    const int i = min(lane, pg.n_seqs - 1), r0 = begin(i), end = begin(i + 1), len = pg_len(pg, i);
     const bool on = lane < pg.n_seqs;
-    const int n = on ? max(begin(lane + 1) - begin(lane), 0) : 0;
-    const int tiles = (n * G + ROWS - 1) / ROWS, off = on ? min(max(pg_len(pg, lane) - n, 0), pg.capacity) : 0;
+    const int n = on ? max(end - r0, 0) : 0;
+    const int tiles = (n * G + ROWS - 1) / ROWS, off = on ? min(max(len - n, 0), pg.capacity) : 0;
     // tiles of this lane's sequence at level t or above; counts fit a float exactly
     auto first_at = [&](int t) {
         const long want = ((long)t * 128 - off) * G;
@@ -223,26 +245,26 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
     int upto = mine;                             // inclusive sum over the lanes
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += o;
+        const int v = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += v;
     }
     const unsigned long long past = __ballot(upto > left);
-    s = __builtin_amdgcn_readfirstlane(past ? __builtin_ctzll(past) : 0);
-    const int tile = from + left - (upto - mine);
-    f0 = __builtin_amdgcn_readfirstlane(__shfl(tile, s, 64)) * ROWS;
-    return past != 0 && f0 >= 0;
+    o.s = __builtin_amdgcn_readfirstlane(past ? __builtin_ctzll(past) : 0);
+    o.f0 = __builtin_amdgcn_readlane(from + left - (upto - mine), o.s) * ROWS;
+    o.r0 = __builtin_amdgcn_readlane(r0, o.s);
+    o.n = __builtin_amdgcn_readlane(n, o.s);
+    o.len = __builtin_amdgcn_readlane(len, o.s);
+    return past != 0 && o.f0 >= 0;
 }
 
 // SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions)
 template <typename T, typename C, bool SMALL>
-__global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) void paged_prefill(qk_paged_attn_args a,
-                                                                                                int slots) {
-    constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N;
-    constexpr int RB = PpShape<T, C>::RB, WR = PpShape<T, C>::WR, KG = PpShape<T, C>::KG, ROWS = PpShape<T, C>::ROWS;
+__global__ __launch_bounds__(PP_THREADS) void paged_prefill(qk_paged_attn_args a, int slots) {
+    constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, WR = PP_WR, KG = PP_KG, ROWS = PP_ROWS;
     constexpr bool DIRECT = NK == 1;
     constexpr int NBUF = DIRECT ? 2 : 1;
     constexpr int STAGE = 2 * NK * PP_PLANE;              // bytes of one K and V tile
-    constexpr int JOIN = (KG - 1) * WR * RB * (16384 + 512);
+    constexpr int JOIN = (KG - 1) * WR * (16384 + 512);
     constexpr int BYTES = KG * NBUF * STAGE > JOIN ? KG * NBUF * STAGE : JOIN;
     __shared__ __attribute__((aligned(1024))) unsigned char lds_all[BYTES];
 
@@ -251,12 +273,13 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     const int wave = wid % WR, kg = wid / WR;
     const int ql = lane & 31, hl = lane >> 5;
     const int G = a.heads / pg.kv_heads, kvh = blockIdx.x % pg.kv_heads;
-    int s, f0;
-    if (!pp_tile<ROWS>(pg, G, (int)(blockIdx.x / pg.kv_heads), slots, s, f0)) return;     // block-uniform, as the next
-    const int r0 = pp_begin(pg, s), n = max(pp_begin(pg, s + 1) - r0, 0);
+    PpTile tile;
+    if (!pp_tile<ROWS>(pg, G, (int)(blockIdx.x / pg.kv_heads), slots, tile)) return;      // block-uniform, as the next
+    const int s = __builtin_amdgcn_readfirstlane(tile.s), f0 = __builtin_amdgcn_readfirstlane(tile.f0),
+              r0 = __builtin_amdgcn_readfirstlane(tile.r0), n = __builtin_amdgcn_readfirstlane(tile.n),
+              len = __builtin_amdgcn_readfirstlane(tile.len);
     const int frows = n * G;
     if (f0 >= frows) return;
-    const int len = pg_len(pg, s);
     const int off0 = len - n;                             // position of the sequence's first new row (< 0: sees nothing)
     const int lastf = min(f0 + ROWS, frows) - 1;
     const int kend = min(max(off0 + lastf / G + 1, 0), pg.capacity);
@@ -264,38 +287,25 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     const int chunk = max(a.chunk, (need + PP_KT - 1) / PP_KT * PP_KT), split = blockIdx.y;
     const int k0s = (int)min((long)split * chunk, (long)kend), k1 = (int)min((long)k0s + chunk, (long)kend);
 
-    // this lane's rows
-    int head[RB], qrow[RB], pos[RB];
-    bool on[RB];
-#pragma unroll
-    for (int x = 0; x < RB; x++) {
-        const int f = f0 + 32 * (RB * wave + x) + ql;
-        on[x] = f < frows;
-        const int qi = on[x] ? f / G : 0;
-        head[x] = kvh * G + (on[x] ? f % G : 0);
-        qrow[x] = r0 + qi;
-        pos[x] = on[x] ? off0 + qi : -1;
-    }
-    auto orow = [&](int x) { return (size_t)qrow[x] * a.heads + head[x]; };
+    // this lane's row
+    const int fw = f0 + 32 * wave, f = fw + ql;
+    const bool on = f < frows, wave_on = fw < frows;
+    const int qi = on ? f / G : 0, pos = on ? off0 + qi : -1;
+    const size_t orow = (size_t)(r0 + qi) * a.heads + kvh * G + (on ? f % G : 0);
     if (k0s >= k1 && a.nsplit > 1) {
-#pragma unroll
-        for (int x = 0; x < RB; x++)
-            if (on[x] && hl == 0 && kg == 0) {
-                float *ml = a.part_ml + 2 * (orow(x) * a.nsplit + split);
-                ml[0] = -INFINITY;
-                ml[1] = 0.0f;
-            }
+        if (on && hl == 0 && kg == 0) {
+            float *ml = a.part_ml + 2 * (orow * a.nsplit + split);
+            ml[0] = -INFINITY;
+            ml[1] = 0.0f;
+        }
         return;
     }
-    // the wave's first and last positions (rows do not fall with f)
-    const int fw = f0 + 32 * RB * wave;
-    const bool wave_on = fw < frows;
-    const int pos_lo = off0 + fw / G, pos_hi = off0 + min(fw + 32 * RB - 1, frows - 1) / G;
+    const int pos_lo = off0 + fw / G;                     // the wave's first position (rows do not fall with f)
 
-    bf16x8 q[RB][8][NQ];
+    bf16x8 q[8][NQ];
     const float sc = NQ == 1 ? a.scale * PG_LOG2E : 1.0f;
-    pp_f32x16 o[RB][4];
-    float m[RB], l[RB];
+    pp_f32x16 o[4];
+    float m, l;
 
     // ---- staging: the group's waves take SROWS rows of its tile each; a lane's rows RPL of them ----
     constexpr int SROWS = PP_KT / WR, RSTEP = DIRECT ? 4 : 2, RPL = SROWS / RSTEP;
@@ -309,46 +319,52 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     const int smask = (1 << pg.page_shift) - 1;
     const int *const table = pg.table + (size_t)s * pg.table_stride;
     auto tile_k0 = [&](int t) { return k0s + PP_KT * (KG * t + kg); };
-    // Where the wave's rows of tile t lie.  Pages of at least SROWS positions hold them in one page
-    // (the tiles start at multiples of 32): one offset from the pages' start, without vector
-    // arithmetic.  Rows past the split's end are read at its last key (any row does: their scores
-    // are masked), rows without a page from the first page's start.
+    // Where the wave's rows of tile t lie, and which of its keys are there.  Pages of at least
+    // SROWS positions hold the wave's rows in one page (the tiles start at multiples of 32): one
+    // offset from the pages' start, without vector arithmetic.  Rows past the split's end are
+    // read at its last key (any row does: their scores are masked), rows without a page from the
+    // first page's start.  The page ids come 64 tiles at a time, a lane each: ones that were loaded
+    // every turn would be waited for behind the tiles' loads.  Smaller pages: a lane a key, and
+    // that wait.
     const size_t pstride = ((size_t)pg.kv_heads << pg.page_shift) * ROWB;
     const unsigned char *const pages[2] = {(const unsigned char *)pg.k + ((size_t)kvh << pg.page_shift) * ROWB,
                                            (const unsigned char *)pg.v + ((size_t)kvh << pg.page_shift) * ROWB};
-    auto locate = [&](int t, int i0) {
-        const int at = min(tile_k0(t) + SROWS * wave, k1 - 1);
-        return ((unsigned)i0 < (unsigned)pg.n_pages ? i0 : 0) * pstride + (unsigned)(at & smask) * ROWB;
+    constexpr int PIECES = PP_KT / SROWS;                 // parts of a tile that are in one page each
+    int own_ids = 0, keys_there = 0, ids_at = INT_MIN / 2; // of tiles ids_at + lane: the wave's rows' page, Where.seen
+    auto refill = [&](int t) {
+        ids_at = t;
+        const long kt = min(k0s + (long)PP_KT * (KG * (t + lane) + kg), (long)k1);
+        const int left = k1 - (int)kt;
+        int id[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) id[i] = table[min((int)kt + SROWS * i, k1 - 1) >> pg.page_shift];
+        unsigned there = 0;
+        own_ids = 0;
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const bool page = (unsigned)id[i] < (unsigned)pg.n_pages;
+            there |= page ? ((1u << SROWS) - 1) << (SROWS * i) : 0u;
+            if (i == wave && page) own_ids = id[i];
+        }
+        keys_there = (int)(there & (left >= PP_KT ? ~0u : (1u << left) - 1));
     };
-    // Page ids come 64 tiles at a time, a lane each: one that was loaded every turn would be
-    // waited for behind the tiles' loads.  Where that does not do (smaller pages; a page missing
-    // in the split's range, so that a tile's keys have to be asked one by one) every tile asks
-    // for its 32 keys' pages and waits.
-    int missing = 0;
-    for (int p = (k0s >> pg.page_shift) + (int)threadIdx.x; p <= (k1 - 1) >> pg.page_shift; p += PpShape<T, C>::THREADS)
-        missing |= (unsigned)table[p] >= (unsigned)pg.n_pages;
-    const bool fast = !__syncthreads_or(missing) && !SMALL;
-    int idv = 0, idv_at = INT_MIN / 2;                    // pages of tiles idv_at + lane
     struct Where {
         size_t off;
-        int id;                                           // of key lane % 32, where the tile asked for them
+        int id;                                           // SMALL: of key lane % 32
         unsigned seen;                                    // keys that are there, a bit each
     };
     auto where = [&](int t) {
-        Where w;
-        const int left = k1 - tile_k0(t);
-        w.seen = left >= PP_KT ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-        if (fast) {
-            if (t - idv_at >= 64) {
-                idv_at = t;
-                idv = table[min(min(tile_k0(0), k1 - 1) + (long)KG * PP_KT * (t + lane) + SROWS * wave, (long)k1 - 1) >> pg.page_shift];
-            }
-            w.id = 0;
-            w.off = locate(t, __builtin_amdgcn_readlane(idv, t - idv_at));
-        } else {
+        Where w = {};
+        if constexpr (SMALL) {
+            const int left = k1 - tile_k0(t);
             w.id = table[min(tile_k0(t) + ql, k1 - 1) >> pg.page_shift];
+            w.seen = left >= PP_KT ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
             w.seen &= (unsigned)__ballot((unsigned)w.id < (unsigned)pg.n_pages);
-            w.off = locate(t, __builtin_amdgcn_readlane(w.id, SROWS * wave));
+        } else {
+            if (t - ids_at >= 64) refill(t);
+            const int at = min(tile_k0(t) + SROWS * wave, k1 - 1) & smask;
+            w.off = __builtin_amdgcn_readlane(own_ids, t - ids_at) * pstride + (unsigned)at * ROWB;
+            w.seen = (unsigned)__builtin_amdgcn_readlane(keys_there, t - ids_at);
         }
         return w;
     };
@@ -411,63 +427,68 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     };
 
     // Barriers by hand: behind __syncthreads() the compiler has every LDS read wait for loads
-    // that are still on their way to LDS.  `landed`: this wave's are there but for the last turn's
-    // 2 RPL.
-    auto barrier = [&](bool landed) {
-        if (landed) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * RPL));
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    };
+    // that are still on their way to LDS.
+    auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     const int nt = (k1 - k0s + KG * PP_KT - 1) / (KG * PP_KT);       // tiles of a group
-    pp_f32x16 st[RB];
-    bf16x8 pt[RB][2][NQ];
-    [[maybe_unused]] bf16x8 one[RB][2];
+    pp_f32x16 st;
+    bf16x8 pt[2][NQ];
+    [[maybe_unused]] bf16x8 one[2];
 
     // S^T of the tile in K buffer buf
     auto scores = [&](int buf) {
-#pragma unroll
-        for (int x = 0; x < RB; x++) st[x] = (pp_f32x16){};
+        st = (pp_f32x16){};
 #pragma unroll
         for (int t = 0; t < 8; t++) {
             bf16x8 kf[NK];
 #pragma unroll
             for (int y = 0; y < NK; y++) kf[y] = kfrag(buf, y, t);
-#pragma unroll
-            for (int x = 0; x < RB; x++) st[x] = pp_products<NK, NQ>(kf, q[x][t], st[x]);
+            st = pp_products<NK, NQ>(kf, q[t], st);
         }
     };
-    // The matrix part of a turn: V of one tile and K of the next, product by product in turn (the
-    // scores are one chain of sums), fragments read AHEAD steps before their products.
+    // The matrix part of a turn: V of one tile and K of the next, fragments read AHEAD steps before
+    // their products.  The scores are one chain of sums: products in turn where a step has
+    // few.  Six pairs have K's first, and V's fragments read only a step's length before.
     auto matrix = [&](int vbuf, int kbuf) {
         constexpr int PAIRS = PpPairs<NK, NQ>::N, AHEAD = PAIRS == 1 ? 3 : 1, RING = AHEAD + 1;
+        constexpr bool TURNS = PAIRS < 6;
+        constexpr int VAHEAD = TURNS ? AHEAD : 0, VRING = VAHEAD + 1;
         constexpr auto L = PpPairs<NK, NQ>::make();
-        bf16x8 kf[RING][NK], vf[RING][NK];
-        auto read = [&](int u) {
+        bf16x8 kf[RING][NK], vf[VRING][NK];
+        auto read_k = [&](int u) {
 #pragma unroll
-            for (int y = 0; y < NK; y++) {
-                kf[u % RING][y] = kfrag(kbuf, y, u);
-                vf[u % RING][y] = vfrag(vbuf, y, u & 3, u >> 2);
-            }
+            for (int y = 0; y < NK; y++) kf[u % RING][y] = kfrag(kbuf, y, u);
         };
+        auto read_v = [&](int u) {
 #pragma unroll
-        for (int x = 0; x < RB; x++) st[x] = (pp_f32x16){};
+            for (int y = 0; y < NK; y++) vf[u % VRING][y] = vfrag(vbuf, y, u & 3, u >> 2);
+        };
+        st = (pp_f32x16){};
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) read(u);
+        for (int u = 0; u < AHEAD; u++) {
+            read_k(u);
+            if (VAHEAD) read_v(u);
+        }
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            if (u + AHEAD < 8) read(u + AHEAD);
+            if (u + AHEAD < 8) read_k(u + AHEAD);
+            if (u + VAHEAD < 8) read_v(u + VAHEAD);
 #pragma unroll
-            for (int n = 0; n < PAIRS; n++)
+            for (int n = 0; n < PAIRS; n++) {
+                st = pp_mfma(kf[u % RING][L.a[n]], q[u][L.b[n]], st);
+                if (TURNS) o[u & 3] = pp_mfma(vf[u % VRING][L.a[n]], pt[u >> 2][L.b[n]], o[u & 3]);
+            }
+            if (!TURNS) {
 #pragma unroll
-                for (int x = 0; x < RB; x++) {
-                    st[x] = pp_mfma(kf[u % RING][L.a[n]], q[x][u][L.b[n]], st[x]);
-                    o[x][u & 3] = pp_mfma(vf[u % RING][L.a[n]], pt[x][u >> 2][L.b[n]], o[x][u & 3]);
-                }
+                for (int n = 0; n < PAIRS; n++)
+                    o[u & 3] = pp_mfma(vf[u % VRING][L.a[n]], pt[u >> 2][L.b[n]], o[u & 3]);
+            }
         }
-        __builtin_amdgcn_sched_group_barrier(0x100, 3 * NK * AHEAD, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, (TURNS ? 3 : 1) * NK * AHEAD, 0);
 #pragma unroll
         for (int u = 0; u < 8; u++) {
             if (u + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 3 * NK, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2 * RB * PAIRS, 0);
+            else if (!TURNS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * NK, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * PAIRS, 0);
         }
     };
     // The probabilities of the tile at k0.  The maximum that they are taken against follows the
@@ -475,50 +496,44 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     // for it, and most tiles leave the accumulators alone.
     auto softmax = [&](int k0, unsigned seen, auto guarded) {
         if (seen != 0xffffffffu || k0 + PP_KT - 1 > pos_lo) {                  // wave-uniform
+            const int last = pos - k0;
+            const unsigned bits = (last >= 31 ? seen : last < 0 ? 0u : seen & ((2u << last) - 1)) >> (4 * hl);
 #pragma unroll
-            for (int x = 0; x < RB; x++) {
-                const int last = pos[x] - k0;
-                const unsigned bits = (last >= 31 ? seen : last < 0 ? 0u : seen & ((2u << last) - 1)) >> (4 * hl);
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if ((int)(bits << (31 - 8 * (r / 4) - r % 4)) >= 0) st[x][r] = -INFINITY;
-            }
+            for (int r = 0; r < 16; r++)
+                if ((int)(bits << (31 - 8 * (r / 4) - r % 4)) >= 0) st[r] = -INFINITY;
         }
+        float mx = st[0];
 #pragma unroll
-        for (int x = 0; x < RB; x++) {
-            float mx = st[x][0];
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[r]);
+        float other = mx;
+        swap32(mx, other);
+        mx = fmaxf(mx, other) * sc;
+        if (__any(mx > m + 8.0f)) {
+            const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - pg_ref(mn));
+            m = mn;
+            l *= corr;
 #pragma unroll
-            for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[x][r]);
-            float other = mx;
-            swap32(mx, other);
-            mx = fmaxf(mx, other) * sc;
-            if (__any(mx > m[x] + 8.0f)) {
-                const float mn = fmaxf(m[x], mx), corr = __builtin_amdgcn_exp2f(m[x] - pg_ref(mn));
-                m[x] = mn;
-                l[x] *= corr;
+            for (int d = 0; d < 4; d++) o[d] *= corr;
+        }
+        const float ref = pg_ref(m);
+        float p[16], sum = 0.0f;
 #pragma unroll
-                for (int d = 0; d < 4; d++) o[x][d] *= corr;
-            }
-            const float ref = pg_ref(m[x]);
-            float p[16], sum = 0.0f;
+        for (int r = 0; r < 16; r++) {
+            p[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sc, -ref));
+            sum += p[r];
+        }
+        l += sum;
+        pp_terms8<NQ>(p, pt[0]);
+        pp_terms8<NQ>(p + 8, pt[1]);
+        if constexpr (decltype(guarded)::value) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                p[r] = __builtin_amdgcn_exp2f(fmaf(st[x][r], sc, -ref));
-                sum += p[r];
-            }
-            l[x] += sum;
-            pp_terms8<NQ>(p, pt[x][0]);
-            pp_terms8<NQ>(p + 8, pt[x][1]);
-            if constexpr (decltype(guarded)::value) {
+            for (int j = 0; j < 2; j++) {
+                float v[8];
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = p[8 * j + i] > 0.0f ? 1.0f : 0.0f;
-                    bf16x8 t[1];
-                    pp_terms8<1>(v, t);
-                    one[x][j] = t[0];
-                }
+                for (int i = 0; i < 8; i++) v[i] = p[8 * j + i] > 0.0f ? 1.0f : 0.0f;
+                bf16x8 t[1];
+                pp_terms8<1>(v, t);
+                one[j] = t[0];
             }
         }
     };
@@ -527,26 +542,24 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     // most 32 of them
     auto values_guarded = [&](int buf) {
 #pragma unroll
-        for (int d = 0; d < 4; d++)
+        for (int d = 0; d < 4; d++) {
+            pp_f32x16 cnt = {};
 #pragma unroll
-            for (int x = 0; x < RB; x++) {
-                pp_f32x16 cnt = {};
+            for (int j = 0; j < 2; j++) {
+                bf16x8 vf[NK], cls;
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    bf16x8 vf[NK], cls;
-#pragma unroll
-                    for (int y = NK - 1; y >= 0; y--) vf[y] = pp_finite(vfrag(buf, y, d, j), cls);
-                    o[x][d] = pp_products<NK, NQ>(vf, pt[x][j], o[x][d]);
-                    cnt = pp_mfma(cls, one[x][j], cnt);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int k = (int)cnt[r], pi = k & 63, ni = k >> 6 & 63;
-                    if (k >= 4096 || (pi && ni)) o[x][d][r] = NAN;
-                    else if (k) o[x][d][r] += pi ? INFINITY : -INFINITY;
-                }
+                for (int y = NK - 1; y >= 0; y--) vf[y] = pp_finite(vfrag(buf, y, d, j), cls);
+                o[d] = pp_products<NK, NQ>(vf, pt[j], o[d]);
+                cnt = pp_mfma(cls, one[j], cnt);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int k = (int)cnt[r], pi = k & 63, ni = k >> 6 & 63;
+                if (k >= 4096 || (pi && ni)) o[d][r] = NAN;
+                else if (k) o[d][r] += pi ? INFINITY : -INFINITY;
+            }
+        }
     };
 
     // What a walk begins with: its first tiles on their way.
@@ -554,14 +567,14 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     unsigned seen1 = 0, seen2 = 0;                        // of the next softmax's tile, and of the one behind it
     float4 kr[DIRECT ? 2 : RPL], vr[DIRECT ? 2 : RPL];
     auto prime = [&]() {
-        idv_at = INT_MIN / 2;
+        ids_at = INT_MIN / 2;
         next_v = where(0);
         next_k = where(1);
         seen1 = next_v.seen;
         seen2 = next_k.seen;
         if constexpr (DIRECT) {
             fetch(0, next_v, 0, 0);
-            fetch(1, next_k, 0, 1);
+            if (nt > 1) fetch(1, next_k, 0, 1);
             fetch(0, next_v, 1, 0);
         } else {
             load(0, next_v, 0, kr);
@@ -573,21 +586,18 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
     // part.  Waves in step would leave the matrix cores idle in their vector parts.
     auto walk = [&](auto guarded) {
 #pragma unroll
-        for (int x = 0; x < RB; x++) {
-#pragma unroll
-            for (int d = 0; d < 4; d++) o[x][d] = (pp_f32x16){};
-            m[x] = -INFINITY;
-            l[x] = 0.0f;
-        }
+        for (int d = 0; d < 4; d++) o[d] = (pp_f32x16){};
+        m = -INFINITY;
+        l = 0.0f;
         if (nt == 0) return;                              // block-uniform
         if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         else put(0, kr);
-        barrier(false);
-        if (KG == 2 && kg == 1) barrier(false);
+        barrier();
+        if (kg == 1) barrier();
         for (int i = -1; i < nt; i++) {
             if (wave_on) {
-                // past the last tile the scores are of its last key again, and not used
-                const int vbuf = DIRECT ? i & 1 : 0, kbuf = DIRECT ? (i + 1) & 1 : 0;
+                // past the last tile the scores are of what the buffer held, and not used
+                const int vbuf = i & (NBUF - 1), kbuf = (i + 1) & (NBUF - 1);
                 if constexpr (decltype(guarded)::value) {
                     if (i >= 0) values_guarded(vbuf);
                     scores(kbuf);
@@ -596,18 +606,24 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
                     else scores(kbuf);
                 }
             }
-            barrier(false);
+            barrier();
             const unsigned seen = seen1;
             seen1 = seen2;
             if constexpr (DIRECT) {
                 // over K of tile i + 1 and V of tile i, which are read
                 next_v = next_k;
-                next_k = where(i + 3);
-                seen2 = next_k.seen;
-                fetch(i + 3, next_k, 0, (i + 1) & 1);
-                fetch(i + 2, next_v, 1, i & 1);
+                if (i + 3 < nt) {
+                    next_k = where(i + 3);
+                    seen2 = next_k.seen;
+                    fetch(i + 3, next_k, 0, (i + 1) & 1);
+                }
+                if (i + 2 < nt) fetch(i + 2, next_v, 1, i & 1);
                 if (wave_on && i + 1 < nt) softmax(tile_k0(i + 1), seen, guarded);
-            } else {
+                // the last turn's loads are there
+                if (i + 3 < nt) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * RPL));
+                else if (i + 2 < nt) __builtin_amdgcn_s_waitcnt(vmcnt_imm(RPL));
+                else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            } else if (i + 1 < nt) {
                 if (i >= 0) {
                     next_v = next_k;
                     next_k = where(i + 2);
@@ -615,126 +631,102 @@ __global__ __launch_bounds__((PpShape<T, C>::THREADS), (PpShape<T, C>::OCC)) voi
                 }
                 load(i + 2, next_k, 0, kr);
                 load(i + 1, next_v, 1, vr);
-                if (wave_on && i + 1 < nt) softmax(tile_k0(i + 1), seen, guarded);
+                if (wave_on) softmax(tile_k0(i + 1), seen, guarded);
                 put(0, kr);
                 put(1, vr);
             }
-            barrier(DIRECT);
+            barrier();
         }
-        if (KG == 2 && kg == 0) barrier(false);
-        // nothing may land later: the tiles' memory is used again, and then another block's
-        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        if (kg == 0) barrier();
     };
     if (nt > 0) prime();                                  // block-uniform
 
     // queries: dims 16 t + 8 hl .. + 7; fp32 ones take the scale along
 #pragma unroll
-    for (int x = 0; x < RB; x++)
-#pragma unroll
-        for (int t = 0; t < 8; t++) {
-            const T *qp = (const T *)a.q + orow(x) * PG_HD + 16 * t + 8 * hl;
-            if constexpr (NQ == 1) {
-                q[x][t][0] = *reinterpret_cast<const bf16x8 *>(qp);
-            } else {
-                const float4 x0 = pg_load4(qp), x1 = pg_load4(qp + 4);
-                const float fs = a.scale * PG_LOG2E;
-                const float v[8] = {x0.x * fs, x0.y * fs, x0.z * fs, x0.w * fs, x1.x * fs, x1.y * fs, x1.z * fs, x1.w * fs};
-                pp_terms8<NQ>(v, q[x][t]);
-            }
+    for (int t = 0; t < 8; t++) {
+        const T *qp = (const T *)a.q + orow * PG_HD + 16 * t + 8 * hl;
+        if constexpr (NQ == 1) {
+            q[t][0] = *reinterpret_cast<const bf16x8 *>(qp);
+        } else {
+            const float4 x0 = pg_load4(qp), x1 = pg_load4(qp + 4);
+            const float fs = a.scale * PG_LOG2E;
+            const float v[8] = {x0.x * fs, x0.y * fs, x0.z * fs, x0.w * fs, x1.x * fs, x1.y * fs, x1.z * fs, x1.w * fs};
+            pp_terms8<NQ>(v, q[t]);
         }
+    }
     walk(PpBool<false>());
     float z = 0.0f;
 #pragma unroll
-    for (int x = 0; x < RB; x++)
+    for (int d = 0; d < 4; d++)
 #pragma unroll
-        for (int d = 0; d < 4; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) z = fmaf(o[x][d][r], 0.0f, z);
+        for (int r = 0; r < 16; r++) z = fmaf(o[d][r], 0.0f, z);
     // 0 times what is infinite or no number is none
     if (__syncthreads_or(z != 0.0f)) {
         if (nt > 0) prime();
         walk(PpBool<true>());
-        if constexpr (KG > 1) __syncthreads();
+        __syncthreads();
     }
 
-    float L[RB];
+    float L = l, other = l;
+    swap32(L, other);
+    L += other;
+    // the second group's sums over the buffers that were last read before the barrier
+    float4 *const po = reinterpret_cast<float4 *>(lds_all + wave * 16384) + lane;
+    float2 *const pm = reinterpret_cast<float2 *>(lds_all + WR * 16384 + wave * 512) + lane;
+    if (kg == 1) {
 #pragma unroll
-    for (int x = 0; x < RB; x++) {
-        float u = l[x], v = l[x];
-        swap32(u, v);
-        L[x] = u + v;
-    }
-    if constexpr (KG == 2) {
-        // the second group's sums over the buffers that were last read before the barrier
-#pragma unroll
-        for (int x = 0; x < RB; x++) {
-            float4 *po = reinterpret_cast<float4 *>(lds_all + (wave * RB + x) * 16384) + lane;
-            float2 *pm = reinterpret_cast<float2 *>(lds_all + WR * RB * 16384 + (wave * RB + x) * 512) + lane;
-            if (kg == 1) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int d = i / 4, r = 4 * (i % 4);
-                    po[64 * i] = make_float4(o[x][d][r], o[x][d][r + 1], o[x][d][r + 2], o[x][d][r + 3]);
-                }
-                *pm = make_float2(m[x], L[x]);
-            }
+        for (int i = 0; i < 16; i++) {
+            const int d = i / 4, r = 4 * (i % 4);
+            po[64 * i] = make_float4(o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
         }
-        __syncthreads();
-        if (kg == 1) return;
-#pragma unroll
-        for (int x = 0; x < RB; x++) {
-            const float4 *po = reinterpret_cast<const float4 *>(lds_all + (wave * RB + x) * 16384) + lane;
-            const float2 ml = *(reinterpret_cast<const float2 *>(lds_all + WR * RB * 16384 + (wave * RB + x) * 512) + lane);
-            const float mn = fmaxf(m[x], ml.x), ref = pg_ref(mn);
-            const float c0 = __builtin_amdgcn_exp2f(m[x] - ref), c1 = __builtin_amdgcn_exp2f(ml.x - ref);
-            m[x] = mn;
-            L[x] = fmaf(L[x], c0, ml.y * c1);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int d = i / 4, r = 4 * (i % 4);
-                const float4 v = po[64 * i];
-                o[x][d][r] = fmaf(v.x, c1, o[x][d][r] * c0);
-                o[x][d][r + 1] = fmaf(v.y, c1, o[x][d][r + 1] * c0);
-                o[x][d][r + 2] = fmaf(v.z, c1, o[x][d][r + 2] * c0);
-                o[x][d][r + 3] = fmaf(v.w, c1, o[x][d][r + 3] * c0);
-            }
-        }
+        *pm = make_float2(m, L);
     }
+    __syncthreads();
+    if (kg == 1) return;
+    const float2 ml = *pm;
+    const float mn = fmaxf(m, ml.x), ref = pg_ref(mn);
+    const float c0 = __builtin_amdgcn_exp2f(m - ref), c1 = __builtin_amdgcn_exp2f(ml.x - ref);
+    m = mn;
+    L = fmaf(L, c0, ml.y * c1);
 #pragma unroll
-    for (int x = 0; x < RB; x++) {
-        if (!on[x]) continue;
-        if (a.nsplit == 1) {
-            // 0 only where no key was seen: the largest p is 1
-            const float inv = L[x] == 0.0f ? 0.0f : 1.0f / L[x];
-            T *dst = (T *)a.out + orow(x) * PG_HD + 4 * hl;
+    for (int i = 0; i < 16; i++) {
+        const int d = i / 4, r = 4 * (i % 4);
+        const float4 v = po[64 * i];
+        o[d][r] = fmaf(v.x, c1, o[d][r] * c0);
+        o[d][r + 1] = fmaf(v.y, c1, o[d][r + 1] * c0);
+        o[d][r + 2] = fmaf(v.z, c1, o[d][r + 2] * c0);
+        o[d][r + 3] = fmaf(v.w, c1, o[d][r + 3] * c0);
+    }
+    if (!on) return;
+    if (a.nsplit == 1) {
+        // 0 only where no key was seen: the largest p is at least 2^-8
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        T *dst = (T *)a.out + orow * PG_HD + 4 * hl;
 #pragma unroll
-            for (int d = 0; d < 4; d++)
+        for (int d = 0; d < 4; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    pg_store4(dst + 32 * d + 2 * r, make_float4(o[x][d][r] * inv, o[x][d][r + 1] * inv,
-                                                                o[x][d][r + 2] * inv, o[x][d][r + 3] * inv));
-        } else {
-            const size_t at = orow(x) * a.nsplit + split;
-            float *dst = a.part_o + at * PG_HD + 4 * hl;
+            for (int r = 0; r < 16; r += 4)
+                pg_store4(dst + 32 * d + 2 * r,
+                          make_float4(o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv));
+    } else {
+        const size_t at = orow * a.nsplit + split;
+        float *dst = a.part_o + at * PG_HD + 4 * hl;
 #pragma unroll
-            for (int d = 0; d < 4; d++)
+        for (int d = 0; d < 4; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    *reinterpret_cast<float4 *>(dst + 32 * d + 2 * r) =
-                        make_float4(o[x][d][r], o[x][d][r + 1], o[x][d][r + 2], o[x][d][r + 3]);
-            if (hl == 0) {
-                a.part_ml[2 * at] = m[x];
-                a.part_ml[2 * at + 1] = L[x];
-            }
+            for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<float4 *>(dst + 32 * d + 2 * r) =
+                    make_float4(o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+        if (hl == 0) {
+            a.part_ml[2 * at] = m;
+            a.part_ml[2 * at + 1] = L;
         }
     }
 }
 
-#define PP_PLAN_ROWS 128          // rows of the plan's tiles
-
 extern "C" void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_heads, int max_len, int *nsplit,
                                       int *chunk) {
-    const long tiles = (long)rows * (heads / kv_heads) / PP_PLAN_ROWS + n_seqs;
+    const long tiles = (long)rows * (heads / kv_heads) / PP_ROWS + n_seqs;
     const long blocks = tiles * kv_heads;
     long n = (512 + blocks - 1) / blocks;
     if (n > QK_PAGED_MAX_SPLIT) n = QK_PAGED_MAX_SPLIT;
@@ -748,12 +740,12 @@ extern "C" void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_he
 
 template <typename T, typename C>
 static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
-    using S = PpShape<T, C>;
-    const long slots = (long)a->pg.rows * (a->heads / a->pg.kv_heads) / S::ROWS + a->pg.n_seqs;
-    if (slots * a->pg.kv_heads > 0x7fffffffL) return QWEN_HIP_EINVAL;
-    const dim3 grid((unsigned)(slots * a->pg.kv_heads), (unsigned)a->nsplit);
-    if ((1 << a->pg.page_shift) < PP_KT / S::WR) paged_prefill<T, C, true><<<grid, S::THREADS, 0, s>>>(*a, (int)slots);
-    else paged_prefill<T, C, false><<<grid, S::THREADS, 0, s>>>(*a, (int)slots);
+    const qk_paged &pg = a->pg;
+    const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS + pg.n_seqs;
+    if (slots * pg.kv_heads > 0x7fffffffL) return QWEN_HIP_EINVAL;
+    const dim3 grid((unsigned)(slots * pg.kv_heads), (unsigned)a->nsplit);
+    if ((1 << pg.page_shift) < PP_KT / PP_WR) paged_prefill<T, C, true><<<grid, PP_THREADS, 0, s>>>(*a, (int)slots);
+    else paged_prefill<T, C, false><<<grid, PP_THREADS, 0, s>>>(*a, (int)slots);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }
 
