@@ -479,7 +479,8 @@ int qwen_hip_argmax_matvec_bf16(const float *x, const uint16_t *W_bf16,
  * be captured into a graph; what a call needs besides is in the workspace that
  * the caller passes.  A workspace is free again when the call's kernels have
  * run: calls that may overlap (two streams, two graphs replayed at once) need
- * one each; its contents do not matter.  rows == 0 launches nothing.
+ * one each; its contents do not matter.  No rows or no sequences: nothing to
+ * launch.
  * ------------------------------------------------------------------------ */
 
 /* One layer's cache.  Position p of sequence s is slot p % page_size of page

@@ -70,7 +70,7 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
     if (!q_norm != !k_norm || !cos_vals != !sin_vals) QK_REFUSE("%s: one norm or one rotation table of two", op);
     if (q_norm && !(eps >= 0.0f && eps <= FLT_MAX)) QK_REFUSE("%s: eps %g", op, (double)eps);
     if (n_pos < 0) QK_REFUSE("%s: n_pos %d", op, n_pos);
-    if (batch->rows == 0) return 0;
+    if (batch->rows == 0 || kv->n_seqs == 0) return 0;       /* no row is a sequence's */
     if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
     if (!q_out || !q || !k || !v) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(q_out) || !qk_aligned16(q) || !qk_aligned16(k) || !qk_aligned16(v) || !qk_aligned16(q_norm) ||
@@ -143,7 +143,7 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
     if (prefill && !batch->row_start) QK_REFUSE("%s: no row_start", op);
     if (!prefill && batch->row_start) QK_REFUSE("%s: one row per sequence: row_start has to be NULL", op);
     if (!(scale >= 1e-30f && scale <= 1e30f)) QK_REFUSE("%s: scale %g", op, (double)scale);
-    if (batch->rows == 0) return 0;
+    if (batch->rows == 0 || kv->n_seqs == 0) return 0;       /* no row is a sequence's */
     if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
     if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);

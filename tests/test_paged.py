@@ -108,6 +108,13 @@ def test_no_rows_is_no_call(qa):
     assert qa.lib().qwen_hip_paged_attention_ws_bytes(None, None, 4) == 0
 
 
+def test_no_sequences_is_no_call(qa):
+    """rows of no sequence are left as they are; row_start has one entry then"""
+    for k in (dict(kvd=dict(n_seqs=0), bd=dict(rows=3)), dict(kvd=dict(n_seqs=0), bd=dict(rows=500))):
+        assert append(qa, **k) == 0
+        assert attend(qa, "prefill", **k) == 0
+
+
 def sample(qa, **k):
     d = dict(tokens=P, logits=P, row_stride=1000, rows=2, vocab=1000, temperature=P, top_k=P, top_p=P, min_p=P, u=P,
              ws=P, ws_bytes=1 << 40)
