@@ -363,7 +363,7 @@ __global__ __launch_bounds__(PP_THREADS) void paged_prefill(qk_paged_attn_args a
         } else {
             if (t - ids_at >= 64) refill(t);
             const int at = min(tile_k0(t) + SROWS * wave, k1 - 1) & smask;
-            w.off = __builtin_amdgcn_readlane(own_ids, t - ids_at) * pstride + (unsigned)at * ROWB;
+            w.off = __builtin_amdgcn_readlane(own_ids, t - ids_at) * pstride + (size_t)at * ROWB;
             w.seen = (unsigned)__builtin_amdgcn_readlane(keys_there, t - ids_at);
         }
         return w;

@@ -330,6 +330,39 @@ def test_past_32_bit_offsets(qa, gpu):
     check(out[:1], want[2:], tol[2:])
 
 
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+def test_past_32_bits_in_a_page(qa, gpu, which):
+    """one page of 2^24 positions, the sequence ending where a slot's byte offset has passed 2^32.  Keys
+    and values are 0 but for the last 40 positions, whose scores are near 200: what is before them
+    weighs e^-200 each, so the answer is theirs alone."""
+    page, length, n = 1 << 24, (1 << 23) + 77, 3 if which == "prefill" else 1
+    g = T.Generator().manual_seed(8)
+    k, v = (T.zeros(1, 1, page, HD, device="cuda") for _ in range(2))
+    q = T.randn(1, HD, generator=g).repeat(n, 1)
+    kk = q[:1] * (200 / SCALE / float((q[0] * q[0]).sum())) + 0.05 * T.randn(40, HD, generator=g)
+    vv = T.randn(40, HD, generator=g)
+    k[0, 0, length - 40:length], v[0, 0, length - 40:length] = kk.cuda(), vv.cuda()
+    table, lens = T.zeros(1, 1, dtype=T.int32, device="cuda"), T.tensor([length], dtype=T.int32, device="cuda")
+    start = T.tensor([0, n], dtype=T.int32, device="cuda")
+    kv = qa.PagedKV(k.data_ptr(), v.data_ptr(), table.data_ptr(), qa.ST_F32, 1, page, 1, HD, 1, 1)
+    b = qa.PagedBatch(start.data_ptr() if which == "prefill" else None, lens.data_ptr(), n, length)
+    L, by = qa.lib(), (C.byref(kv), C.byref(b))
+    need = L.qwen_hip_paged_attention_ws_bytes(*by, 1)
+    ws, dq = T.empty(max(need, 16), dtype=T.uint8, device="cuda"), q.cuda()
+    out = T.empty_like(dq)
+    call = getattr(L, "qwen_hip_paged_attention_" + which)
+    qa.check(call(*by, out.data_ptr(), dq.data_ptr(), qa.ST_F32, 1, SCALE, ws.data_ptr(), need, None))
+    T.cuda.synchronize()
+    for i in range(n):
+        see = 40 - (n - 1 - i)
+        x, y, z = kk[:see].double(), vv[:see].double(), q[i].double()
+        sc = x @ z * SCALE
+        w, e = T.softmax(sc, 0), 2.0 ** -24
+        # paged_util's bound; weights of 0 add nothing to the sums, which join 64 splits at most
+        rel = 2 * (136 * e * (x.abs() @ z.abs() * SCALE) + 4 * e * (1 + sc.abs())).max() + 2 * (see + 64 + 8) * e
+        assert bool(((out[i].cpu().double() - w @ y).abs() <= 1.1 * (rel * (w @ y.abs()) + e * (w @ y).abs())).all())
+
+
 def test_two_streams(qa, gpu):
     """two calls that may overlap, on streams of their own with a workspace each"""
     ps = [Paged(70 + i, [900, 33, 500], group=2, kv_heads=2, page=16).gpu(qa) for i in range(2)]

@@ -174,3 +174,34 @@ def test_same_every_time(qa, gpu):
     kw = dict(k=[0, 100] * 16, p=[0.95] * 32, u=rnd(20, 32))
     first = draw(qa, x, **kw)
     assert all(draw(qa, x, **kw) == first for _ in range(3))
+
+
+def test_largest_sizes(qa, gpu):
+    """the largest vocabulary, by the list and (nearly equal logits) by selection; the most rows"""
+    vocab = 1 << 20
+    kw = dict(k=[0, 50], p=[0.9, 0.99], u=rnd(21, 2))
+    check(qa, logits(22, 2, vocab, 3.0), **kw)
+    check(qa, logits(23, 2, vocab, 0.01), k=[0, 700000], p=[0.5, 0.8], u=rnd(24, 2))
+    rows = 1 << 16
+    x = logits(25, rows, 3, 1.0)
+    got, u = draw(qa, x, u=rnd(26, rows)), rnd(26, rows)
+    for r in list(range(0, rows, 997)) + [rows - 1]:
+        assert got[r] in allowed(x[r].double().numpy(), 1.0, 0, 1.0, 0.0, np.float32(u[r]).item())
+    assert set(got) == {0, 1, 2}
+
+
+def test_two_streams(qa, gpu):
+    """two draws that may overlap, a workspace and a stream each"""
+    xs, us = [logits(27 + i, 16, 60000, 2.0) for i in range(2)], [rnd(29 + i, 16) for i in range(2)]
+    p = [0.9] * 16
+    want = [draw(qa, x, p=p, u=u) for x, u in zip(xs, us)]
+    need = qa.lib().qwen_hip_sample_ws_bytes(16, 60000)
+    d = [(x.cuda(), T.tensor(p).cuda(), T.tensor(u).cuda(), T.empty(need, dtype=T.uint8, device="cuda"),
+          T.empty(16, dtype=T.int32, device="cuda"), T.cuda.Stream()) for x, u in zip(xs, us)]
+    T.cuda.synchronize()
+    for _ in range(5):
+        for x, q, u, ws, out, st in d:
+            qa.check(qa.lib().qwen_hip_sample(out.data_ptr(), x.data_ptr(), 60000, 16, 60000, None, None, q.data_ptr(),
+                                              None, u.data_ptr(), ws.data_ptr(), need, st.cuda_stream))
+    T.cuda.synchronize()
+    assert [t[4].cpu().tolist() for t in d] == want
