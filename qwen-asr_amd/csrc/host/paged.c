@@ -101,8 +101,8 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
  * Whether single tokens run on the matrix cores, as prompts of one row do: where many heads share
  * a bf16 cache's rows, the vector units are what bounds the other kernel.  Microseconds, vector
  * kernel against matrix kernel, 24 sequences of 500 to 6001 positions, 8 kv heads:
- *   bf16 rows, 4 heads a kv head: 59, 66; 8: 104, 73; 16: 139, 74
- *   fp32 rows (split into three terms), 8: 104, 101; 16: 139, 123
+ *   bf16 rows, 4 heads a kv head: 59, 66; 8: 104, 59; 16: 139, 60
+ *   fp32 rows (split into three terms), 8: 104, 88; 16: 139, 89
  * 24 sequences of 131 to 530, bf16, 5 heads: 26, 25; 16: 40, 26.  fp32 pages take the matrix
  * kernel longer throughout (8 heads: 138, 234).
  */
@@ -113,8 +113,8 @@ static int tokens_by_matrix(int act_bf16, int cache_bf16, int group) {
 /* splits of an attention call and the workspace it needs */
 static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int *nsplit, int *chunk) {
     if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;
-    if (matrix) qk_paged_prefill_plan(p->rows, p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
-    else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, max_len, nsplit, chunk);
+    if (matrix) qk_paged_prefill_plan(p->rows, p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
+    else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
     if (*nsplit == 1) return 0;
     return (size_t)p->rows * heads * *nsplit * (QWEN_HIP_HEAD_DIM + 2) * sizeof(float);
 }
