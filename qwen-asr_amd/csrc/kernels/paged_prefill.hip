@@ -40,11 +40,11 @@
 // partials paged_merge joins.
 //
 // Measured (8 kv heads, 2 heads each; the card's large bf16 product: 1290 TFLOP/s):
-//   one prompt of 8191 rows, bf16: 311 us, the causal half's products at 880 TFLOP/s; bound by
+//   one prompt of 8191 rows, bf16: 307 us, the causal half's products at 900 TFLOP/s; bound by
 //     what a turn of 64 keys reads from LDS and the softmax beside the products (tiles
 //     staged through registers: 1.24 times the time; 64 rows a wave, one wave a SIMD: 2.1;
 //     three buffers, loads among the products: 1.20)
-//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 79 us;
+//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 72 to 79 us;
 //     bound by the products, and by what a block does before and behind them
 //     (about 11 us of its 31: tile search, first tiles, join)
 //   31 new rows behind 993, all fp32: 22 us, a chain of first loads and the join's launch

@@ -487,7 +487,7 @@ typedef struct {
     const int *row_start;     /* [n_seqs + 1], NULL: row i belongs to sequence i */
     const int *kv_len;        /* [n_seqs] */
     int cache_bf16, n_pages, page_shift, kv_heads, n_seqs, table_stride, rows;
-    int capacity;             /* min(table_stride << page_shift, INT_MAX) */
+    int capacity;             /* min(table_stride << page_shift, 2^30) */
 } qk_paged;
 
 typedef struct {
