@@ -102,9 +102,9 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
  * a bf16 cache's rows, the vector units are what bounds the other kernel.  Microseconds, vector
  * kernel against matrix kernel, 24 sequences of 500 to 6001 positions, 8 kv heads:
  *   bf16 rows, 4 heads a kv head: 59, 59; 8: 104, 59; 16: 138, 61
- *   fp32 rows (split into three terms), 8: 104, 88; 16: 138, 89
+ *   fp32 rows (split into three terms), 8: 99, 88; 16: 138, 89
  * and of 131 to 530: bf16 rows, 5 heads: 22, 21; 16: 32, 22; fp32 rows, 8: 23, 26; 16: 32, 27.
- * fp32 pages take the matrix kernel longer throughout (8 heads: 138, 234).
+ * fp32 pages take the matrix kernel longer throughout (8 heads: 108, 234).
  */
 static int tokens_by_matrix(int act_bf16, int cache_bf16, int group) {
     return cache_bf16 && group > (act_bf16 ? 4 : 8);

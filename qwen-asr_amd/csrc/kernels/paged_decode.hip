@@ -10,50 +10,43 @@
 // heads on a bf16 cache run on the matrix cores instead (csrc/host/paged.c).
 //
 // Block (sequence x kv head x up to 8 heads, split): four waves take the split's
-// keys in turns.  L lanes own one key (128 / L dims a lane, in 8-dim chunks L
-// apart, so that the lanes of a load read whole lines), each such group with
-// statistics of its own, joined at the end: over the wave by halving exchanges,
-// over the waves in LDS.  Fewer lanes a key mean fewer steps of the sum over them
-// and fewer lanes that compute the same exponential, but more registers for
-// queries and outputs: 8 lanes for one or two heads (4 lanes: 68 us against 49 at
-// the second size below), 16 for four and eight.  Loads of a turn (U keys' K and V
-// a group) are all in flight before the first product, the page ids of the next
-// turn before those.
+// keys in turns.  L lanes own one key (128 / L dims a lane, in 16-byte chunks L
+// apart, so that a load of the wave reads whole lines: with 32 bytes a lane, fp32
+// pages took 114 us instead of 84), each such group with statistics of its own, joined
+// at the end: over the wave by halving exchanges, over the waves in LDS.  Fewer lanes
+// a key mean fewer steps of the sum over them and fewer lanes that compute the same
+// exponential, but more registers for queries and outputs.  Loads of a turn (U keys'
+// K and V a group) are all in flight before the first product, the page ids of the
+// next turn before those.  L, U by heads and page type, 24 sequences of 500 to 6001:
+//   1 and 2 heads, bf16: 8, 2 (2 heads: 47 us; 8, 4: 50; 16, 4: 48; 4, 4: 68)
+//   4 heads, bf16: 16, 4 (58 us; 16, 2: 60); fp32 likewise (88; 32, 4: 92)
+//   8 heads: 16, 4 (fp32: 114 us; 16, 2: 118; 32, 4: 136)
 //
-// Measured, kernel and join, 8 kv heads, bf16 cache (a device copy moves 4.8 TB/s):
-//   64 sequences of 31 to 4097 positions, bf16 rows, 2 heads each: 49 us, 4.5 TB/s
-//   3 sequences of 20011 to 32769, fp32 rows, 4 heads each: 67 us, 4.9 TB/s
+// Measured, kernel and join, 8 kv heads (a device copy moves 4.8 TB/s):
+//   64 sequences of 31 to 4097 positions, bf16, 2 heads each: 46.5 us, 4.8 TB/s
+//   3 sequences of 20011 to 32769, fp32 rows on bf16 pages, 4 heads each: 66 us, 4.9 TB/s
+//   24 sequences of 500 to 6001, all fp32, 1 head each: 81 us, 5.3 TB/s; 8 heads: 108 us,
+//     bound by the vector units
 // One short sequence is the time of two launches (11 us).
 #include "paged.h"
 
-// 8 values of a cached row as they lie in memory, widened at their use.  NT: rows that are
-// read once pass by the caches (64 streams, 224 MB of pages: 56 us without, 49 with).
+// 16 bytes of a cached row as they lie in memory, widened at their use.  NT: rows that are
+// read once pass by the caches (64 sequences, 222 MB of pages: 54 us without, 48 with; fp32
+// pages, 24 sequences: 93 and 83).
 typedef uint32_t pd_u32x4 __attribute__((ext_vector_type(4)));
-template <bool NT>
-__device__ __forceinline__ pd_u32x4 pd_load16(const void *p) {
-    const pd_u32x4 *q = (const pd_u32x4 *)p;
-    if constexpr (NT) return __builtin_nontemporal_load(q);
-    else return *q;
-}
 template <typename C>
 struct PdRaw {
-    static constexpr int N = sizeof(C) / 2;
-    pd_u32x4 w[N];
+    static constexpr int N = 16 / sizeof(C);
+    pd_u32x4 w;
     template <bool NT>
     __device__ __forceinline__ void load(const C *p) {
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = pd_load16<NT>((const pd_u32x4 *)p + i);
+        if constexpr (NT) w = __builtin_nontemporal_load((const pd_u32x4 *)p);
+        else w = *(const pd_u32x4 *)p;
     }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = (pd_u32x4){0u, 0u, 0u, 0u};
-    }
-    __device__ __forceinline__ void get(float (&x)[8]) const {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if constexpr (N == 2) x[i] = __uint_as_float(w[i / 4][i % 4]);
-            else x[i] = i % 2 ? bf16_hi(w[0][i / 2]) : bf16_lo(w[0][i / 2]);
-        }
+    __device__ __forceinline__ void zero() { w = (pd_u32x4){0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (N == 4) return __uint_as_float(w[i]);
+        else return i % 2 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
     }
 };
 
@@ -75,7 +68,9 @@ __device__ __forceinline__ int pd_chunk(int len, int chunk, int nsplit) {
 
 template <typename T, typename C, int GT, int L, int U, bool NT>
 __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gchunks) {
-    constexpr int D = PG_HD / L, NC = D / 8, KEYS = 64 / L;      // dims and chunks a lane, keys a wave at once
+    // dims a lane, in NC chunks of 16 bytes (CD dims); keys a wave at once
+    constexpr int D = PG_HD / L, CD = PdRaw<C>::N, NC = D / CD, KEYS = 64 / L;
+    static_assert(NC * CD * L == PG_HD, "lanes a key");
     const qk_paged &pg = a.pg;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % L, grp = lane / L;
     const int G = a.heads / pg.kv_heads;
@@ -100,8 +95,8 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
     // rows of a kv head: page id * rstride + slot (the host has seen that they fit an int)
     const int *const table = pg.table + (size_t)s * pg.table_stride;
     const int rstride = pg.kv_heads << pg.page_shift, smask = (1 << pg.page_shift) - 1;
-    const C *kp = (const C *)pg.k + ((size_t)kvh << pg.page_shift) * PG_HD + 8 * c;
-    const C *vp = (const C *)pg.v + ((size_t)kvh << pg.page_shift) * PG_HD + 8 * c;
+    const C *kp = (const C *)pg.k + ((size_t)kvh << pg.page_shift) * PG_HD + CD * c;
+    const C *vp = (const C *)pg.v + ((size_t)kvh << pg.page_shift) * PG_HD + CD * c;
     constexpr int TURN = KEYS * U;                    // keys of one wave's turn
     int pid[U];
     auto ids = [&](int kb) {
@@ -114,15 +109,16 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
     float q[GT][D];
 #pragma unroll
     for (int g = 0; g < GT; g++) {
-        const T *qp = (const T *)a.q + (qrow + min(g, gn - 1)) * PG_HD + 8 * c;
+        const T *qp = (const T *)a.q + (qrow + min(g, gn - 1)) * PG_HD + CD * c;
         const float f = a.scale * PG_LOG2E;
 #pragma unroll
-        for (int i = 0; i < NC; i++) {
-            const float4 x = pg_load4(qp + 8 * L * i), y = pg_load4(qp + 8 * L * i + 4);
-            float *o = &q[g][8 * i];
-            o[0] = x.x * f; o[1] = x.y * f; o[2] = x.z * f; o[3] = x.w * f;
-            o[4] = y.x * f; o[5] = y.y * f; o[6] = y.z * f; o[7] = y.w * f;
-        }
+        for (int i = 0; i < NC; i++)
+#pragma unroll
+            for (int e = 0; e < CD; e += 4) {
+                const float4 x = pg_load4(qp + CD * L * i + e);
+                float *o = &q[g][CD * i + e];
+                o[0] = x.x * f; o[1] = x.y * f; o[2] = x.z * f; o[3] = x.w * f;
+            }
     }
     float m[GT], l[GT], o[GT * D];
 #pragma unroll
@@ -145,8 +141,8 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
             const size_t row = (unsigned)((page ? pid[u] : 0) * rstride + (min(key, k1 - 1) & smask));
 #pragma unroll
             for (int i = 0; i < NC; i++) {
-                kr[u][i].template load<NT>(kp + row * PG_HD + 8 * L * i);
-                vr[u][i].template load<NT>(vp + row * PG_HD + 8 * L * i);
+                kr[u][i].template load<NT>(kp + row * PG_HD + CD * L * i);
+                vr[u][i].template load<NT>(vp + row * PG_HD + CD * L * i);
             }
         }
         if (kb + 4 * TURN < k1) ids(kb + 4 * TURN);   // the next turn's pages
@@ -156,14 +152,11 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
 #pragma unroll
             for (int g = 0; g < GT; g++) sc[u][g] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NC; i++) {
-                float x[8];
-                kr[u][i].get(x);
+            for (int i = 0; i < NC; i++)
 #pragma unroll
                 for (int g = 0; g < GT; g++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) sc[u][g] = fmaf(q[g][8 * i + e], x[e], sc[u][g]);
-            }
+                    for (int e = 0; e < CD; e++) sc[u][g] = fmaf(q[g][CD * i + e], kr[u][i][e], sc[u][g]);
 #pragma unroll
             for (int g = 0; g < GT; g++) {
                 const float d = group_sum<L>(sc[u][g]);
@@ -210,14 +203,12 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int i = 0; i < NC; i++) {
-                float x[8];
-                vr[u][i].get(x);
+            for (int i = 0; i < NC; i++)
 #pragma unroll
                 for (int g = 0; g < GT; g++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) o[g * D + 8 * i + e] = fmaf(sc[u][g], x[e], o[g * D + 8 * i + e]);
-            }
+                    for (int e = 0; e < CD; e++)
+                        o[g * D + CD * i + e] = fmaf(sc[u][g], vr[u][i][e], o[g * D + CD * i + e]);
     }
 
     // the wave's groups, then the four waves
@@ -238,8 +229,8 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
     pd_gather<GT * D, 32, L>(o, lane, base);
 #pragma unroll
     for (int i = 0; i < GT * D * L / 64; i++) {
-        const int n = base + i, g = n / D, e = n % D;             // dim: chunk e / 8 of this lane's
-        so[wave][g][8 * c + 8 * L * (e / 8) + e % 8] = o[i];
+        const int n = base + i, g = n / D, e = n % D;             // dim: chunk e / CD of this lane's
+        so[wave][g][CD * c + CD * L * (e / CD) + e % CD] = o[i];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < gn * (PG_HD / 4); i += 256) {
@@ -360,10 +351,13 @@ extern "C" void qk_paged_decode_plan(int n_seqs, int heads, int kv_heads, int ca
                                      int *chunk) {
     const int G = heads / kv_heads, gt = decode_gt(G);
     const long blocks = (long)n_seqs * kv_heads * ((G + gt - 1) / gt);
-    // 4096 blocks where there are keys for them (64 sequences of up to 4097, bf16: 48.8 us; 8192: 51.3, 2048: 49.8,
-    // 1024: 71.6), of 128 keys at least (16 sequences of 530, fp32: 17 us; 64 keys: 20), and one where that saves
-    // the join's launch (1 sequence of 300, bf16: 8.7 us against 10.7; fp32: 11.1, 10.7; of 200: 8.5, 11.2)
-    long n = (4096 + blocks - 1) / blocks;
+    // Blocks, where there are keys for them: 8192 of one or two heads (64 sequences of up to 4097, bf16: 46.7 us; 4096:
+    // 48.5, 2048: 58.2), fewer of more, whose joins weigh more (24 of up to 6001, 4 heads, bf16: 58.4 us with 4096,
+    // 60.7 with 8192; 8 heads, fp32: 108 us with 2048, 114 and 125).  Of 128 keys at least (16 sequences of 1000, bf16:
+    // 14.2 us; 64 keys: 17.0), and one where that saves the join's launch (1 sequence of 300, bf16: 8.7 us against
+    // 10.7; fp32: 11.1, 10.7; of 200: 8.5, 11.2).
+    const long target = gt == 8 ? 2048 : gt == 4 ? 4096 : 8192;
+    long n = (target + blocks - 1) / blocks;
     n = n > QK_PAGED_MAX_SPLIT ? QK_PAGED_MAX_SPLIT : n;
     long c = (max_len + n - 1) / n;
     c = (c + 63) / 64 * 64;
@@ -378,8 +372,9 @@ template <typename T, typename C>
 static void decode_dispatch(const qk_paged_attn_args *a, hipStream_t s) {
     const int G = a->heads / a->pg.kv_heads, gt = decode_gt(G), gc = (G + gt - 1) / gt;
     const dim3 grid((unsigned)(a->pg.rows * a->pg.kv_heads * gc), (unsigned)a->nsplit);
-    if (gt == 1) paged_decode<T, C, 1, 8, 4, true><<<grid, 256, 0, s>>>(*a, gc);
-    else if (gt == 2) paged_decode<T, C, 2, 8, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+    constexpr int L = sizeof(C) == 4 ? 16 : 8, U = sizeof(C) == 4 ? 4 : 2;
+    if (gt == 1) paged_decode<T, C, 1, L, U, true><<<grid, 256, 0, s>>>(*a, gc);
+    else if (gt == 2) paged_decode<T, C, 2, L, U, true><<<grid, 256, 0, s>>>(*a, gc);
     else if (gt == 4) paged_decode<T, C, 4, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
     else if (gc == 1) paged_decode<T, C, 8, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
     else paged_decode<T, C, 8, 16, 4, false><<<grid, 256, 0, s>>>(*a, gc);      // every block of heads reads the rows
