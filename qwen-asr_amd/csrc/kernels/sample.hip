@@ -32,8 +32,8 @@
 //
 // Bound by the launches for one row (151936 entries: 4 + 5 + 7 + 7 us), by the arithmetic
 // of the weights for many (about 40 vector instructions each, in hist for every
-// entry, in pick for those kept; 64 rows: 9 + 15 + 20 + 9 us, where one reading of
-// the rows takes 8).
+// entry, in pick for those kept) beside three readings of the rows for many (64 rows:
+// 9 + 15 + 18 + 9 us, where one reading takes 8).
 #include "common.h"
 #include "qk_kernels.h"
 #include "qwen_asr_hip.h"
@@ -340,6 +340,22 @@ __device__ __forceinline__ SmCut sm_cut(const SmPar &p, const unsigned (&n)[SM_P
     return c;
 }
 
+// A logit below which no entry is of a class up to the last one that is kept or listed, or,
+// where all are kept, as likely as min-p asks; -infinity: none is left out.  d = M - l of class B
+// or less has d c scale < B + 1 up to the few roundings of 2^-24 that sm_y makes: a part in 10^5 is
+// more than those.
+__device__ __forceinline__ float sm_cut_logit(const SmPar &p, const SmCut &c) {
+    const int last = max(max(c.lo - 1, c.hi), c.bk);
+    double d;
+    if (last < SM_BINS - 2) d = (double)(last + 1) / ((double)p.scale * (double)p.c);
+    else if (c.lo == SM_BINS && p.lim < INFINITY) d = ((double)p.lim + (double)p.lim_lo) / (double)p.c + 1e-30;
+    else return -INFINITY;
+    const double at = (double)p.M - d * 1.00001;
+    float f = (float)at;
+    if ((double)f > at) f = nextafterf(f, -INFINITY);
+    return f == f ? f : -INFINITY;
+}
+
 __global__ __launch_bounds__(256) void sample_pick(qk_sample_args a, int nb) {
     const int row = blockIdx.x / nb, b = blockIdx.x % nb, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     SmRow &w = ((SmRow *)a.ws)[row];
@@ -381,32 +397,53 @@ __global__ __launch_bounds__(256) void sample_pick(qk_sample_args a, int nb) {
     __shared__ unsigned n, at;
     if (threadIdx.x == 0) n = 0;
     __syncthreads();
-    auto entries = [&](auto min_p) {
-        for (; s < subs; s += nb * 4) {
-            float now[PL];
-#pragma unroll
-            for (int j = 0; j < PL; j++) now[j] = l[j];
-            if (s + nb * 4 < subs) load(s + nb * 4);
-            // With branches: an entry that is not kept costs no weight, which saves more
-            // than 16 unbroken chains overlap (64 rows of 151936: 20.3 us against 25.7).
-            unsigned long long sum = 0;
-#pragma unroll
-            for (int j = 0; j < PL; j++) {
-                const SmY v = sm_y(p, now[j]);
-                if (v.bin < c.lo) {
-                    if (!min_p() || sm_likely(p, v)) sum += sm_weight(v);
-                } else if (v.bin <= c.hi || v.bin == c.bk) {
-                    const unsigned i = atomicAdd(&n, 1u);
-                    if (i < SM_CAND)
-                        list[i] = (unsigned long long)__float_as_uint(now[j]) << 32 | (unsigned)(s * SM_SUB + 64 * j + lane);
-                }
-            }
-            sum = sm_wave_sum(sum);
-            if (lane == 63) w.sub[s] = sum;
+    auto entry = [&](float x, int i, unsigned long long &sum) {
+        const SmY v = sm_y(p, x);
+        if (v.bin < c.lo) {
+            // with a branch: an entry that is not kept costs no weight
+            if (p.lim == INFINITY || sm_likely(p, v)) sum += sm_weight(v);
+        } else if (v.bin <= c.hi || v.bin == c.bk) {
+            const unsigned k = atomicAdd(&n, 1u);
+            if (k < SM_CAND) list[k] = (unsigned long long)__float_as_uint(x) << 32 | (unsigned)i;
         }
     };
-    if (p.lim < INFINITY) entries([] { return true; });
-    else entries([] { return false; });
+    // Logits below `cut` are in no class that is kept or listed.  The others of a partial sum are
+    // packed in LDS first: few lanes of a wave have one, and all would wait for its weight (64 rows,
+    // top-p: 49.7 us for the four launches, 51.8 without).
+    const float cut = sm_cut_logit(p, c);
+    __shared__ float qx[4][SM_SUB];
+    __shared__ unsigned short qi[4][SM_SUB];
+    for (; s < subs; s += nb * 4) {
+        float now[PL];
+#pragma unroll
+        for (int j = 0; j < PL; j++) now[j] = l[j];
+        if (s + nb * 4 < subs) load(s + nb * 4);
+        unsigned long long sum = 0;
+        if (cut == -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < PL; j++) entry(now[j], s * SM_SUB + 64 * j + lane, sum);
+        } else {
+            int len = 0;
+#pragma unroll
+            for (int j = 0; j < PL; j++) {
+                const bool hit = now[j] >= cut;
+                const unsigned long long hits = __ballot(hit);
+                if (hit) {
+                    const int k = len + __popcll(hits & ((1ull << lane) - 1));
+                    qx[wave][k] = now[j];
+                    qi[wave][k] = (unsigned short)(64 * j + lane);
+                }
+                len += __popcll(hits);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            for (int k = lane; k < len; k += 64) entry(qx[wave][k], s * SM_SUB + qi[wave][k], sum);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        sum = sm_wave_sum(sum);
+        if (lane == 63) w.sub[s] = sum;
+    }
     __syncthreads();
     if (n == 0) return;
     if (threadIdx.x == 0) at = atomicAdd(&w.n_cand, n);
