@@ -111,9 +111,10 @@ static int tokens_by_matrix(int act_bf16, int cache_bf16, int group) {
 }
 
 /* splits of an attention call and the workspace it needs */
-static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int *nsplit, int *chunk) {
+static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int *rows2, int *nsplit, int *chunk) {
     if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;
-    if (matrix) qk_paged_prefill_plan(p->rows, p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
+    *rows2 = 0;
+    if (matrix) *rows2 = qk_paged_prefill_plan(p, heads, max_len, nsplit, chunk);
     else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
     if (*nsplit == 1) return 0;
     return (size_t)p->rows * heads * *nsplit * (QWEN_HIP_HEAD_DIM + 2) * sizeof(float);
@@ -121,14 +122,14 @@ static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_l
 
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
-    int nsplit, chunk;
+    int rows2, nsplit, chunk;
     if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || p.rows == 0) return 0;
     const int group = heads / p.kv_heads;
     size_t need = 0;
     /* of either type of rows */
     for (int bf16 = 0; bf16 <= 1; bf16++) {
         const int matrix = p.row_start || tokens_by_matrix(bf16, p.cache_bf16, group);
-        const size_t n = attention_plan(&p, matrix, heads, batch->max_len, &nsplit, &chunk);
+        const size_t n = attention_plan(&p, matrix, heads, batch->max_len, &rows2, &nsplit, &chunk);
         need = n > need ? n : need;
     }
     return need;
@@ -149,7 +150,7 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);
     if (out == q) QK_REFUSE("%s: out cannot be q", op);
     const int matrix = prefill || tokens_by_matrix(dtype == QWEN_HIP_ST_BF16, a.pg.cache_bf16, heads / a.pg.kv_heads);
-    const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, &a.nsplit, &a.chunk);
+    const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, &a.rows2, &a.nsplit, &a.chunk);
     if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);
     a.out = out;

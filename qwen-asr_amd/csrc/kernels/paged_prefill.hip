@@ -181,10 +181,9 @@ struct PpTerms {
 
 // A block: WR waves over the rows, 32 each, and KG groups of such waves over the keys (tiles in turn,
 // joined in LDS).
-#define PP_WR 4
 #define PP_KG 2
-#define PP_ROWS (32 * PP_WR)
-#define PP_THREADS (64 * PP_WR * PP_KG)
+#define PP_ROWS(WR) (32 * (WR))
+#define PP_THREADS(WR) (64 * (WR) * PP_KG)
 
 // First row of sequence i (i = n_seqs: the end of the last); without row_start each has one
 __device__ __forceinline__ int pp_begin(const qk_paged &pg, int i) {
@@ -258,9 +257,9 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
 }
 
 // SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions)
-template <typename T, typename C, bool SMALL>
-__global__ __launch_bounds__(PP_THREADS) void paged_prefill(qk_paged_attn_args a, int slots) {
-    constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, WR = PP_WR, KG = PP_KG, ROWS = PP_ROWS;
+template <typename T, typename C, bool SMALL, int WR>
+__global__ __launch_bounds__(PP_THREADS(WR), 2) void paged_prefill(qk_paged_attn_args a, int slots) {
+    constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, KG = PP_KG, ROWS = PP_ROWS(WR);
     constexpr bool DIRECT = NK == 1;
     constexpr int NBUF = DIRECT ? 2 : 1;
     constexpr int STAGE = 2 * NK * PP_PLANE;              // bytes of one K and V tile
@@ -727,38 +726,46 @@ __global__ __launch_bounds__(PP_THREADS) void paged_prefill(qk_paged_attn_args a
     }
 }
 
-extern "C" void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_heads, int cache_bf16, int max_len,
-                                      int *nsplit, int *chunk) {
-    const long tiles = (long)rows * (heads / kv_heads) / PP_ROWS + n_seqs;
-    const long blocks = tiles * kv_heads;
-    // A CU runs one block at a time: 1.5 blocks each (24 single tokens of 500 to 6001 positions, 8 heads a kv
-    // head, bf16: 59 us, as with 256 blocks; 512: 73; 4 chunks of 30 rows behind 1970, bf16: 17.8, 18.2, 21.7;
-    // behind 970, fp32: 29.0, 31.9, 28.7)
-    long n = (384 + blocks - 1) / blocks;
+extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk) {
+    const long f = (long)p->rows * (heads / p->kv_heads);
+    // Blocks of 64 rows run two to a CU, one's begin and end beside the other's products, but read every key twice as
+    // often; on fp32 pages their tiles do not fit LDS twice.  bf16, 128 and 64 rows: 16 prompts of 300 to 1000, 151 and
+    // 141 us; 8 of 60 to 400, 28 and 19; 24 single tokens of 131 to 530, 8 heads a kv head, 21 and 15; but 4 prompts
+    // of 1000 to 4000, 300 and 310, one of 8191, 303 and 338.  Where the keys are split, up to 768: 4 chunks of 30 rows
+    // on fp32 rows, 500 positions, 17.3 and 16.5; 1000, 18.6 and 20.3.
+    const int rows2 = p->cache_bf16 && p->page_shift >= 4 &&
+                      max_len <= ((f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 2048 : 768);
+    const long blocks = (f / PP_ROWS(rows2 ? 2 : 4) + p->n_seqs) * p->kv_heads;
+    // 1.5 blocks of 128 rows for each CU (24 single tokens of 500 to 6001 positions, 8 heads a kv head, bf16: 59 us, as
+    // with 256 blocks; 512: 73; 4 chunks of 30 rows behind 970, fp32: 29.0, 31.9, 28.7), 1.25 of 64 (4 chunks of 30
+    // rows behind 470, bf16: 13.6 us, as with 256 blocks; 512: 14.8)
+    long n = ((rows2 ? 320 : 384) + blocks - 1) / blocks;
     if (n > QK_PAGED_MAX_SPLIT) n = QK_PAGED_MAX_SPLIT;
     long c = (max_len + n - 1) / n;
     c = (c + 63) / 64 * 64;
     if (c < 64) c = 64;
     // one block where that saves the join's launch (30 rows, 100 positions: bf16 9.4 us against 11.7, fp32 rows 12.1
     // against 13.4, but on an fp32 cache 20.1 against 19.2; 130 positions, fp32 rows: 13.9, 13.6)
-    if (cache_bf16 && max_len <= 128) c = 128;
+    if (p->cache_bf16 && max_len <= 128) c = 128;
     n = (max_len + c - 1) / c;
     *nsplit = n < 1 ? 1 : (int)n;
     *chunk = (int)c;
+    return rows2;
 }
 
-template <typename T, typename C>
+template <typename T, typename C, int WR>
 static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     const qk_paged &pg = a->pg;
-    const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS + pg.n_seqs;
+    const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS(WR) + pg.n_seqs;
     if (slots * pg.kv_heads > 0x7fffffffL) return QWEN_HIP_EINVAL;
     const dim3 grid((unsigned)(slots * pg.kv_heads), (unsigned)a->nsplit);
-    if ((1 << pg.page_shift) < PP_KT / PP_WR) paged_prefill<T, C, true><<<grid, PP_THREADS, 0, s>>>(*a, (int)slots);
-    else paged_prefill<T, C, false><<<grid, PP_THREADS, 0, s>>>(*a, (int)slots);
+    if ((1 << pg.page_shift) < PP_KT / WR) paged_prefill<T, C, true, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
+    else paged_prefill<T, C, false, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }
 
 extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
-    if (a->act_bf16) return a->pg.cache_bf16 ? prefill_launch<uint16_t, uint16_t>(a, s) : prefill_launch<uint16_t, float>(a, s);
-    return a->pg.cache_bf16 ? prefill_launch<float, uint16_t>(a, s) : prefill_launch<float, float>(a, s);
+    if (!a->pg.cache_bf16) return a->act_bf16 ? prefill_launch<uint16_t, float, 4>(a, s) : prefill_launch<float, float, 4>(a, s);
+    if (a->rows2) return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 2>(a, s) : prefill_launch<float, uint16_t, 2>(a, s);
+    return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 4>(a, s) : prefill_launch<float, uint16_t, 4>(a, s);
 }

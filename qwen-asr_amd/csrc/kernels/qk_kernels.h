@@ -510,14 +510,15 @@ typedef struct {
     const void *q;
     int act_bf16, heads;
     float scale;
+    int rows2;                /* prompts: blocks of 64 rows instead of 128 */
     int nsplit, chunk;        /* keys per split, unless a sequence is longer than nsplit of them */
     float *part_o, *part_ml;  /* nsplit > 1 */
 } qk_paged_attn_args;
 #define QK_PAGED_MAX_SPLIT 64
 /* splits and keys per split for sequences of up to max_len positions */
 void qk_paged_decode_plan(int n_seqs, int heads, int kv_heads, int cache_bf16, int max_len, int *nsplit, int *chunk);
-void qk_paged_prefill_plan(int rows, int n_seqs, int heads, int kv_heads, int cache_bf16, int max_len, int *nsplit,
-                           int *chunk);
+/* returns qk_paged_attn_args.rows2 */
+int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk);
 int qk_paged_decode_launch(const qk_paged_attn_args *a, hipStream_t s);
 int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s);
 /* joins the partials into out */

@@ -429,3 +429,27 @@ def test_many_heads_any_max_len(qa, gpu, act, group):
     p = Paged(63, [1, 900, 130, 0], group=group, kv_heads=1, page=32, act=act, cache="bf16").gpu(qa)
     for max_len in (0, 1, 100, 2 ** 31 - 1):
         check(p.attention(qa, SCALE, max_len=max_len), *p.reference(SCALE))
+
+
+# ---------------------------------------------------------------------------
+# prompts: both block shapes (max_len decides), and walks longer than 64 tiles
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("max_len", [64, 700, 900, 5000])
+@pytest.mark.parametrize("page", [2, 8, 16, 32])
+def test_prefill_block_shapes(qa, gpu, act, max_len, page):
+    """rows and infinite values of every block shape on bf16 pages, a page missing"""
+    p = Paged(67, [1, 70, 33, 190, 64, 150], new=[1, 70, 0, 131, 2, 97], group=2, kv_heads=2, page=page, act=act,
+              cache="bf16", front=3, back=5)
+    p.table[3, 64 // page] = p.n_pages
+    p.v[p.page_of(5, 80), 1, 80 % page, 9] = math.inf
+    p.v[p.page_of(5, 130), 1, 130 % page, 9] = math.nan
+    check(p.gpu(qa).attention(qa, SCALE, max_len=max_len), *p.reference(SCALE))
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_prefill_long_walk(qa, gpu, act, cache):
+    """one block walks 9000 keys: the page ids are read more than once"""
+    p = Paged(68, [9000], new=[3], group=2, kv_heads=1, page=16, act=act, cache=cache)
+    p.table[0, 300] = -1
+    check(p.gpu(qa).attention(qa, SCALE, max_len=64), *p.reference(SCALE))
