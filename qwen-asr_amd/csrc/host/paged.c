@@ -100,15 +100,13 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
 /*
  * Whether single tokens run on the matrix cores, as prompts of one row do: where many heads share
  * a bf16 cache's rows, the vector units are what bounds the other kernel.  Microseconds, vector
- * kernel against matrix kernel, 24 sequences of 500 to 6001 positions, 8 kv heads:
- *   bf16 rows, 4 heads a kv head: 59, 59; 8: 104, 59; 16: 138, 61
- *   fp32 rows (split into three terms), 8: 99, 88; 16: 138, 89
- * and of 131 to 530: bf16 rows, 5 heads: 22, 21; 16: 32, 22; fp32 rows, 8: 23, 26; 16: 32, 27.
+ * kernel against matrix kernel, 8 kv heads, 24 sequences of 500 to 6001 positions:
+ *   bf16 rows, 2 heads a kv head: 48, 58; 4: 59, 59; 8: 98, 59; 16: 141, 61
+ *   fp32 rows (split into three terms), 4: 59, 89; 8: 98, 89; 16: 141, 90
+ * and of 131 to 530: bf16 rows, 2: 12, 15; 4: 15, 15; 5: 23, 15; fp32 rows, 4: 15, 19; 8: 23, 20.
  * fp32 pages take the matrix kernel longer throughout (8 heads: 108, 234).
  */
-static int tokens_by_matrix(int act_bf16, int cache_bf16, int group) {
-    return cache_bf16 && group > (act_bf16 ? 4 : 8);
-}
+static int tokens_by_matrix(int cache_bf16, int group) { return cache_bf16 && group > 4; }
 
 /* splits of an attention call and the workspace it needs */
 static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int *rows2, int *nsplit, int *chunk) {
@@ -124,15 +122,8 @@ size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen
     qk_paged p;
     int rows2, nsplit, chunk;
     if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || p.rows == 0) return 0;
-    const int group = heads / p.kv_heads;
-    size_t need = 0;
-    /* of either type of rows */
-    for (int bf16 = 0; bf16 <= 1; bf16++) {
-        const int matrix = p.row_start || tokens_by_matrix(bf16, p.cache_bf16, group);
-        const size_t n = attention_plan(&p, matrix, heads, batch->max_len, &rows2, &nsplit, &chunk);
-        need = n > need ? n : need;
-    }
-    return need;
+    const int matrix = p.row_start || tokens_by_matrix(p.cache_bf16, heads / p.kv_heads);
+    return attention_plan(&p, matrix, heads, batch->max_len, &rows2, &nsplit, &chunk);
 }
 
 static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch,
@@ -149,7 +140,7 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
     if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);
     if (out == q) QK_REFUSE("%s: out cannot be q", op);
-    const int matrix = prefill || tokens_by_matrix(dtype == QWEN_HIP_ST_BF16, a.pg.cache_bf16, heads / a.pg.kv_heads);
+    const int matrix = prefill || tokens_by_matrix(a.pg.cache_bf16, heads / a.pg.kv_heads);
     const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, &a.rows2, &a.nsplit, &a.chunk);
     if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);

@@ -21,7 +21,7 @@
 // B[8 hl + i][l & 31], i = 0..7, and holds D[8 (r / 4) + 4 hl + r % 4][l & 31],
 // r = 0..15.  The rows of a kv head's query heads are flattened, row f = query
 // f / G, head f % G, so a few queries of many heads fill a tile as well; a wave
-// owns 32 of them, a block 128 of one sequence.  Per tile of 32 keys:
+// owns 32 of them, a block 64 or 128 of one sequence.  Per tile of 32 keys:
 //   S^T = K Q^T      A = K rows from LDS, B = the wave's queries, in registers;
 //   softmax          a row lives in the two lanes l, l ^ 32;
 //   O^T += V^T P^T   B = the probabilities where S^T left them: k slot 8 hl + i
@@ -31,10 +31,12 @@
 // LDS rows are 256 bytes, their 16-byte chunks in an order by row (swz) that
 // keeps both kinds of reads free of bank conflicts.
 //
-// A block is eight waves: two groups of four, every other tile of keys each, joined
-// in LDS at the end.  The second group runs half a turn behind the first, so that on
-// every SIMD one wave's products meet another's softmax.  bf16 pages go straight
-// to LDS (two buffers a group); fp32 pages pass through registers, split on the way.
+// A block is two groups of waves, every other tile of keys each, joined in LDS at the
+// end: groups of four (128 rows), or of two (64 rows) where that is the faster (see the
+// plan).  The second group runs half a turn behind the first, so that with four waves
+// each SIMD has one wave's products beside another's softmax; of 64-row blocks a CU
+// runs two.  bf16 pages go straight to LDS (two buffers a group); fp32 pages pass
+// through registers, split on the way.
 //
 // Blocks go out longest first; few rows split the keys over blocks, whose
 // partials paged_merge joins.
