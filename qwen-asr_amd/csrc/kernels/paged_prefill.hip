@@ -260,7 +260,7 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
 
 // SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions)
 template <typename T, typename C, bool SMALL, int WR>
-__global__ __launch_bounds__(PP_THREADS(WR), 2) void paged_prefill(qk_paged_attn_args a, int slots) {
+__global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) void paged_prefill(qk_paged_attn_args a, int slots) {
     constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, KG = PP_KG, ROWS = PP_ROWS(WR);
     constexpr bool DIRECT = NK == 1;
     constexpr int NBUF = DIRECT ? 2 : 1;
@@ -731,12 +731,15 @@ __global__ __launch_bounds__(PP_THREADS(WR), 2) void paged_prefill(qk_paged_attn
 extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk) {
     const long f = (long)p->rows * (heads / p->kv_heads);
     // Blocks of 64 rows run two to a CU, one's begin and end beside the other's products, but read every key twice as
-    // often; on fp32 pages their tiles do not fit LDS twice.  bf16, 128 and 64 rows: 16 prompts of 300 to 1000, 151 and
+    // often.  bf16, 128 and 64 rows: 16 prompts of 300 to 1000, 151 and
     // 141 us; 8 of 60 to 400, 28 and 19; 24 single tokens of 131 to 530, 8 heads a kv head, 21 and 15; but 4 prompts
     // of 1000 to 4000, 300 and 310, one of 8191, 303 and 338.  Where the keys are split, up to 768: 4 chunks of 30 rows
-    // on fp32 rows, 500 positions, 17.3 and 16.5; 1000, 18.6 and 20.3.
-    const int rows2 = p->cache_bf16 && p->page_shift >= 4 &&
-                      max_len <= ((f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 2048 : 768);
+    // on fp32 rows, 500 positions, 17.3 and 16.5; 1000, 18.6 and 20.3.  On fp32 pages their tiles do not fit LDS twice,
+    // but sequences of no more rows leave half of a larger block's waves idle, and one wave a SIMD has the registers
+    // for six products without spills (fp32 rows, 31 behind 993: 22.4 and 19.8 us; 16 of 16 to 31 behind up to 600,
+    // 46.7 and 35.8).
+    const int fits = (f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 2048 : 768;
+    const int rows2 = p->page_shift >= 4 && (p->cache_bf16 ? max_len <= fits : f <= PP_ROWS(2) * (long)p->n_seqs);
     const long blocks = (f / PP_ROWS(rows2 ? 2 : 4) + p->n_seqs) * p->kv_heads;
     // 1.5 blocks of 128 rows for each CU (24 single tokens of 500 to 6001 positions, 8 heads a kv head, bf16: 59 us, as
     // with 256 blocks; 512: 73; 4 chunks of 30 rows behind 970, fp32: 29.0, 31.9, 28.7), 1.25 of 64 (4 chunks of 30
@@ -767,7 +770,10 @@ static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
 }
 
 extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
-    if (!a->pg.cache_bf16) return a->act_bf16 ? prefill_launch<uint16_t, float, 4>(a, s) : prefill_launch<float, float, 4>(a, s);
+    if (!a->pg.cache_bf16) {
+        if (a->act_bf16) return prefill_launch<uint16_t, float, 4>(a, s);        // 31 rows behind 600: 64 rows a block 16.4 us, 15.0
+        return a->rows2 ? prefill_launch<float, float, 2>(a, s) : prefill_launch<float, float, 4>(a, s);
+    }
     if (a->rows2) return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 2>(a, s) : prefill_launch<float, uint16_t, 2>(a, s);
     return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 4>(a, s) : prefill_launch<float, uint16_t, 4>(a, s);
 }

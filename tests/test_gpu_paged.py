@@ -453,3 +453,15 @@ def test_prefill_long_walk(qa, gpu, act, cache):
     p = Paged(68, [9000], new=[3], group=2, kv_heads=1, page=16, act=act, cache=cache)
     p.table[0, 300] = -1
     check(p.gpu(qa).attention(qa, SCALE, max_len=64), *p.reference(SCALE))
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("page", [2, 8, 16, 64])
+def test_prefill_short_chunks(qa, gpu, act, cache, page):
+    """a few rows each behind pasts, split and unsplit, with what the masks leave out undefined"""
+    p = Paged(69, [500, 33, 129, 0, 64], new=[31, 2, 17, 0, 12], group=2, kv_heads=2, page=page, act=act, cache=cache, front=1)
+    p.table[0, 96 // page] = -7
+    p.v[p.page_of(2, 118), 1, 118 % page, 9] = -math.inf
+    p.gpu(qa)
+    for max_len in (64, 500, 3000):
+        check(p.attention(qa, SCALE, max_len=max_len), *p.reference(SCALE))
