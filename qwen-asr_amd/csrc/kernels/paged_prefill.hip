@@ -46,10 +46,10 @@
 //     what a turn of 64 keys reads from LDS and the softmax beside the products (tiles
 //     staged through registers: 1.24 times the time; 64 rows a wave, one wave a SIMD: 2.1;
 //     three buffers, loads among the products: 1.20)
-//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 72 to 79 us;
+//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 71 to 76 us;
 //     bound by the products, and by what a block does before and behind them
 //     (about 11 us of its 31: tile search, first tiles, join)
-//   31 new rows behind 993, all fp32: 22 us, a chain of first loads and the join's launch
+//   31 new rows behind 993, all fp32: 19.4 us, a chain of first loads and the join's launch
 //
 // Masked keys: a masked score is -inf before the maximum, but 0 times what the
 // cache holds is no number where that is infinite or none.  Such a V
