@@ -376,13 +376,16 @@ static void decode_dispatch(const qk_paged_attn_args *a, hipStream_t s) {
     if (gt == 1) paged_decode<T, C, 1, L, U, true><<<grid, 256, 0, s>>>(*a, gc);
     else if (gt == 2) paged_decode<T, C, 2, L, U, true><<<grid, 256, 0, s>>>(*a, gc);
     else if (gt == 4) paged_decode<T, C, 4, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
-    else if (gc == 1) paged_decode<T, C, 8, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
-    else paged_decode<T, C, 8, 16, 4, false><<<grid, 256, 0, s>>>(*a, gc);      // every block of heads reads the rows
+    else if constexpr (sizeof(C) == 4) {              // more than four heads on bf16 pages do not come here
+        if (gc == 1) paged_decode<T, C, 8, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+        else paged_decode<T, C, 8, 16, 4, false><<<grid, 256, 0, s>>>(*a, gc);  // every block of heads reads the rows
+    }
 }
 
 extern "C" int qk_paged_decode_launch(const qk_paged_attn_args *a, hipStream_t s) {
     const int G = a->heads / a->pg.kv_heads, gt = decode_gt(G);
     if ((long)a->pg.rows * a->pg.kv_heads * ((G + gt - 1) / gt) > 0x7fffffffL) return QWEN_HIP_EINVAL;
+    if (a->pg.cache_bf16 && gt == 8) return QWEN_HIP_EINVAL;
     if (a->act_bf16) {
         if (a->pg.cache_bf16) decode_dispatch<uint16_t, uint16_t>(a, s);
         else decode_dispatch<uint16_t, float>(a, s);

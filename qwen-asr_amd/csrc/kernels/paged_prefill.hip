@@ -258,7 +258,8 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
     return past != 0 && o.f0 >= 0;
 }
 
-// SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions)
+// SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions).  Two waves a SIMD, but for
+// 64-row blocks on fp32 pages, which LDS lets only one of onto a CU.
 template <typename T, typename C, bool SMALL, int WR>
 __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) void paged_prefill(qk_paged_attn_args a, int slots) {
     constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, KG = PP_KG, ROWS = PP_ROWS(WR);
@@ -764,7 +765,10 @@ static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS(WR) + pg.n_seqs;
     if (slots * pg.kv_heads > 0x7fffffffL) return QWEN_HIP_EINVAL;
     const dim3 grid((unsigned)(slots * pg.kv_heads), (unsigned)a->nsplit);
-    if ((1 << pg.page_shift) < PP_KT / WR) paged_prefill<T, C, true, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
+    // the plan takes 64 rows for pages of 16 positions and more
+    constexpr bool SOME_SMALL = WR == 4;
+    if (SOME_SMALL && (1 << pg.page_shift) < PP_KT / WR)
+        paged_prefill<T, C, SOME_SMALL, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
     else paged_prefill<T, C, false, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }
