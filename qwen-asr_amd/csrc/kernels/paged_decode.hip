@@ -18,7 +18,8 @@
 // exponential, but more registers for queries and outputs.  Loads of a turn (U keys'
 // K and V a group) are all in flight before the first product, the page ids of the
 // next turn before those.  L, U by heads and page type, 24 sequences of 500 to 6001:
-//   1 and 2 heads, bf16: 8, 2 (2 heads: 47 us; 8, 4: 50; 16, 4: 48; 4, 4: 68)
+//   1 and 2 heads, bf16: 8, 2 (2 heads: 47 us; 8, 4: 50; 16, 4: 48; 4, 4: 68); fp32: 16, 4
+//     (84 us; 8, 4: 86; 16, 2: 85)
 //   4 heads, bf16: 16, 4 (58 us; 16, 2: 60); fp32 likewise (88; 32, 4: 92)
 //   8 heads: 16, 4 (fp32: 114 us; 16, 2: 118; 32, 4: 136)
 //
