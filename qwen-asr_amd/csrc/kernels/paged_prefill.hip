@@ -14,8 +14,10 @@
 // queries the probabilities are split as well, so such a call is as exact as fp32
 // products (3 matrix products a pair on a bf16 cache, 6 on an fp32 one, against
 // 16 times the time of one on the fp32 matrix cores).  With bf16 queries the
-// probabilities are rounded to bf16 (half a step is 2^-9 of each, as for the
-// result itself).
+// probabilities are held in two terms, each rounded to nearest even (2^-17 of them), and
+// so are fp32 values (the upper two of their three): one term alone is off by as much as
+// the result's own rounding, 1.3 to 1.4 times the error of an fp32 softmax rounded once
+// (8191 rows: 0.0021 and 0.0016 of the result's norm; 306 us with one, 392 with two).
 //
 // Layout.  Lane l (hl = l >> 5) of the MFMA supplies A[l & 31][8 hl + i] and
 // B[8 hl + i][l & 31], i = 0..7, and holds D[8 (r / 4) + 4 hl + r % 4][l & 31],
@@ -42,10 +44,10 @@
 // partials paged_merge joins.
 //
 // Measured (8 kv heads, 2 heads each; the card's large bf16 product: 1290 TFLOP/s):
-//   one prompt of 8191 rows, bf16: 307 us, the causal half's products at 900 TFLOP/s; bound by
-//     what a turn of 64 keys reads from LDS and the softmax beside the products (tiles
-//     staged through registers: 1.24 times the time; 64 rows a wave, one wave a SIMD: 2.1;
-//     three buffers, loads among the products: 1.20)
+//   one prompt of 8191 rows, bf16: 392 us, the causal half's products (three for two, by the
+//     probabilities' second term) at 1050 TFLOP/s; bound by them and the softmax beside them
+//     (with one term, in 306 us, tiles staged through registers took 1.24 times the time; 64
+//     rows a wave, one wave a SIMD: 2.1; three buffers, loads among the products: 1.20)
 //   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 71 to 76 us;
 //     bound by the products, and by what a block does before and behind them
 //     (about 11 us of its 31: tile search, first tiles, join)
@@ -99,12 +101,20 @@ __device__ __forceinline__ void pp_split2(float a, float b, uint32_t (&w)[3]) {
     }
 }
 
-// NT terms (1: rounded to nearest even) of 8 values as MFMA operands
+// NT terms of 8 values as MFMA operands: 1, rounded to nearest even; 2, each rounded so, x to 2^-17; 3, x itself
 template <int NT>
 __device__ __forceinline__ void pp_terms8(const float *x, bf16x8 (&t)[NT]) {
     if constexpr (NT == 1) {
         t[0] = __builtin_bit_cast(bf16x8, make_uint4(bf16_pack2(x[0], x[1]), bf16_pack2(x[2], x[3]),
                                                      bf16_pack2(x[4], x[5]), bf16_pack2(x[6], x[7])));
+    } else if constexpr (NT == 2) {
+        uint4 hi, lo;
+        bf16_split2(x[0], x[1], hi.x, lo.x);
+        bf16_split2(x[2], x[3], hi.y, lo.y);
+        bf16_split2(x[4], x[5], hi.z, lo.z);
+        bf16_split2(x[6], x[7], hi.w, lo.w);
+        t[0] = __builtin_bit_cast(bf16x8, hi);
+        t[1] = __builtin_bit_cast(bf16x8, lo);
     } else {
         uint32_t w[4][3];
 #pragma unroll
@@ -114,17 +124,25 @@ __device__ __forceinline__ void pp_terms8(const float *x, bf16x8 (&t)[NT]) {
     }
 }
 
-// The term pairs (i, j), i + j <= 2, of a product of NA by NB terms, small ones first
+// The term pairs (i, j) of a product of NA by NB terms, small ones first: i + j <= 2, or <= 1 where B is
+// held in two terms
 template <int NA, int NB>
 struct PpPairs {
-    static constexpr int N = NA * NB == 9 ? 6 : NA * NB;
+    static constexpr int MOST = NB == 2 ? 1 : 2;
+    static constexpr int count() {
+        int n = 0;
+        for (int i = 0; i < NA; i++)
+            for (int j = 0; j < NB; j++) n += i + j <= MOST;
+        return n;
+    }
+    static constexpr int N = count();
     struct List {
         int a[N], b[N];
     };
     static constexpr List make() {
         List l = {};
         int n = 0;
-        for (int sum = 2; sum >= 0; sum--)
+        for (int sum = MOST; sum >= 0; sum--)
             for (int i = NA - 1; i >= 0; i--)
                 for (int j = NB - 1; j >= 0; j--)
                     if (i + j == sum) {
@@ -262,7 +280,9 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
 // 64-row blocks on fp32 pages, which LDS lets only one of onto a CU.
 template <typename T, typename C, bool SMALL, int WR>
 __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) void paged_prefill(qk_paged_attn_args a, int slots) {
-    constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, KG = PP_KG, ROWS = PP_ROWS(WR);
+    // terms of the queries, the keys, the probabilities, the values
+    constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, NP = NQ == 1 ? 2 : NQ, NV = NQ == 1 && NK == 3 ? 2 : NK;
+    constexpr int KG = PP_KG, ROWS = PP_ROWS(WR);
     constexpr bool DIRECT = NK == 1;
     constexpr int NBUF = DIRECT ? 2 : 1;
     constexpr int STAGE = 2 * NK * PP_PLANE;              // bytes of one K and V tile
@@ -409,7 +429,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             pp_split2(st[i].z, st[i].w, w1);
             // terms below an infinite one come out as none: see pp_finite
 #pragma unroll
-            for (int t = 0; t < NK; t++) *reinterpret_cast<uint2 *>(plane(0, v, t) + at) = make_uint2(w0[t], w1[t]);
+            for (int t = 0; t < (v ? NV : NK); t++) *reinterpret_cast<uint2 *>(plane(0, v, t) + at) = make_uint2(w0[t], w1[t]);
         }
     };
 
@@ -433,7 +453,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     const int nt = (k1 - k0s + KG * PP_KT - 1) / (KG * PP_KT);       // tiles of a group
     pp_f32x16 st;
-    bf16x8 pt[2][NQ];
+    bf16x8 pt[2][NP];
     [[maybe_unused]] bf16x8 one[2];
 
     // S^T of the tile in K buffer buf
@@ -451,18 +471,20 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
     // their products.  The scores are one chain of sums: products in turn where a step has
     // few.  Six pairs have K's first, and V's fragments read only a step's length before.
     auto matrix = [&](int vbuf, int kbuf) {
-        constexpr int PAIRS = PpPairs<NK, NQ>::N, AHEAD = PAIRS == 1 ? 3 : 1, RING = AHEAD + 1;
-        constexpr bool TURNS = PAIRS < 6;
+        // products a step: of K, of V
+        constexpr int KP = PpPairs<NK, NQ>::N, VP = PpPairs<NV, NP>::N, AHEAD = KP == 1 ? 3 : 1, RING = AHEAD + 1;
+        constexpr bool TURNS = KP < 6;
         constexpr int VAHEAD = TURNS ? AHEAD : 0, VRING = VAHEAD + 1;
-        constexpr auto L = PpPairs<NK, NQ>::make();
-        bf16x8 kf[RING][NK], vf[VRING][NK];
+        constexpr auto LK = PpPairs<NK, NQ>::make();
+        constexpr auto LV = PpPairs<NV, NP>::make();
+        bf16x8 kf[RING][NK], vf[VRING][NV];
         auto read_k = [&](int u) {
 #pragma unroll
             for (int y = 0; y < NK; y++) kf[u % RING][y] = kfrag(kbuf, y, u);
         };
         auto read_v = [&](int u) {
 #pragma unroll
-            for (int y = 0; y < NK; y++) vf[u % VRING][y] = vfrag(vbuf, y, u & 3, u >> 2);
+            for (int y = 0; y < NV; y++) vf[u % VRING][y] = vfrag(vbuf, y, u & 3, u >> 2);
         };
         st = (pp_f32x16){};
 #pragma unroll
@@ -475,22 +497,22 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             if (u + AHEAD < 8) read_k(u + AHEAD);
             if (u + VAHEAD < 8) read_v(u + VAHEAD);
 #pragma unroll
-            for (int n = 0; n < PAIRS; n++) {
-                st = pp_mfma(kf[u % RING][L.a[n]], q[u][L.b[n]], st);
-                if (TURNS) o[u & 3] = pp_mfma(vf[u % VRING][L.a[n]], pt[u >> 2][L.b[n]], o[u & 3]);
+            for (int n = 0; n < (KP > VP ? KP : VP); n++) {
+                if (n < KP) st = pp_mfma(kf[u % RING][LK.a[n]], q[u][LK.b[n]], st);
+                if (TURNS && n < VP) o[u & 3] = pp_mfma(vf[u % VRING][LV.a[n]], pt[u >> 2][LV.b[n]], o[u & 3]);
             }
             if (!TURNS) {
 #pragma unroll
-                for (int n = 0; n < PAIRS; n++)
-                    o[u & 3] = pp_mfma(vf[u % VRING][L.a[n]], pt[u >> 2][L.b[n]], o[u & 3]);
+                for (int n = 0; n < VP; n++)
+                    o[u & 3] = pp_mfma(vf[u % VRING][LV.a[n]], pt[u >> 2][LV.b[n]], o[u & 3]);
             }
         }
-        __builtin_amdgcn_sched_group_barrier(0x100, (TURNS ? 3 : 1) * NK * AHEAD, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, (NK + (TURNS ? 2 * NV : 0)) * AHEAD, 0);
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            if (u + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 3 * NK, 0);
-            else if (!TURNS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * NK, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2 * PAIRS, 0);
+            if (u + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, NK + 2 * NV, 0);
+            else if (!TURNS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * NV, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, KP + VP, 0);
         }
     };
     // The probabilities of the tile at k0.  The maximum that they are taken against follows the
@@ -525,8 +547,8 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             sum += p[r];
         }
         l += sum;
-        pp_terms8<NQ>(p, pt[0]);
-        pp_terms8<NQ>(p + 8, pt[1]);
+        pp_terms8<NP>(p, pt[0]);
+        pp_terms8<NP>(p + 8, pt[1]);
         if constexpr (decltype(guarded)::value) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -548,10 +570,10 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             pp_f32x16 cnt = {};
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                bf16x8 vf[NK], cls;
+                bf16x8 vf[NV], cls;
 #pragma unroll
-                for (int y = NK - 1; y >= 0; y--) vf[y] = pp_finite(vfrag(buf, y, d, j), cls);
-                o[d] = pp_products<NK, NQ>(vf, pt[j], o[d]);
+                for (int y = NV - 1; y >= 0; y--) vf[y] = pp_finite(vfrag(buf, y, d, j), cls);
+                o[d] = pp_products<NV, NP>(vf, pt[j], o[d]);
                 cnt = pp_mfma(cls, one[j], cnt);
                 __builtin_amdgcn_sched_barrier(0);
             }
