@@ -48,6 +48,9 @@ static int paged_view(const char *op, const qwen_hip_paged_kv *kv, const qwen_hi
     return 0;
 }
 
+/* no row is a sequence's: nothing to launch, nothing to plan (a plan divides by the blocks of its sequences) */
+static int no_call(const qk_paged *p) { return p->rows == 0 || p->n_seqs == 0; }
+
 /* ... and the pointers that a call with rows reads */
 static int paged_pointers(const char *op, const qk_paged *p) {
     if (!p->k || !p->v || !p->table || !p->kv_len) QK_REFUSE("%s: a pointer of the cache or the batch is NULL", op);
@@ -70,7 +73,7 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
     if (!q_norm != !k_norm || !cos_vals != !sin_vals) QK_REFUSE("%s: one norm or one rotation table of two", op);
     if (q_norm && !(eps >= 0.0f && eps <= FLT_MAX)) QK_REFUSE("%s: eps %g", op, (double)eps);
     if (n_pos < 0) QK_REFUSE("%s: n_pos %d", op, n_pos);
-    if (batch->rows == 0 || kv->n_seqs == 0) return 0;       /* no row is a sequence's */
+    if (no_call(&a.pg)) return 0;
     if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
     if (!q_out || !q || !k || !v) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(q_out) || !qk_aligned16(q) || !qk_aligned16(k) || !qk_aligned16(v) || !qk_aligned16(q_norm) ||
@@ -121,7 +124,7 @@ static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_l
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
     int rows2, nsplit, chunk;
-    if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || p.rows == 0) return 0;
+    if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
     const int matrix = p.row_start || tokens_by_matrix(p.cache_bf16, heads / p.kv_heads);
     return attention_plan(&p, matrix, heads, batch->max_len, &rows2, &nsplit, &chunk);
 }
@@ -135,7 +138,7 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
     if (prefill && !batch->row_start) QK_REFUSE("%s: no row_start", op);
     if (!prefill && batch->row_start) QK_REFUSE("%s: one row per sequence: row_start has to be NULL", op);
     if (!(scale >= 1e-30f && scale <= 1e30f)) QK_REFUSE("%s: scale %g", op, (double)scale);
-    if (batch->rows == 0 || kv->n_seqs == 0) return 0;       /* no row is a sequence's */
+    if (no_call(&a.pg)) return 0;
     if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
     if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);

@@ -115,6 +115,15 @@ def test_no_sequences_is_no_call(qa):
         assert attend(qa, "prefill", **k) == 0
 
 
+@pytest.mark.parametrize("rows", [1, 3, 31, 63, 500])
+@pytest.mark.parametrize("heads,dtype", [(2, "f32"), (4, "f32"), (4, "bf16"), (16, "bf16")])
+def test_no_sequences_need_no_workspace(qa, rows, heads, dtype):
+    """the size that a program asks for before such a call"""
+    a, b = kv(qa, n_seqs=0, dtype=qa.ST_F32 if dtype == "f32" else qa.ST_BF16, table_stride=4096), batch(qa, rows=rows)
+    assert qa.lib().qwen_hip_paged_attention_ws_bytes(C.byref(a), C.byref(b), heads) == 0
+    assert attend(qa, "prefill", kvd=dict(n_seqs=0, table_stride=4096), bd=dict(rows=rows), heads=heads, ws=None, ws_bytes=0) == 0
+
+
 def sample(qa, **k):
     d = dict(tokens=P, logits=P, row_stride=1000, rows=2, vocab=1000, temperature=P, top_k=P, top_p=P, min_p=P, u=P,
              ws=P, ws_bytes=1 << 40)
