@@ -425,8 +425,9 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             const int r = SROWS * wave + RSTEP * i + srow0;
             const int at = 256 * r + 16 * ((ql >> 1) ^ swz(r)) + 8 * (ql & 1);
             uint32_t w0[3], w1[3];
-            pp_split2(st[i].x, st[i].y, w0);
-            pp_split2(st[i].z, st[i].w, w1);
+            // quiet: what is no number by its lower half alone would have an infinite upper term
+            pp_split2(__builtin_canonicalizef(st[i].x), __builtin_canonicalizef(st[i].y), w0);
+            pp_split2(__builtin_canonicalizef(st[i].z), __builtin_canonicalizef(st[i].w), w1);
             // terms below an infinite one come out as none: see pp_finite
 #pragma unroll
             for (int t = 0; t < (v ? NV : NK); t++) *reinterpret_cast<uint2 *>(plane(0, v, t) + at) = make_uint2(w0[t], w1[t]);

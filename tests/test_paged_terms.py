@@ -113,3 +113,43 @@ def test_bf16_rows_probabilities(qa, gpu, which, cache, group):
     want, tol = bounds(p, 1.0, 16, WEIGHTS[cache])
     for max_len in (64, 300, 5000):                # both block shapes, split and unsplit
         check(p.attention(qa, 1.0, max_len=max_len), want, tol)
+
+
+# ---------------------------------------------------------------------------
+# what is no number, by any of its bits
+# ---------------------------------------------------------------------------
+NANS = [0x7f800001, 0x7f80ffff, 0xff800001 - (1 << 32), 0x7fc00000, 0x7fffffff, -1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", NANS)
+def test_undefined_values_by_any_bits(qa, gpu, which, act, bits):
+    """a value of an fp32 cache is undefined whichever half of its word says so: the rows that see it are, and no
+    others"""
+    p = Paged(5, [70, 20], new=None if which == "decode" else [70, 20], group=2, kv_heads=2, page=16, act=act)
+    for x, s, pos, h, d in ((p.v, 0, 40, 0, 3), (p.v, 0, 69, 1, 100), (p.k, 1, 10, 1, 64)):
+        x.view(T.int32)[p.page_of(s, pos), h, pos % p.page, d] = bits
+    p.gpu(qa)
+    assert int(p.d["v"].view(T.int32)[p.page_of(0, 40), 0, 40 % p.page, 3]) == bits
+    check(p.attention(qa, 1.0 / math.sqrt(HD)), *p.reference(1.0 / math.sqrt(HD)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", NANS)
+@pytest.mark.parametrize("cache", ["f32", "bf16"])
+def test_append_undefined_by_any_bits(qa, gpu, cache, bits):
+    """an undefined element of an fp32 row stays one in the pages"""
+    import ctypes as C
+    p = Paged(6, [3], group=1, kv_heads=1, page=4, cache=cache).gpu(qa)
+    x = T.ones(1, 3 * HD)
+    x.view(T.int32)[0, HD + 5] = x.view(T.int32)[0, 2 * HD + 6] = bits
+    x, out = x.cuda(), T.zeros(1, HD, device="cuda")
+    b = x.data_ptr()
+    qa.check(qa.lib().qwen_hip_paged_append(C.byref(p.c_kv), C.byref(p.c_batch), out.data_ptr(), b, b + 4 * HD,
+                                            b + 8 * HD, p.c_act, HD, HD, 1, None, None, 0.0, None, None, 0, None))
+    T.cuda.synchronize()
+    i = p.page_of(0, 2)
+    k, v = p.d["k"][i, 0, 2].float().cpu(), p.d["v"][i, 0, 2].float().cpu()
+    assert T.isnan(k).nonzero().tolist() == [[5]] and T.isnan(v).nonzero().tolist() == [[6]]
