@@ -536,8 +536,8 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
  * packed rows (row_start given; sequences may have no rows, one, or all of their
  * positions).  Softmax statistics and sums in fp32.  fp32 rows: products exact to
  * 2^-24 on either cache type; bf16 rows: _prefill, and _decode of more than four
- * heads a kv head on a bf16 cache, hold the probabilities to 2^-17 and the values of an
- * fp32 cache to 2^-15 (two bf16 terms each) before they meet.  A key with an infinite element makes the rows that see
+ * heads a kv head on a bf16 cache, hold the probabilities, and the values of an fp32
+ * cache, to 2^-17 (two bf16 terms) before they meet.  A key with an infinite element makes the rows that see
  * it undefined (NaN); what a row does not see never reaches it.  The workspace
  * holds the partial results of a split over the positions. */
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);

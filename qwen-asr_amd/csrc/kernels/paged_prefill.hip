@@ -7,14 +7,16 @@
 // on v_mfma_f32_32x32x16_bf16, with fp32 statistics and sums.
 //
 // Operands.  bf16 values go to the matrix cores as they are.  An fp32 value is
-// the sum of three bf16 terms, x = h + m + l: h the upper 16 bits, m those of
-// x - h, l those of x - h - m; 8 + 8 + 8 significant bits hold all 24, so the split
+// the sum of three bf16 terms, x = h + m + l: h is x rounded to nearest, m what is left
+// of x rounded so, l what is left then, which has no more than 8 bits: the split
 // is exact.  Products of two such values keep the term pairs (i, j) with i + j <= 2
-// (h is term 0): the dropped ones are below 2^-24 of the product.  With fp32
+// (h is term 0): m is at most 2^-8 and l 2^-17 of the value's power of two, so the
+// dropped ones are below 2^-24 of the product, of either sign (terms that are cut off
+// instead of rounded drop up to 2^-21, always towards 0).  With fp32
 // queries the probabilities are split as well, so such a call is as exact as fp32
 // products (3 matrix products a pair on a bf16 cache, 6 on an fp32 one, against
 // 16 times the time of one on the fp32 matrix cores).  With bf16 queries the
-// probabilities are held in two terms, each rounded to nearest even (2^-17 of them), and
+// probabilities are held in two terms (2^-17 of them), and
 // so are fp32 values (the upper two of their three): one term alone is off by as much as
 // the result's own rounding, 1.3 to 1.4 times the error of an fp32 softmax rounded once
 // (8191 rows: 0.0021 and 0.0016 of the result's norm; 306 us with one, 392 with two).
@@ -90,19 +92,24 @@ __device__ __forceinline__ void pp_lds_load16(const unsigned char *p, unsigned c
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p), "s"(at) : "memory");
 }
 
-// the three terms of two values, each pair in one word (a low)
+// the three terms of two values, each pair in one word (a low).  ANY: the largest values would round to an
+// infinite h, so it ends at the largest bf16; then m says what the value is, infinite or no number as that
+#define PP_BF16_MAX 0x1.fep127f
+template <bool ANY>
 __device__ __forceinline__ void pp_split2(float a, float b, uint32_t (&w)[3]) {
-#pragma unroll
-    for (int t = 0; t < 3; t++) {
-        const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-        w[t] = __builtin_amdgcn_perm(ub, ua, 0x07060302);          // upper halves
-        a -= __uint_as_float(ua & 0xffff0000u);
-        b -= __uint_as_float(ub & 0xffff0000u);
-    }
+    if constexpr (ANY) w[0] = bf16_pack2(__builtin_amdgcn_fmed3f(a, -PP_BF16_MAX, PP_BF16_MAX),
+                                         __builtin_amdgcn_fmed3f(b, -PP_BF16_MAX, PP_BF16_MAX));
+    else w[0] = bf16_pack2(a, b);
+    a -= bf16_lo(w[0]);
+    b -= bf16_hi(w[0]);
+    w[1] = bf16_pack2(a, b);
+    a -= bf16_lo(w[1]);
+    b -= bf16_hi(w[1]);
+    w[2] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);      // upper halves: all that is left
 }
 
 // NT terms of 8 values as MFMA operands: 1, rounded to nearest even; 2, each rounded so, x to 2^-17; 3, x itself
-template <int NT>
+template <int NT, bool ANY = false>
 __device__ __forceinline__ void pp_terms8(const float *x, bf16x8 (&t)[NT]) {
     if constexpr (NT == 1) {
         t[0] = __builtin_bit_cast(bf16x8, make_uint4(bf16_pack2(x[0], x[1]), bf16_pack2(x[2], x[3]),
@@ -118,7 +125,7 @@ __device__ __forceinline__ void pp_terms8(const float *x, bf16x8 (&t)[NT]) {
     } else {
         uint32_t w[4][3];
 #pragma unroll
-        for (int i = 0; i < 4; i++) pp_split2(x[2 * i], x[2 * i + 1], w[i]);
+        for (int i = 0; i < 4; i++) pp_split2<ANY>(x[2 * i], x[2 * i + 1], w[i]);
 #pragma unroll
         for (int k = 0; k < 3; k++) t[k] = __builtin_bit_cast(bf16x8, make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]));
     }
@@ -170,8 +177,7 @@ __device__ __forceinline__ bf16x8 pp_vfrag(const unsigned char *p, const unsigne
 }
 
 // The lanes' words with every element that is infinite or no number replaced by
-// 0 (lower terms of an infinite value are none); cls gets 1, 64 or 4096 in the
-// places of +inf, -inf and no number.
+// 0; cls gets 1, 64 or 4096 in the places of +inf, -inf and no number.
 __device__ __forceinline__ bf16x8 pp_finite(bf16x8 v, bf16x8 &cls) {
     uint4 w = __builtin_bit_cast(uint4, v), k = make_uint4(0u, 0u, 0u, 0u);
     uint32_t *pw = &w.x, *pk = &k.x;
@@ -186,6 +192,15 @@ __device__ __forceinline__ bf16x8 pp_finite(bf16x8 v, bf16x8 &cls) {
             }
         }
     cls = __builtin_bit_cast(bf16x8, k);
+    return __builtin_bit_cast(bf16x8, w);
+}
+
+// v with 0 in the places that cls says something of
+__device__ __forceinline__ bf16x8 pp_cleared(bf16x8 v, bf16x8 cls) {
+    uint4 w = __builtin_bit_cast(uint4, v), k = __builtin_bit_cast(uint4, cls);
+    uint32_t *pw = &w.x, *pk = &k.x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) pw[i] &= (pk[i] & 0xffffu ? 0u : 0xffffu) | (pk[i] >> 16 ? 0u : 0xffff0000u);
     return __builtin_bit_cast(bf16x8, w);
 }
 
@@ -425,10 +440,8 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             const int r = SROWS * wave + RSTEP * i + srow0;
             const int at = 256 * r + 16 * ((ql >> 1) ^ swz(r)) + 8 * (ql & 1);
             uint32_t w0[3], w1[3];
-            // quiet: what is no number by its lower half alone would have an infinite upper term
-            pp_split2(__builtin_canonicalizef(st[i].x), __builtin_canonicalizef(st[i].y), w0);
-            pp_split2(__builtin_canonicalizef(st[i].z), __builtin_canonicalizef(st[i].w), w1);
-            // terms below an infinite one come out as none: see pp_finite
+            pp_split2<true>(st[i].x, st[i].y, w0);
+            pp_split2<true>(st[i].z, st[i].w, w1);
 #pragma unroll
             for (int t = 0; t < (v ? NV : NK); t++) *reinterpret_cast<uint2 *>(plane(0, v, t) + at) = make_uint2(w0[t], w1[t]);
         }
@@ -572,8 +585,13 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 bf16x8 vf[NV], cls;
+                if constexpr (NK == 1) {
+                    vf[0] = pp_finite(vfrag(buf, 0, d, j), cls);
+                } else {                                  // see pp_split2
+                    vf[1] = pp_finite(vfrag(buf, 1, d, j), cls);
 #pragma unroll
-                for (int y = NV - 1; y >= 0; y--) vf[y] = pp_finite(vfrag(buf, y, d, j), cls);
+                    for (int y = 0; y < NV; y += 2) vf[y] = pp_cleared(vfrag(buf, y, d, j), cls);
+                }
                 o[d] = pp_products<NV, NP>(vf, pt[j], o[d]);
                 cnt = pp_mfma(cls, one[j], cnt);
                 __builtin_amdgcn_sched_barrier(0);
@@ -679,7 +697,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         for (int t = 0; t < 8; t++) {
             const float4 x0 = pg_load4(qp + 16 * t), x1 = pg_load4(qp + 16 * t + 4);
             const float v[8] = {x0.x * fs, x0.y * fs, x0.z * fs, x0.w * fs, x1.x * fs, x1.y * fs, x1.z * fs, x1.w * fs};
-            pp_terms8<NQ>(v, q[t]);
+            pp_terms8<NQ, true>(v, q[t]);
         }
     }
     walk(PpBool<false>());

@@ -153,3 +153,117 @@ def test_append_undefined_by_any_bits(qa, gpu, cache, bits):
     i = p.page_of(0, 2)
     k, v = p.d["k"][i, 0, 2].float().cpu(), p.d["v"][i, 0, 2].float().cpu()
     assert T.isnan(k).nonzero().tolist() == [[5]] and T.isnan(v).nonzero().tolist() == [[6]]
+
+
+# ---------------------------------------------------------------------------
+# fp32 rows: every operand in three terms, whose products lose 2^-24 at most
+# ---------------------------------------------------------------------------
+# Half steps of fp32 that a score of one product may be off by: one for the dropped terms, one step
+# of the sum that adds the largest term, and those of the sums before it, a part in 256 of it.
+ONE_PRODUCT = 3.5
+
+
+def first_order(p, scale, roundings):
+    """(out, tolerance) to first order in the scores' errors: d out = sum w_j (v_j - out) d s_j.  A
+    score is off by `roundings` half steps of itself (none where the key's element is a power of two:
+    then its product is the query's terms moved), and, as the difference to the largest that the
+    exponential takes, by 6 of 1 + |difference| (the scaling's two roundings, which all keys of a
+    query of one dim share, the difference's own, the exponential's ulp and its argument); the
+    sums over n keys by n + 8 half steps of their absolute terms each."""
+    out = T.zeros(p.rows, p.heads, HD, dtype=T.float64)
+    tol = T.zeros_like(out)
+    for row, h, q, k, v in by_row(p):
+        sc = k @ q * scale
+        w, n = T.softmax(sc, 0), k.shape[0]
+        o = w @ v
+        moved = T.frexp(k[:, int(q.abs().argmax())])[0].abs() == 0.5
+        off = T.where(moved, 0.0, roundings * E * sc.abs()) + 6 * E * (1 + (sc - sc.max()).abs())
+        out[row, h] = o
+        tol[row, h] = 1.1 * ((w * off) @ (v - o).abs() + 2 * (n + 8) * E * (w @ v.abs()) + U.HALF[p.act] * o.abs()) + 1e-37
+    return out.view(p.rows, -1), tol.view(p.rows, -1)
+
+
+def parts(x, n, cut=False):
+    """n bf16 terms of fp32 values, each rounded to nearest even or cut off"""
+    got, left, most = [], x.float(), T.finfo(T.bfloat16).max
+    for _ in range(n):
+        t = (left.view(T.int32) & -65536).view(T.float32) if cut else left.clamp(-most, most).bfloat16().float()
+        got.append(t.double())
+        left = left - t
+    return got
+
+
+def emulate_terms(p, scale, n=3, cut=False, which="qkpv"):
+    """the attention with the products of n terms (pairs i + j < n) of the operands in `which` against exact values"""
+    def times(a, b, product, names):
+        if not all(x in which for x in names):
+            return product(a, b)
+        return sum(product(x, y) for i, x in enumerate(parts(a, n, cut)) for j, y in enumerate(parts(b, n, cut)) if i + j < n)
+
+    out = T.zeros(p.rows, p.heads, HD, dtype=T.float64)
+    for row, h, q, k, v in by_row(p):
+        sc = times(k, q, lambda a, b: a @ b, "qk") * scale
+        x = T.exp(sc - sc.max()).float().double()
+        out[row, h] = times(x, v, lambda a, b: a @ b, "pv") / x.sum()
+    return out.view(p.rows, -1)
+
+
+F32_LENS = [2, 2, 3, 4, 9, 33]
+
+
+def near(which, cache, group):
+    """scores of hundreds within a few units: queries and every other key a little below 1 + 2^-7, where terms
+    that are cut off leave the most behind, the other keys 1"""
+    p = one_dim(40 + group, "f32", cache, group, F32_LENS * 4, None if which == "decode" else [2, 1, 3, 2, 5, 20] * 4)
+    low = lambda *s: 1 + 2.0 ** -7 - T.randint(1, 100, s, generator=p.g).double() * 2.0 ** -23
+    p.q = T.where(p.q == 0, 0.0, 512 * low(*p.q.shape)).float()
+    k = low(*p.k.shape)
+    k[:, :, ::2] = 1.0
+    p.k = T.where(T.isnan(p.k.double()), math.nan, k).to(p.k.dtype)
+    return p, math.log(2.0)
+
+
+def test_f32_rows_case_sees_terms_cut_off():
+    """three terms that are cut off, not rounded, lose up to 2^-21 of a product"""
+    p, scale = near("prefill", "f32", 8)
+    want, tol = first_order(p, scale, ONE_PRODUCT)
+    assert outside(emulate_terms(p, scale, cut=True, which="qk"), want, tol) > 0.02 * want.numel()
+
+
+def test_products_of_three_terms():
+    """what the pairs i + j <= 2 drop: below 2^-24 of the product to nearest, up to 2^-21 cut off"""
+    g = T.Generator().manual_seed(9)
+    x, y = ((1 + T.rand(1 << 20, generator=g)).float() for _ in range(2))
+    x[:4096], y[:4096] = 1 + 2.0 ** -7 - T.rand(4096, generator=g) * 2.0 ** -16, 1 + 2.0 ** -7 - T.rand(4096, generator=g) * 2.0 ** -16
+    x[4096:8192], y[4096:8192] = 1 + 2.0 ** -8 - T.rand(4096, generator=g) * 2.0 ** -15, 1 + 2.0 ** -8 - T.rand(4096, generator=g) * 2.0 ** -15
+    loss = lambda cut: float(((sum(a * b for i, a in enumerate(parts(x, 3, cut)) for j, b in enumerate(parts(y, 3, cut))
+                                   if i + j <= 2)) / (x.double() * y.double()) - 1).abs().max())
+    assert loss(False) <= 2.0 ** -24 < 4 * 2.0 ** -24 < loss(True) < 2.0 ** -21
+    for z in (x, y, T.tensor([3.4e38, -3.39e38, 1e-30])):
+        assert T.equal(sum(parts(z, 3, False)), z.double())     # three terms are the value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("group", [1, 2, 4, 8])
+def test_f32_rows_near_scores(qa, gpu, group, which):
+    p, scale = near(which, "f32", group)
+    p.gpu(qa)
+    want, tol = first_order(p, scale, ONE_PRODUCT)
+    for max_len in (33, 300, 5000):
+        check(p.attention(qa, scale, max_len=max_len), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+def test_f32_largest_numbers(qa, gpu, which):
+    """queries and keys that round to an infinity as bf16"""
+    p = Paged(90, [2, 2], new=None if which == "decode" else [1, 1], group=2, kv_heads=1, page=16)
+    big = T.finfo(T.float32).max
+    p.q.zero_()
+    p.q[0, [5, HD + 5]], p.q[1, [5, HD + 5]] = T.tensor([big, -big]), T.tensor([2.0 ** -126, -2.0 ** -126])
+    i, j = p.page_of(0, 0), p.page_of(1, 0)
+    p.k[i, 0, :2], p.k[j, 0, :2] = 0.0, 0.0
+    p.k[i, 0, 0, 5], p.k[i, 0, 1, 5] = 2.0 ** -126, 2.0 ** -125
+    p.k[j, 0, 0, 5], p.k[j, 0, 1, 5] = big, -big
+    check(p.gpu(qa).attention(qa, math.log(2.0)), *first_order(p, math.log(2.0), ONE_PRODUCT))
