@@ -83,7 +83,7 @@ def outside(got, want, tol):
 
 
 # ---------------------------------------------------------------------------
-# bf16 rows: probabilities in two terms (2^-17 of each), fp32 values in two (2^-15)
+# bf16 rows: probabilities in two terms, fp32 values in two
 # ---------------------------------------------------------------------------
 WEIGHTS = {"bf16": 2.0 ** -16, "f32": 2.0 ** -14}
 LENS = [2, 3, 16, 40, 300]
@@ -211,6 +211,13 @@ def emulate_terms(p, scale, n=3, cut=False, which="qkpv"):
 F32_LENS = [2, 2, 3, 4, 9, 33]
 
 
+def wide(which, cache, group):
+    """scores some units apart, all of their bits in use"""
+    p = one_dim(20 + group, "f32", cache, group, F32_LENS * 4, None if which == "decode" else [2, 1, 3, 2, 5, 20] * 4)
+    p.k = (2 * p.k.float()).to(p.k.dtype)
+    return p, 1.0
+
+
 def near(which, cache, group):
     """scores of hundreds within a few units: queries and every other key a little below 1 + 2^-7, where terms
     that are cut off leave the most behind, the other keys 1"""
@@ -221,6 +228,32 @@ def near(which, cache, group):
     k[:, :, ::2] = 1.0
     p.k = T.where(T.isnan(p.k.double()), math.nan, k).to(p.k.dtype)
     return p, math.log(2.0)
+
+
+def weights(which, cache, group):
+    """two keys whose scores are exact, one value of 1 and one of 0: the weight itself"""
+    n = 96
+    p = Paged(60 + group, [2] * n, new=None if which == "decode" else [1] * n, group=group, kv_heads=1, page=4, cache=cache)
+    p.q = T.zeros(n, p.heads, HD)
+    p.q[..., 7] = 1.0
+    p.q = p.q.view(n, -1)
+    for s in range(n):
+        i = p.page_of(s, 0)
+        p.k[i, :, :2, 7] = T.randint(-24, 25, (1, 2), generator=p.g).to(p.k.dtype) / 16
+        p.v[i, :, 0], p.v[i, :, 1] = 1.0, 0.0
+    return p, 1.0
+
+
+CASES = [(wide, "f32", "qk"), (wide, "bf16", "qk"), (weights, "f32", "pv"), (weights, "bf16", "pv"), (near, "f32", "qk")]
+
+
+@pytest.mark.parametrize("make,cache,operands", CASES[:-1])
+def test_f32_rows_case_sees_two_terms(make, cache, operands):
+    """operands in two terms are outside of the bound, in three (to nearest) inside"""
+    p, scale = make("prefill", cache, 8)
+    want, tol = first_order(p, scale, ONE_PRODUCT)
+    assert outside(emulate_terms(p, scale, 2, which=operands), want, tol) > 0.005 * want.numel()
+    assert outside(emulate_terms(p, scale), want, tol) == 0
 
 
 def test_f32_rows_case_sees_terms_cut_off():
@@ -246,12 +279,30 @@ def test_products_of_three_terms():
 @pytest.mark.gpu
 @pytest.mark.parametrize("which", ["decode", "prefill"])
 @pytest.mark.parametrize("group", [1, 2, 4, 8])
-def test_f32_rows_near_scores(qa, gpu, group, which):
-    p, scale = near(which, "f32", group)
+@pytest.mark.parametrize("make,cache,operands", CASES)
+def test_f32_rows_terms(qa, gpu, make, cache, operands, group, which):
+    p, scale = make(which, cache, group)
     p.gpu(qa)
     want, tol = first_order(p, scale, ONE_PRODUCT)
     for max_len in (33, 300, 5000):
         check(p.attention(qa, scale, max_len=max_len), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("cache", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [1, 2, 8])
+def test_f32_rows_one_key(qa, gpu, which, cache, group):
+    """a row that sees one key gets its value, bit for bit: the largest numbers, which round to an infinity as
+    bf16, among them"""
+    p = Paged(80 + group, [1] * 40, new=None if which == "decode" else [1] * 40, group=group, kv_heads=2, page=16, cache=cache)
+    big = T.finfo(T.float32).max if cache == "f32" else T.finfo(T.bfloat16).max
+    for s in range(0, 40, 3):
+        p.v[p.page_of(s, 0), :, 0, 11], p.v[p.page_of(s, 0), :, 0, 90] = big, -big * (1 - 2.0 ** -10)
+    p.gpu(qa)
+    want = T.stack([p.v[p.page_of(s, 0), :, 0].float().repeat_interleave(group, 0).flatten() for s in range(40)])
+    for max_len in (1, 300, 5000):
+        assert T.equal(p.attention(qa, 1.0, max_len=max_len).cpu(), want)
 
 
 @pytest.mark.gpu
@@ -267,3 +318,11 @@ def test_f32_largest_numbers(qa, gpu, which):
     p.k[i, 0, 0, 5], p.k[i, 0, 1, 5] = 2.0 ** -126, 2.0 ** -125
     p.k[j, 0, 0, 5], p.k[j, 0, 1, 5] = big, -big
     check(p.gpu(qa).attention(qa, math.log(2.0)), *first_order(p, math.log(2.0), ONE_PRODUCT))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("cache", ["f32", "bf16"])
+def test_nearly_even_weights(qa, gpu, which, cache):
+    p = Paged(34, [257, 64], new=None if which == "decode" else [40, 64], group=8, kv_heads=2, page=16, cache=cache)
+    check(p.gpu(qa).attention(qa, 1e-3), *p.reference(1e-3))
