@@ -539,7 +539,11 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
  * heads a kv head on a bf16 cache, hold the probabilities, and the values of an fp32
  * cache, to 2^-17 (two bf16 terms) before they meet.  A key with an infinite element makes the rows that see
  * it undefined (NaN); what a row does not see never reaches it.  The workspace
- * holds the partial results of a split over the positions. */
+ * holds the partial results of a split over the positions; ws_bytes is what a batch
+ * needs.  A smaller batch may need more than a larger one, whose rows fill the card
+ * without a split; none needs more than QWEN_HIP_PAGED_ATTENTION_WS_MAX, which serves
+ * a program that keeps one workspace for all its batches. */
+#define QWEN_HIP_PAGED_ATTENTION_WS_MAX ((size_t)49 << 20)
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);
 int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
                                     const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,

@@ -48,6 +48,10 @@ class PagedBatch(C.Structure):
     _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("rows", C.c_int), ("max_len", C.c_int)]
 
 
+# no batch's attention needs a larger workspace
+PAGED_ATTENTION_WS_MAX = 49 << 20
+
+
 def build(jobs=8):
     """Compile the library in-tree (hipcc for gfx950 + gcc)."""
     subprocess.run(["make", "-s", "-C", HERE, f"-j{jobs}"], check=True)

@@ -2,6 +2,7 @@
 is checked before anything is launched, so these run without a GPU (the pointers are never read)."""
 import ctypes as C
 import math
+import random
 
 import pytest
 
@@ -96,6 +97,32 @@ def test_attention_workspace_refused(qa, which):
     for bad in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=P + 4)):
         assert attend(qa, which, kvd=kvd, bd=bd, **bad) == EINVAL
         assert "workspace" in qa.last_error()
+
+
+def ws_bytes(qa, rows, n_seqs, heads, kv_heads, max_len, dtype, page, packed):
+    a = kv(qa, n_seqs=n_seqs, kv_heads=kv_heads, dtype=dtype, page_size=page, table_stride=1 << 16, n_pages=64)
+    b = batch(qa, rows=rows, max_len=max_len, row_start=P if packed else None)
+    return qa.lib().qwen_hip_paged_attention_ws_bytes(C.byref(a), C.byref(b), heads)
+
+
+def test_attention_workspace_bound(qa):
+    """one size for all batches: the need does not grow with the batch (a smaller one is split further)"""
+    need = [ws_bytes(qa, rows, 8, 16, 8, 4096, qa.ST_BF16, 64, True) for rows in (8000, 4000, 2500, 2000, 512)]
+    assert need[0] == 0 and need[2] > need[4] > 0
+    most, rng = {True: 0, False: 0}, random.Random(1)
+    for i in range(60000):
+        kv_heads = rng.choice([1, 1, 2, 3, 5, 8, 16])
+        heads = kv_heads * rng.choice([1, 2, 3, 4, 5, 7, 8, 9, 16, 64])
+        n_seqs = min(int(2 ** rng.uniform(0, 14)), (1 << 20) // heads)
+        packed = rng.random() < 0.6
+        # around the borders of the plans as well
+        near = rng.choice([128, 64]) * rng.randint(1, 400) + rng.choice([-1, 0, 1]) if rng.random() < 0.5 else int(2 ** rng.uniform(0, 17))
+        rows = max(1, min(near, (1 << 23) // heads)) if packed else n_seqs
+        most[packed] = max(most[packed], ws_bytes(qa, rows, n_seqs, heads, kv_heads, int(2 ** rng.uniform(0, 20)),
+                                                  rng.choice([qa.ST_F32, qa.ST_BF16]), rng.choice([1, 16, 64]), packed))
+    # below it, and not by much
+    assert qa.PAGED_ATTENTION_WS_MAX / 2 < most[True] <= qa.PAGED_ATTENTION_WS_MAX
+    assert qa.PAGED_ATTENTION_WS_MAX / 8 < most[False] <= qa.PAGED_ATTENTION_WS_MAX
 
 
 def test_no_rows_is_no_call(qa):
