@@ -804,7 +804,8 @@ template <typename T, typename C, int WR>
 static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     const qk_paged &pg = a->pg;
     const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS(WR) + pg.n_seqs;
-    if (slots * pg.kv_heads > 0x7fffffffL) return QWEN_HIP_EINVAL;
+    // a launch has fewer than 2^32 threads along an axis
+    if (slots * pg.kv_heads > 0xffffffffL / PP_THREADS(WR)) return QWEN_HIP_EINVAL;
     const dim3 grid((unsigned)(slots * pg.kv_heads), (unsigned)a->nsplit);
     // the plan takes 64 rows for pages of 16 positions and more
     constexpr bool SOME_SMALL = WR == 4;

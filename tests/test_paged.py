@@ -125,6 +125,14 @@ def test_attention_workspace_bound(qa):
     assert qa.PAGED_ATTENTION_WS_MAX / 8 < most[False] <= qa.PAGED_ATTENTION_WS_MAX
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_blocks_than_a_launch_has_refused(qa, dtype):
+    """sequences without rows have a block a kv head all the same: more than 2^32 threads are no launch"""
+    kvd = dict(n_seqs=1 << 22, kv_heads=8, dtype=qa.ST_F32 if dtype == "f32" else qa.ST_BF16)
+    assert attend(qa, "prefill", kvd=kvd, bd=dict(rows=1), heads=8) == EINVAL
+    assert "qk_paged_prefill_launch" in qa.last_error()
+
+
 def test_no_rows_is_no_call(qa):
     """no rows: nothing to launch, whatever the pointers"""
     none = dict(k=None, v=None, table=None)
