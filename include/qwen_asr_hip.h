@@ -523,26 +523,28 @@ typedef struct {
  * apart, those of k and v kv_stride (at least a row, multiples of 16 bytes).
  * q_out may be q (q_stride == heads * head_dim).  All arithmetic in fp32, rounded
  * once to nearest even.  Pointers 16-byte aligned.  A row at a negative position
- * or at one from n_pos on is left out altogether. */
+ * or at one from n_pos or the table's end on is left out altogether, its query too. */
 int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *q_out,
                           const void *q, const void *k, const void *v, int dtype, long q_stride, long kv_stride,
                           int heads, const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
                           const float *sin_vals, int n_pos, hipStream_t s);
 
 /* Causal attention over the cache, q and out [rows][heads * head_dim] of
- * `dtype` (out not q): a row sees the positions up to its own that are there;
+ * `dtype` (out apart from q): a row sees the positions up to its own that are there;
  * one that sees none gets 0.  heads is a multiple of kv_heads; `scale` positive,
  * 1e-30 .. 1e30.  _decode takes one row per sequence (row_start NULL), _prefill
  * packed rows (row_start given; sequences may have no rows, one, or all of their
- * positions).  Softmax statistics and sums in fp32.  fp32 rows: products exact to
- * 2^-24 on either cache type; bf16 rows: _prefill, and _decode of more than four
- * heads a kv head on a bf16 cache, hold the probabilities, and the values of an fp32
- * cache, to 2^-17 (two bf16 terms) before they meet.  A key with an infinite element makes the rows that see
- * it undefined (NaN); what a row does not see never reaches it.  The workspace
- * holds the partial results of a split over the positions; ws_bytes is what a batch
- * needs.  A smaller batch may need more than a larger one, whose rows fill the card
- * without a split; none needs more than QWEN_HIP_PAGED_ATTENTION_WS_MAX, which serves
- * a program that keeps one workspace for all its batches. */
+ * positions; of prompts and single tokens on fp32 pages, or of tokens behind long
+ * pasts, a call each takes less time than one for both).  Softmax statistics and
+ * sums in fp32.  fp32 rows: products exact to 2^-24 on either cache type; bf16 rows:
+ * _prefill, and _decode of more than four heads a kv head on a bf16 cache, hold the
+ * probabilities, and the values of an fp32 cache, to 2^-17 (two bf16 terms) before
+ * they meet.  A key with an infinite element makes the rows that see it undefined
+ * (NaN); what a row does not see never reaches it.  The workspace holds the partial
+ * results of a split over the positions; ws_bytes is what a batch needs.  A smaller
+ * batch may need more than a larger one, whose rows fill the card without a split;
+ * none needs more than QWEN_HIP_PAGED_ATTENTION_WS_MAX, which serves a program that
+ * keeps one workspace for all its batches. */
 #define QWEN_HIP_PAGED_ATTENTION_WS_MAX ((size_t)49 << 20)
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);
 int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,

@@ -104,9 +104,9 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
  * Whether single tokens run on the matrix cores, as prompts of one row do: where many heads share
  * a bf16 cache's rows, the vector units are what bounds the other kernel.  Microseconds, vector
  * kernel against matrix kernel, 8 kv heads, 24 sequences of 500 to 6001 positions:
- *   bf16 rows, 2 heads a kv head: 48, 58; 4: 59, 59; 8: 98, 59; 16: 141, 61
+ *   bf16 rows, 2 heads a kv head: 49, 66; 4: 59, 66; 8: 98, 66; 16: 141, 67
  *   fp32 rows (split into three terms), 4: 59, 89; 8: 98, 89; 16: 141, 90
- * and of 131 to 530: bf16 rows, 2: 12, 15; 4: 15, 15; 5: 23, 15; fp32 rows, 4: 15, 19; 8: 23, 20.
+ * and of 131 to 530: bf16 rows, 2: 13, 16; 4: 16, 16; 5: 23, 16; fp32 rows, 4: 15, 19; 8: 23, 20.
  * fp32 pages take the matrix kernel longer throughout (8 heads: 108, 234).
  */
 static int tokens_by_matrix(int cache_bf16, int group) { return cache_bf16 && group > 4; }

@@ -50,10 +50,12 @@
 //     probabilities' second term) at 1050 TFLOP/s; bound by them and the softmax beside them
 //     (with one term, in 306 us, tiles staged through registers took 1.24 times the time; 64
 //     rows a wave, one wave a SIMD: 2.1; three buffers, loads among the products: 1.20)
-//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 71 to 76 us;
+//   8 prompts of 101 to 1515 rows, fp32 rows on a bf16 cache (three products for one): 71 to 81 us;
 //     bound by the products, and by what a block does before and behind them
 //     (about 11 us of its 31: tile search, first tiles, join)
-//   31 new rows behind 993, all fp32: 19.4 us, a chain of first loads and the join's launch
+//   the same on fp32 pages (six products for one; more than 64 rows a sequence: about 50 registers
+//     spill): 159 us; bf16 rows on fp32 pages (three for one): 82 us
+//   31 new rows behind 993, all fp32: 19.6 to 20.7 us, a chain of first loads and the join's launch
 //
 // Masked keys: a masked score is -inf before the maximum, but 0 times what the
 // cache holds is no number where that is infinite or none.  Such a V
@@ -683,7 +685,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         if (kg == 0) barrier();
     };
     // Queries: dims 16 t + 8 hl .. + 7.  bf16 ones are on their way before the page ids are waited
-    // for (16 prompts of 300 to 1000 rows: 155 us behind them, 150 before); fp32 ones, which are
+    // for (16 prompts of 300 to 1000 rows: 154 us behind them, 151 before); fp32 ones, which are
     // split and take the scale along, would cost registers there (8 prompts on a bf16 cache: 72, 77).
     const T *const qp = (const T *)a.q + orow * PG_HD + 8 * hl;
     if constexpr (NQ == 1) {
@@ -773,26 +775,28 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
 extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk) {
     const long f = (long)p->rows * (heads / p->kv_heads);
     // Blocks of 64 rows run two to a CU, one's begin and end beside the other's products, but read every key twice as
-    // often.  bf16, 128 and 64 rows: 16 prompts of 300 to 1000, 151 and
-    // 141 us; 8 of 60 to 400, 28 and 19; 24 single tokens of 131 to 530, 8 heads a kv head, 21 and 15; but 4 prompts
-    // of 1000 to 4000, 300 and 310, one of 8191, 303 and 338.  Where the keys are split, up to 768: 4 chunks of 30 rows
-    // on fp32 rows, 500 positions, 17.3 and 16.5; 1000, 18.6 and 20.3.  On fp32 pages their tiles do not fit LDS twice,
+    // often.  bf16, 128 and 64 rows: 16 prompts of 300 to 1000, 4 heads a kv head, 163 and
+    // 151 us; 8 of 60 to 400, 2 heads, 32 and 16; 24 single tokens of 131 to 530, 8 heads, 22 and 16; but 4 prompts
+    // of 1000 to 4000, 362 and 370, one of 8191, 392 and 426.  Where the keys are split, up to 768: 4 chunks of 30 rows
+    // on fp32 rows, 500 positions, 17.3 and 16.6; 1000, 19.3 and 20.7.  On fp32 pages their tiles do not fit LDS twice,
     // but sequences of no more rows leave half of a larger block's waves idle, and one wave a SIMD has the registers
-    // for six products without spills (fp32 rows, 31 behind 993: 22.4 and 19.8 us; 16 of 16 to 31 behind up to 600,
-    // 46.7 and 35.8).
+    // for six products with hardly a spill (fp32 rows, 31 behind 993: 22.6 and 20.6 us; 16 of 16 to 32 behind up to 600,
+    // 46.6 and 38.0).  The host knows the mean of the sequences' rows alone, and goes by that: a long prompt among many
+    // short ones gets blocks of 64 rows too (512 rows beside 31 tokens of 1000 positions, fp32: 164 and 114 us; of 4000:
+    // 430 and 299; 4 of 500 beside 60 of 1000, whose mean is above: 250).
     const int fits = (f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 2048 : 768;
     const int rows2 = p->page_shift >= 4 && (p->cache_bf16 ? max_len <= fits : f <= PP_ROWS(2) * (long)p->n_seqs);
     const long blocks = (f / PP_ROWS(rows2 ? 2 : 4) + p->n_seqs) * p->kv_heads;
-    // 1.5 blocks of 128 rows for each CU (24 single tokens of 500 to 6001 positions, 8 heads a kv head, bf16: 59 us, as
-    // with 256 blocks; 512: 73; 4 chunks of 30 rows behind 970, fp32: 29.0, 31.9, 28.7), 1.25 of 64 (4 chunks of 30
-    // rows behind 470, bf16: 13.6 us, as with 256 blocks; 512: 14.8)
+    // 1.5 blocks of 128 rows for each CU (24 single tokens of 500 to 6001 positions, 8 heads a kv head, bf16: 66 us, as
+    // with 256 blocks; 512: 79; 4 chunks of 30 rows behind 970, fp32: 28.4, 31.5, 25.5), 1.25 of 64 (4 chunks of 30
+    // rows behind 470, bf16: 14.2 us, as with 256 blocks; 512: 15.9)
     long n = ((rows2 ? 320 : 384) + blocks - 1) / blocks;
     if (n > QK_PAGED_MAX_SPLIT) n = QK_PAGED_MAX_SPLIT;
     long c = (max_len + n - 1) / n;
     c = (c + 63) / 64 * 64;
     if (c < 64) c = 64;
-    // one block where that saves the join's launch (30 rows, 100 positions: bf16 9.4 us against 11.7, fp32 rows 12.1
-    // against 13.4, but on an fp32 cache 20.1 against 19.2; 130 positions, fp32 rows: 13.9, 13.6)
+    // one block where that saves the join's launch (30 rows, 100 positions: bf16 10.2 us against 13.5, fp32 rows 11.7
+    // against 14.3, but on an fp32 cache 18.8 against 18.6, and of 130 positions 22.7 against 18.5)
     if (p->cache_bf16 && max_len <= 128) c = 128;
     n = (max_len + c - 1) / c;
     *nsplit = n < 1 ? 1 : (int)n;
@@ -817,7 +821,7 @@ static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
 
 extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     if (!a->pg.cache_bf16) {
-        if (a->act_bf16) return prefill_launch<uint16_t, float, 4>(a, s);        // 31 rows behind 600: 64 rows a block 16.4 us, 15.0
+        if (a->act_bf16) return prefill_launch<uint16_t, float, 4>(a, s);        // 31 rows behind 600: 64 rows a block 17.6 us, 16.4; 16 of 16 to 32: 33.0, 27.8
         return a->rows2 ? prefill_launch<float, float, 2>(a, s) : prefill_launch<float, float, 4>(a, s);
     }
     if (a->rows2) return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 2>(a, s) : prefill_launch<float, uint16_t, 2>(a, s);

@@ -30,11 +30,12 @@
 // A row whose threshold classes hold more than SM_CAND entries (nearly equal
 // logits) takes a radix selection over the row in the last launch instead.
 //
-// Bound by the launches for one row (151936 entries: 4 + 5 + 7 + 7 us), by the arithmetic
-// of the weights for many (about 40 vector instructions each, in hist for every
-// entry, in pick for those kept) beside three readings of the rows for many (64 rows:
-// 9 + 15 + 18 + 9 us, where one reading takes 8).  Rows that take the first entry
-// alone (temperature 0, top-k 1) ask for no classes: 17 us for one, 29 for 64.
+// Bound by four kernels in a row for one row (151936 entries: 4 + 5 + 7 + 7 us, where a
+// call of one launch takes 8), and for many by three readings of the rows and the last
+// kernel's one block a row (64 rows: 9 + 15 + 18 + 9 us, where one reading takes 8), more than by
+// the arithmetic of the weights (about 40 vector instructions each, in hist for every
+// entry, in pick for those kept: hist takes 10 of its 15 us without any).  Rows that take
+// the first entry alone (temperature 0, top-k 1) ask for no classes: 17 us for one, 29 for 64.
 #include "common.h"
 #include "qk_kernels.h"
 #include "qwen_asr_hip.h"
