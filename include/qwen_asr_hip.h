@@ -529,6 +529,15 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
                           int heads, const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
                           const float *sin_vals, int n_pos, hipStream_t s);
 
+/* The same with a rotation position for each row (rope_pos [rows], device), which is not the
+ * position that it sits at: the drafts of a tree, which sit one behind the other and
+ * turn by their depth (kv_len - rows of the sequence + depth).  The tables are needed.  A
+ * row with a rotation position outside 0 .. n_pos - 1 is left out altogether. */
+int qwen_hip_paged_append_at(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, const int *rope_pos,
+                             void *q_out, const void *q, const void *k, const void *v, int dtype, long q_stride,
+                             long kv_stride, int heads, const float *q_norm, const float *k_norm, float eps,
+                             const float *cos_vals, const float *sin_vals, int n_pos, hipStream_t s);
+
 /* Causal attention over the cache, q and out [rows][heads * head_dim] of
  * `dtype` (out apart from q): a row sees the positions up to its own that are there;
  * one that sees none gets 0.  heads is a multiple of kv_heads; `scale` positive,
@@ -553,6 +562,27 @@ int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_
 int qwen_hip_paged_attention_prefill(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
                                      const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
                                      hipStream_t s);
+
+/* Attention over a window: as the two above (row_start NULL: one row per sequence; given:
+ * packed rows), but a row at position p sees only the positions p - window + 1 .. p and
+ * the first `sinks` ones (0 .. sinks - 1, up to p).  window > 0, sinks >= 0.  Pages that hold
+ * no position that a row sees are not read: their ids may be -1, so a stream that does
+ * not end keeps a window's pages and the first ones. */
+size_t qwen_hip_paged_attention_window_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads,
+                                                int window, int sinks);
+int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
+                                    const void *q, int dtype, int heads, float scale, int window, int sinks, void *ws,
+                                    size_t ws_bytes, hipStream_t s);
+
+/* Attention of drafted tokens, packed rows as in _prefill (or one a sequence): row i of a
+ * sequence's n sees the positions before its drafts (those below kv_len - n), and of the n drafts
+ * the ones whose bit is set in its `words` 64-bit words (tree [rows][words], device, 8-byte
+ * aligned; draft d is bit d % 64 of word d / 64; words 1 .. 4).  A tree's row has the bits of
+ * itself and its ancestors; any other bits do as well, and a row that sees nothing gets 0. */
+size_t qwen_hip_paged_attention_tree_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);
+int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out, const void *q,
+                                  int dtype, int heads, float scale, const uint64_t *tree, int words, void *ws,
+                                  size_t ws_bytes, hipStream_t s);
 
 /* One token per row of logits [rows][vocab] (rows row_stride entries apart), as
  * given by the row's parameters (device arrays [rows], each may be NULL: off):

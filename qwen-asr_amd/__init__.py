@@ -139,6 +139,11 @@ SIGNATURES = [
     ("qwen_hip_paged_attention_ws_bytes", C.c_size_t, [_vp, _vp, _i]),
     ("qwen_hip_paged_attention_decode", _i, [_vp] * 4 + [_i, _i, _f, _vp, C.c_size_t, _vp]),
     ("qwen_hip_paged_attention_prefill", _i, [_vp] * 4 + [_i, _i, _f, _vp, C.c_size_t, _vp]),
+    ("qwen_hip_paged_append_at", _i, [_vp] * 7 + [_i, C.c_long, C.c_long, _i, _vp, _vp, _f, _vp, _vp, _i, _vp]),
+    ("qwen_hip_paged_attention_window_ws_bytes", C.c_size_t, [_vp, _vp, _i, _i, _i]),
+    ("qwen_hip_paged_attention_window", _i, [_vp] * 4 + [_i, _i, _f, _i, _i, _vp, C.c_size_t, _vp]),
+    ("qwen_hip_paged_attention_tree_ws_bytes", C.c_size_t, [_vp, _vp, _i]),
+    ("qwen_hip_paged_attention_tree", _i, [_vp] * 4 + [_i, _i, _f, _vp, _i, _vp, C.c_size_t, _vp]),
     ("qwen_hip_sample_ws_bytes", C.c_size_t, [_i, _i]),
     ("qwen_hip_sample", _i, [_vp, _vp, C.c_long, _i, _i] + [_vp] * 6 + [C.c_size_t, _vp]),
     ("qwen_synth_key", _u64, [_u64, _u64]),

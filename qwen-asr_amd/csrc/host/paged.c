@@ -1,7 +1,8 @@
 /*
  * paged.c - op-level ABI of the paged KV cache: appending rows, attention of
- * single tokens and of packed prompts.  No counterpart in the reference, which
- * keeps one contiguous cache for one stream (qwen_asr_decoder.c:122-160).
+ * single tokens and of packed prompts, over all positions, over a window, of
+ * drafted trees.  No counterpart in the reference, which keeps one contiguous
+ * cache for one stream (qwen_asr_decoder.c:122-160).
  *
  * Host checks cover everything the host can see (types, shapes, alignment,
  * the workspace's size).  Lengths, row starts and page ids are device data:
@@ -58,11 +59,10 @@ static int paged_pointers(const char *op, const qk_paged *p) {
     return 0;
 }
 
-int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *q_out, const void *q,
-                          const void *k, const void *v, int dtype, long q_stride, long kv_stride, int heads,
-                          const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
-                          const float *sin_vals, int n_pos, hipStream_t s) {
-    static const char op[] = "paged_append";
+static int append(const char *op, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, const int *rope_pos,
+                  void *q_out, const void *q, const void *k, const void *v, int dtype, long q_stride, long kv_stride,
+                  int heads, const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
+                  const float *sin_vals, int n_pos, hipStream_t s) {
     qk_paged_append_args a = {0};
     const int rc = paged_view(op, kv, batch, heads, dtype, &a.pg);
     if (rc) return rc;
@@ -96,8 +96,28 @@ int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batc
     a.cos_v = cos_vals;
     a.sin_v = sin_vals;
     a.eps = eps;
+    a.rope_pos = cos_vals ? rope_pos : NULL;
     QK_TRY(qk_paged_append_launch(&a, s));
     return 0;
+}
+
+int qwen_hip_paged_append(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *q_out, const void *q,
+                          const void *k, const void *v, int dtype, long q_stride, long kv_stride, int heads,
+                          const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
+                          const float *sin_vals, int n_pos, hipStream_t s) {
+    return append("paged_append", kv, batch, NULL, q_out, q, k, v, dtype, q_stride, kv_stride, heads, q_norm, k_norm, eps,
+                  cos_vals, sin_vals, n_pos, s);
+}
+
+int qwen_hip_paged_append_at(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, const int *rope_pos,
+                             void *q_out, const void *q, const void *k, const void *v, int dtype, long q_stride,
+                             long kv_stride, int heads, const float *q_norm, const float *k_norm, float eps,
+                             const float *cos_vals, const float *sin_vals, int n_pos, hipStream_t s) {
+    static const char op[] = "paged_append_at";
+    if (kv && batch && kv->n_seqs > 0 && batch->rows > 0 && (!rope_pos || !cos_vals))
+        QK_REFUSE("%s: no rotation positions or no rotation tables", op);
+    return append(op, kv, batch, rope_pos, q_out, q, k, v, dtype, q_stride, kv_stride, heads, q_norm, k_norm, eps,
+                  cos_vals, sin_vals, n_pos, s);
 }
 
 /*
@@ -118,8 +138,15 @@ static int tokens_by_matrix(int cache_bf16, int group) { return cache_bf16 && gr
  * < 2 R T: for prompts 2 x 128 x 384, for single tokens 2 x 8 x 2048 (fewer heads a block: as many).
  * Times 520 bytes, that is below QWEN_HIP_PAGED_ATTENTION_WS_MAX for any batch.
  */
-static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int *rows2, int *nsplit, int *chunk) {
+static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int window, int sinks, int *rows2,
+                             int *nsplit, int *chunk) {
     if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;
+    if (window) {
+        /* what a block walks at most, about: the window and the first positions, and of packed rows as many
+         * positions more as a block has rows, and tiles that are seen in part */
+        const long most = (long)window + sinks + (matrix ? 128 * p->kv_heads / heads + 62 : 0);
+        if (most < max_len) max_len = (int)most;
+    }
     *rows2 = 0;
     if (matrix) *rows2 = qk_paged_prefill_plan(p, heads, max_len, nsplit, chunk);
     else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
@@ -127,30 +154,38 @@ static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_l
     return (size_t)p->rows * heads * *nsplit * (QWEN_HIP_HEAD_DIM + 2) * sizeof(float);
 }
 
+static int by_matrix(const qk_paged *p, int drafts, int heads) {
+    return drafts || p->row_start || tokens_by_matrix(p->cache_bf16, heads / p->kv_heads);
+}
+
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
     int rows2, nsplit, chunk;
     if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
-    const int matrix = p.row_start || tokens_by_matrix(p.cache_bf16, heads / p.kv_heads);
-    return attention_plan(&p, matrix, heads, batch->max_len, &rows2, &nsplit, &chunk);
+    const int matrix = by_matrix(&p, 0, heads);
+    return attention_plan(&p, matrix, heads, batch->max_len, 0, 0, &rows2, &nsplit, &chunk);
 }
 
-static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch,
-                     void *out, const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
-                     hipStream_t s) {
-    qk_paged_attn_args a = {0};
+/* kind: single tokens, packed rows, either, a tree's drafts (those by a.window and a.tree of `mask`) */
+enum { TOKENS, PACKED, EITHER, DRAFTS };
+
+static int attention(const char *op, int kind, const qk_paged_attn_args *mask, const qwen_hip_paged_kv *kv,
+                     const qwen_hip_paged_batch *batch, void *out, const void *q, int dtype, int heads, float scale,
+                     void *ws, size_t ws_bytes, hipStream_t s) {
+    qk_paged_attn_args a = *mask;
     const int rc = paged_view(op, kv, batch, heads, dtype, &a.pg);
     if (rc) return rc;
-    if (prefill && !batch->row_start) QK_REFUSE("%s: no row_start", op);
-    if (!prefill && batch->row_start) QK_REFUSE("%s: one row per sequence: row_start has to be NULL", op);
+    if (kind == PACKED && !batch->row_start) QK_REFUSE("%s: no row_start", op);
+    if (kind == TOKENS && batch->row_start) QK_REFUSE("%s: one row per sequence: row_start has to be NULL", op);
     if (!(scale >= 1e-30f && scale <= 1e30f)) QK_REFUSE("%s: scale %g", op, (double)scale);
     if (no_call(&a.pg)) return 0;
     if (paged_pointers(op, &a.pg)) return QWEN_HIP_EINVAL;
     if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);
     if (out == q) QK_REFUSE("%s: out cannot be q", op);
-    const int matrix = prefill || tokens_by_matrix(a.pg.cache_bf16, heads / a.pg.kv_heads);
-    const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, &a.rows2, &a.nsplit, &a.chunk);
+    if (kind == DRAFTS && !a.tree) QK_REFUSE("%s: no tree", op);
+    const int matrix = by_matrix(&a.pg, kind == DRAFTS, heads);
+    const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, a.window, a.sinks, &a.rows2, &a.nsplit, &a.chunk);
     if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);
     a.out = out;
@@ -169,11 +204,54 @@ static int attention(const char *op, int prefill, const qwen_hip_paged_kv *kv, c
 int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
                                     const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
                                     hipStream_t s) {
-    return attention("paged_attention_decode", 0, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+    const qk_paged_attn_args all = {0};
+    return attention("paged_attention_decode", TOKENS, &all, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
 }
 
 int qwen_hip_paged_attention_prefill(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
                                      const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
                                      hipStream_t s) {
-    return attention("paged_attention_prefill", 1, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+    const qk_paged_attn_args all = {0};
+    return attention("paged_attention_prefill", PACKED, &all, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+}
+
+/* a window of more positions than a length can name, and more first positions than a table holds, are as good as those */
+static int first_positions(int sinks) { return sinks < MAX_CAPACITY ? sinks : (int)MAX_CAPACITY; }
+
+size_t qwen_hip_paged_attention_window_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads,
+                                                int window, int sinks) {
+    qk_paged p;
+    int rows2, nsplit, chunk;
+    if (window <= 0 || sinks < 0 ||
+        paged_view("paged_attention_window_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p))
+        return 0;
+    return attention_plan(&p, by_matrix(&p, 0, heads), heads, batch->max_len, window, first_positions(sinks), &rows2,
+                          &nsplit, &chunk);
+}
+
+int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
+                                    const void *q, int dtype, int heads, float scale, int window, int sinks, void *ws,
+                                    size_t ws_bytes, hipStream_t s) {
+    static const char op[] = "paged_attention_window";
+    if (window <= 0 || sinks < 0) QK_REFUSE("%s: a window of %d positions, %d first ones", op, window, sinks);
+    const qk_paged_attn_args a = {.window = window, .sinks = first_positions(sinks)};
+    return attention(op, EITHER, &a, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+}
+
+size_t qwen_hip_paged_attention_tree_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
+    qk_paged p;
+    int rows2, nsplit, chunk;
+    if (paged_view("paged_attention_tree_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
+    return attention_plan(&p, 1, heads, batch->max_len, 0, 0, &rows2, &nsplit, &chunk);
+}
+
+int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out, const void *q,
+                                  int dtype, int heads, float scale, const uint64_t *tree, int words, void *ws,
+                                  size_t ws_bytes, hipStream_t s) {
+    static const char op[] = "paged_attention_tree";
+    if (words <= 0 || words > QK_TREE_WORDS / 2) QK_REFUSE("%s: %d words of bits a row (1 .. %d)", op, words, QK_TREE_WORDS / 2);
+    if ((uintptr_t)tree % 8) QK_REFUSE("%s: the tree is not 8-byte aligned", op);
+    /* little-endian: bit i of a row is bit i % 32 of its 32-bit word i / 32 */
+    const qk_paged_attn_args a = {.tree = (const uint32_t *)tree, .tree_words = 2 * words};
+    return attention(op, DRAFTS, &a, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
 }

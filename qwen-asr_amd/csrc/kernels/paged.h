@@ -70,3 +70,21 @@ __device__ __forceinline__ void pg_store4(uint16_t *p, float4 v) {
 __device__ __forceinline__ float pg_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 
 #define PG_LOG2E 1.44269504088896341f
+
+// The positions that the rows `first` .. `last` (of one sequence, `end` positions there) see of a
+// window and the first `sinks` positions, without the ones between, as 0 .. end - 1 of their own: v
+// stands for position v below `gap`, for v + shift from there on.  Both are multiples of UNIT (so
+// tiles of that many keys stay in order, and hold a few keys that no row sees).
+struct PgSeen {
+    int gap, shift, end;
+    __device__ __forceinline__ int at(int v) const { return v + (v >= gap ? shift : 0); }
+};
+// first position of the window of a row at position p
+__device__ __forceinline__ int pg_low(long p, int window) { return (int)max(p - window + 1, 0L); }
+template <int UNIT>
+__device__ __forceinline__ PgSeen pg_seen(const qk_paged_attn_args &a, long first, int end) {
+    const int low = pg_low(first, a.window) / UNIT * UNIT, gap = (a.sinks + UNIT - 1) / UNIT * UNIT;
+    if (low <= gap) return {0, 0, end};
+    if (low >= end) return {gap, 0, min(gap, end)};
+    return {gap, low - gap, end - (low - gap)};
+}

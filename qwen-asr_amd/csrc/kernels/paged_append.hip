@@ -28,6 +28,7 @@ struct PgAppend {
     const float *q_norm, *k_norm, *cos_v, *sin_v;
     float eps;
     int n_pos;
+    const int *rope_pos;
 };
 
 template <typename T, typename C>
@@ -55,6 +56,8 @@ __global__ __launch_bounds__(256) void paged_append(PgAppend<T> a) {
         wl = pg_load4(nw + 4 * c);
         wh = pg_load4(nw + 64 + 4 * c);
     }
+    // drafts of one depth turn alike, wherever they sit
+    const int turn = a.rope_pos ? a.rope_pos[row] : 0;
     int s = row, start = row, stop = row + 1;
     if (pg.row_start) {
         s = pg_search<16>(pg.n_seqs, row, [&](int i) { return (long)pg.row_start[i]; });
@@ -66,13 +69,14 @@ __global__ __launch_bounds__(256) void paged_append(PgAppend<T> a) {
     // rows before the first or behind the last sequence are left as they are
     if (!on || s < 0 || s >= pg.n_seqs || row >= stop) return;
     const long p = (long)pg_len(pg, s) - ((long)stop - row);
-    if (p < 0 || p >= a.n_pos || p >= pg.capacity) return;
+    const long by = a.rope_pos ? (long)turn : p;
+    if (p < 0 || p >= pg.capacity || by < 0 || by >= a.n_pos) return;
     const int pos = (int)p;
     const int pid = is_q ? 0 : pg_page(pg, s, pos);
     float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.cos_v) {
-        c4 = pg_load4(a.cos_v + (size_t)pos * PG_HD + 4 * c);
-        s4 = pg_load4(a.sin_v + (size_t)pos * PG_HD + 4 * c);
+        c4 = pg_load4(a.cos_v + (size_t)by * PG_HD + 4 * c);
+        s4 = pg_load4(a.sin_v + (size_t)by * PG_HD + 4 * c);
     }
     if (nw) {
         norm_rope_row16(lo, hi, wl, wh, c4, s4, a.eps);
@@ -100,7 +104,8 @@ __global__ __launch_bounds__(256) void paged_append(PgAppend<T> a) {
 template <typename T>
 static int append_launch(const qk_paged_append_args *x, hipStream_t s) {
     const PgAppend<T> a = {x->pg, (T *)x->q_out, (const T *)x->q, (const T *)x->k, (const T *)x->v, x->q_stride,
-                           x->kv_stride, x->heads, x->q_norm, x->k_norm, x->cos_v, x->sin_v, x->eps, x->n_pos};
+                           x->kv_stride, x->heads, x->q_norm, x->k_norm, x->cos_v, x->sin_v, x->eps, x->n_pos,
+                           x->rope_pos};
     const long blocks = ((long)(x->heads + x->pg.kv_heads) * x->pg.rows + 15) / 16;
     if (blocks > 0x7fffffffL) return QWEN_HIP_EINVAL;
     if (x->pg.cache_bf16) paged_append<T, uint16_t><<<(unsigned)blocks, 256, 0, s>>>(a);

@@ -67,7 +67,8 @@ __device__ __forceinline__ int pd_chunk(int len, int chunk, int nsplit) {
     return max(chunk, (need + 63) & ~63);
 }
 
-template <typename T, typename C, int GT, int L, int U, bool NT>
+// WIN: of a window and the first positions.
+template <typename T, typename C, int GT, int L, int U, bool NT, bool WIN>
 __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gchunks) {
     // dims a lane, in NC chunks of 16 bytes (CD dims); keys a wave at once
     constexpr int D = PG_HD / L, CD = PdRaw<C>::N, NC = D / CD, KEYS = 64 / L;
@@ -79,7 +80,17 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
     const int g0 = blockIdx.x % gchunks * GT, gn = min(GT, G - g0);
     const int h0 = kvh * G + g0, split = blockIdx.y;
     const size_t qrow = (size_t)s * a.heads + h0;
-    const int len = min(pg_len(pg, s), pg.capacity);
+    int len = min(pg_len(pg, s), pg.capacity);
+    PgSeen seen = {};
+    if constexpr (WIN) {
+        seen = pg_seen<1>(a, (long)pg_len(pg, s) - 1, len);
+        len = seen.end;
+    }
+    // position of the key `i` that the row sees
+    auto place = [&](int i) {
+        if constexpr (WIN) return seen.at(i);
+        else return i;
+    };
     const int chunk = pd_chunk(len, a.chunk, a.nsplit);
     const long first = (long)split * chunk;
     if (first >= len && split > 0) {
@@ -102,7 +113,7 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
     int pid[U];
     auto ids = [&](int kb) {
 #pragma unroll
-        for (int u = 0; u < U; u++) pid[u] = k1 > k0 ? table[min(kb + KEYS * u + grp, k1 - 1) >> pg.page_shift] : -1;
+        for (int u = 0; u < U; u++) pid[u] = k1 > k0 ? table[place(min(kb + KEYS * u + grp, k1 - 1)) >> pg.page_shift] : -1;
     };
     ids(k0 + wave * TURN);
 
@@ -139,7 +150,7 @@ __global__ __launch_bounds__(256) void paged_decode(qk_paged_attn_args a, int gc
             const int key = kb + KEYS * u + grp;
             const bool page = (unsigned)pid[u] < (unsigned)pg.n_pages;
             on[u] = page && key < k1;
-            const size_t row = (unsigned)((page ? pid[u] : 0) * rstride + (min(key, k1 - 1) & smask));
+            const size_t row = (unsigned)((page ? pid[u] : 0) * rstride + (place(min(key, k1 - 1)) & smask));
 #pragma unroll
             for (int i = 0; i < NC; i++) {
                 kr[u][i].template load<NT>(kp + row * PG_HD + CD * L * i);
@@ -369,18 +380,29 @@ extern "C" void qk_paged_decode_plan(int n_seqs, int heads, int kv_heads, int ca
     *chunk = (int)c;
 }
 
-template <typename T, typename C>
+template <typename T, typename C, bool WIN>
 static void decode_dispatch(const qk_paged_attn_args *a, hipStream_t s) {
     const int G = a->heads / a->pg.kv_heads, gt = decode_gt(G), gc = (G + gt - 1) / gt;
     const dim3 grid((unsigned)(a->pg.rows * a->pg.kv_heads * gc), (unsigned)a->nsplit);
     constexpr int L = sizeof(C) == 4 ? 16 : 8, U = sizeof(C) == 4 ? 4 : 2;
-    if (gt == 1) paged_decode<T, C, 1, L, U, true><<<grid, 256, 0, s>>>(*a, gc);
-    else if (gt == 2) paged_decode<T, C, 2, L, U, true><<<grid, 256, 0, s>>>(*a, gc);
-    else if (gt == 4) paged_decode<T, C, 4, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+    if (gt == 1) paged_decode<T, C, 1, L, U, true, WIN><<<grid, 256, 0, s>>>(*a, gc);
+    else if (gt == 2) paged_decode<T, C, 2, L, U, true, WIN><<<grid, 256, 0, s>>>(*a, gc);
+    else if (gt == 4) paged_decode<T, C, 4, 16, 4, true, WIN><<<grid, 256, 0, s>>>(*a, gc);
     else if constexpr (sizeof(C) == 4) {              // more than four heads on bf16 pages do not come here
-        if (gc == 1) paged_decode<T, C, 8, 16, 4, true><<<grid, 256, 0, s>>>(*a, gc);
+        if (gc == 1) paged_decode<T, C, 8, 16, 4, true, WIN><<<grid, 256, 0, s>>>(*a, gc);
         // every block of heads reads the rows: 16 heads, 24 sequences of 500 to 6001: 153 us, 166 past the caches
-        else paged_decode<T, C, 8, 16, 4, false><<<grid, 256, 0, s>>>(*a, gc);
+        else paged_decode<T, C, 8, 16, 4, false, WIN><<<grid, 256, 0, s>>>(*a, gc);
+    }
+}
+
+template <bool WIN>
+static void decode_types(const qk_paged_attn_args *a, hipStream_t s) {
+    if (a->act_bf16) {
+        if (a->pg.cache_bf16) decode_dispatch<uint16_t, uint16_t, WIN>(a, s);
+        else decode_dispatch<uint16_t, float, WIN>(a, s);
+    } else {
+        if (a->pg.cache_bf16) decode_dispatch<float, uint16_t, WIN>(a, s);
+        else decode_dispatch<float, float, WIN>(a, s);
     }
 }
 
@@ -388,12 +410,7 @@ extern "C" int qk_paged_decode_launch(const qk_paged_attn_args *a, hipStream_t s
     const int G = a->heads / a->pg.kv_heads, gt = decode_gt(G);
     if ((long)a->pg.rows * a->pg.kv_heads * ((G + gt - 1) / gt) > 0x7fffffffL) return QWEN_HIP_EINVAL;
     if (a->pg.cache_bf16 && gt == 8) return QWEN_HIP_EINVAL;
-    if (a->act_bf16) {
-        if (a->pg.cache_bf16) decode_dispatch<uint16_t, uint16_t>(a, s);
-        else decode_dispatch<uint16_t, float>(a, s);
-    } else {
-        if (a->pg.cache_bf16) decode_dispatch<float, uint16_t>(a, s);
-        else decode_dispatch<float, float>(a, s);
-    }
+    if (a->window) decode_types<true>(a, s);
+    else decode_types<false>(a, s);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }

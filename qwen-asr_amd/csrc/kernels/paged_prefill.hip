@@ -293,9 +293,13 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
     return past != 0 && o.f0 >= 0;
 }
 
+// Which keys a row sees besides its being at or behind their position (causal): of a window and the
+// first positions; or, of drafted rows, the past and what its bits say.
+enum { PP_CAUSAL, PP_WINDOW, PP_TREE };
+
 // SMALL: pages that do not hold a wave's rows of a tile (fewer than 8 positions).  Two waves a SIMD, but for
 // 64-row blocks on fp32 pages, which LDS lets only one of onto a CU.
-template <typename T, typename C, bool SMALL, int WR>
+template <typename T, typename C, bool SMALL, int WR, int MASK>
 __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) void paged_prefill(qk_paged_attn_args a, int slots) {
     // terms of the queries, the keys, the probabilities, the values
     constexpr int NQ = PpTerms<T>::N, NK = PpTerms<C>::N, NP = NQ == 1 ? 2 : NQ, NV = NQ == 1 && NK == 3 ? 2 : NK;
@@ -321,7 +325,17 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
     if (f0 >= frows) return;
     const int off0 = len - n;                             // position of the sequence's first new row (< 0: sees nothing)
     const int lastf = min(f0 + ROWS, frows) - 1;
-    const int kend = min(max(off0 + lastf / G + 1, 0), pg.capacity);
+    int kend = min(max(MASK == PP_TREE ? len : off0 + lastf / G + 1, 0), pg.capacity);
+    PgSeen keys = {};
+    if constexpr (MASK == PP_WINDOW) {
+        keys = pg_seen<PP_KT>(a, (long)off0 + f0 / G, kend);
+        kend = keys.end;
+    }
+    // position of the key that stands at v of those to walk
+    auto place = [&](int v) {
+        if constexpr (MASK == PP_WINDOW) return keys.at(v);
+        else return v;
+    };
     const int need = (int)(((long)kend + a.nsplit - 1) / a.nsplit);
     const int chunk = max(a.chunk, (need + PP_KT - 1) / PP_KT * PP_KT), split = blockIdx.y;
     const int k0s = (int)min((long)split * chunk, (long)kend), k1 = (int)min((long)k0s + chunk, (long)kend);
@@ -340,6 +354,21 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         return;
     }
     const int pos_lo = off0 + fw / G;                     // the wave's first position (rows do not fall with f)
+    // a window's start for this lane's row, and the wave's last one
+    [[maybe_unused]] const int low = MASK == PP_WINDOW ? pg_low(pos, a.window) : 0,
+                               low_hi = MASK == PP_WINDOW ? pg_low((long)off0 + min(fw + 31, frows - 1) / G, a.window) : 0;
+    // a tree's bits of the block's rows (an odd stride keeps the lanes' reads on different banks)
+    constexpr int TSTRIDE = QK_TREE_WORDS + 3, TLOADS = MASK == PP_TREE ? (ROWS * QK_TREE_WORDS + PP_THREADS(WR) - 1) / PP_THREADS(WR) : 1;
+    __shared__ uint32_t tree_bits[MASK == PP_TREE ? ROWS * TSTRIDE : 1];
+    [[maybe_unused]] uint32_t tw[TLOADS];
+    [[maybe_unused]] const int tree_q0 = f0 / G, tree_n = (lastf / G - tree_q0 + 1) * a.tree_words, tree_row = (on ? qi - tree_q0 : 0) * TSTRIDE;
+    if constexpr (MASK == PP_TREE) {
+#pragma unroll
+        for (int i = 0; i < TLOADS; i++) {
+            const int at = (int)threadIdx.x + PP_THREADS(WR) * i;
+            tw[i] = at < tree_n ? a.tree[(size_t)(r0 + tree_q0) * a.tree_words + at] : 0u;
+        }
+    }
 
     bf16x8 q[8][NQ];
     const float sc = NQ == 1 ? a.scale * PG_LOG2E : 1.0f;
@@ -376,7 +405,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         const int left = k1 - (int)kt;
         int id[PIECES];
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) id[i] = table[min((int)kt + SROWS * i, k1 - 1) >> pg.page_shift];
+        for (int i = 0; i < PIECES; i++) id[i] = table[place(min((int)kt + SROWS * i, k1 - 1)) >> pg.page_shift];
         unsigned there = 0;
         own_ids = 0;
 #pragma unroll
@@ -396,12 +425,13 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         Where w = {};
         if constexpr (SMALL) {
             const int left = k1 - tile_k0(t);
-            w.id = table[min(tile_k0(t) + ql, k1 - 1) >> pg.page_shift];
+            if constexpr (MASK == PP_WINDOW) w.id = table[place(min(tile_k0(t) + ql, k1 - 1)) >> pg.page_shift];
+            else w.id = table[min(tile_k0(t) + ql, k1 - 1) >> pg.page_shift];
             w.seen = left >= PP_KT ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
             w.seen &= (unsigned)__ballot((unsigned)w.id < (unsigned)pg.n_pages);
         } else {
             if (t - ids_at >= 64) refill(t);
-            const int at = min(tile_k0(t) + SROWS * wave, k1 - 1) & smask;
+            const int at = place(min(tile_k0(t) + SROWS * wave, k1 - 1)) & smask;
             w.off = __builtin_amdgcn_readlane(own_ids, t - ids_at) * pstride + (size_t)at * ROWB;
             w.seen = (unsigned)__builtin_amdgcn_readlane(keys_there, t - ids_at);
         }
@@ -413,7 +443,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         if constexpr (!SMALL) {
             of_wave(pages[v] + w.off, (unsigned)min(r, max(k1 - 1 - key0, 0)) * ROWB);
         } else {
-            const int at = min(key0 + r, k1 - 1), i1 = __shfl(w.id, SROWS * wave + r, 64);
+            const int at = place(min(key0 + r, k1 - 1)), i1 = __shfl(w.id, SROWS * wave + r, 64);
             of_lane(pages[v] + ((unsigned)i1 < (unsigned)pg.n_pages ? i1 : 0) * pstride + (unsigned)(at & smask) * ROWB);
         }
     };
@@ -535,9 +565,27 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
     // running one only once a row has passed it by 2^8: p stays below that, no sum is the worse
     // for it, and most tiles leave the accumulators alone.
     auto softmax = [&](int k0, unsigned seen, auto guarded) {
-        if (seen != 0xffffffffu || k0 + PP_KT - 1 > pos_lo) {                  // wave-uniform
-            const int last = pos - k0;
-            const unsigned bits = (last >= 31 ? seen : last < 0 ? 0u : seen & ((2u << last) - 1)) >> (4 * hl);
+        bool part;                                                             // wave-uniform
+        if constexpr (MASK == PP_TREE) part = seen != 0xffffffffu || k0 + PP_KT > off0;
+        else part = seen != 0xffffffffu || k0 + PP_KT - 1 > pos_lo;
+        if constexpr (MASK == PP_WINDOW) part = part || (k0 < low_hi && k0 + PP_KT > a.sinks);
+        if (part) {
+            unsigned there = seen;
+            if constexpr (MASK == PP_TREE) {
+                // words of the row's bits, one of ones (the past) before them, one of zeros behind
+                const int d = k0 - off0, at = min((d + 32) >> 5, a.tree_words + 1);
+                if (d > -32) {
+                    const uint32_t *w = tree_bits + tree_row;
+                    there &= __builtin_amdgcn_alignbit(w[min(at + 1, a.tree_words + 1)], w[at], d & 31);
+                }
+            }
+            if constexpr (MASK == PP_WINDOW) {
+                const int before = low - k0, first = a.sinks - k0;
+                there &= (before <= 0 ? ~0u : before >= 32 ? 0u : ~0u << before) |
+                         (first <= 0 ? 0u : first >= 32 ? ~0u : (1u << first) - 1);
+            }
+            const int last = MASK == PP_TREE ? 31 : pos - k0;
+            const unsigned bits = (last >= 31 ? there : last < 0 ? 0u : there & ((2u << last) - 1)) >> (4 * hl);
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 if ((int)(bits << (31 - 8 * (r / 4) - r % 4)) >= 0) st[r] = -INFINITY;
@@ -663,7 +711,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
                     fetch(i + 3, next_k, 0, (i + 1) & 1);
                 }
                 if (i + 2 < nt) fetch(i + 2, next_v, 1, i & 1);
-                if (wave_on && i + 1 < nt) softmax(tile_k0(i + 1), seen, guarded);
+                if (wave_on && i + 1 < nt) softmax(place(tile_k0(i + 1)), seen, guarded);
                 // the last turn's loads are there
                 if (i + 3 < nt) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * RPL));
                 else if (i + 2 < nt) __builtin_amdgcn_s_waitcnt(vmcnt_imm(RPL));
@@ -676,7 +724,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
                 }
                 load(i + 2, next_k, 0, kr);
                 load(i + 1, next_v, 1, vr);
-                if (wave_on) softmax(tile_k0(i + 1), seen, guarded);
+                if (wave_on) softmax(place(tile_k0(i + 1)), seen, guarded);
                 put(0, kr);
                 put(1, vr);
             }
@@ -700,6 +748,17 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
             const float4 x0 = pg_load4(qp + 16 * t), x1 = pg_load4(qp + 16 * t + 4);
             const float v[8] = {x0.x * fs, x0.y * fs, x0.z * fs, x0.w * fs, x1.x * fs, x1.y * fs, x1.z * fs, x1.w * fs};
             pp_terms8<NQ, true>(v, q[t]);
+        }
+    }
+    if constexpr (MASK == PP_TREE) {
+#pragma unroll
+        for (int i = 0; i < TLOADS; i++) {
+            const int at = (int)threadIdx.x + PP_THREADS(WR) * i;
+            if (at < tree_n) tree_bits[at / a.tree_words * TSTRIDE + 1 + at % a.tree_words] = tw[i];
+        }
+        if (threadIdx.x < ROWS) {
+            tree_bits[threadIdx.x * TSTRIDE] = ~0u;
+            tree_bits[threadIdx.x * TSTRIDE + a.tree_words + 1] = 0u;
         }
     }
     walk(PpBool<false>());
@@ -804,7 +863,7 @@ extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, 
     return rows2;
 }
 
-template <typename T, typename C, int WR>
+template <typename T, typename C, int WR, int MASK>
 static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     const qk_paged &pg = a->pg;
     const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS(WR) + pg.n_seqs;
@@ -814,16 +873,22 @@ static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     // the plan takes 64 rows for pages of 16 positions and more
     constexpr bool SOME_SMALL = WR == 4;
     if (SOME_SMALL && (1 << pg.page_shift) < PP_KT / WR)
-        paged_prefill<T, C, SOME_SMALL, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
-    else paged_prefill<T, C, false, WR><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
+        paged_prefill<T, C, SOME_SMALL, WR, MASK><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
+    else paged_prefill<T, C, false, WR, MASK><<<grid, PP_THREADS(WR), 0, s>>>(*a, (int)slots);
     return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
 }
 
-extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
+template <int MASK>
+static int prefill_types(const qk_paged_attn_args *a, hipStream_t s) {
     if (!a->pg.cache_bf16) {
-        if (a->act_bf16) return prefill_launch<uint16_t, float, 4>(a, s);        // 31 rows behind 600: 64 rows a block 17.6 us, 16.4; 16 of 16 to 32: 33.0, 27.8
-        return a->rows2 ? prefill_launch<float, float, 2>(a, s) : prefill_launch<float, float, 4>(a, s);
+        if (a->act_bf16) return prefill_launch<uint16_t, float, 4, MASK>(a, s);        // 31 rows behind 600: 64 rows a block 17.6 us, 16.4; 16 of 16 to 32: 33.0, 27.8
+        return a->rows2 ? prefill_launch<float, float, 2, MASK>(a, s) : prefill_launch<float, float, 4, MASK>(a, s);
     }
-    if (a->rows2) return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 2>(a, s) : prefill_launch<float, uint16_t, 2>(a, s);
-    return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 4>(a, s) : prefill_launch<float, uint16_t, 4>(a, s);
+    if (a->rows2) return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 2, MASK>(a, s) : prefill_launch<float, uint16_t, 2, MASK>(a, s);
+    return a->act_bf16 ? prefill_launch<uint16_t, uint16_t, 4, MASK>(a, s) : prefill_launch<float, uint16_t, 4, MASK>(a, s);
+}
+
+extern "C" int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
+    if (a->tree) return prefill_types<PP_TREE>(a, s);
+    return a->window ? prefill_types<PP_WINDOW>(a, s) : prefill_types<PP_CAUSAL>(a, s);
 }

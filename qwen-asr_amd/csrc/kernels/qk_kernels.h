@@ -498,6 +498,7 @@ typedef struct {
     long q_stride, kv_stride;
     const float *q_norm, *k_norm, *cos_v, *sin_v;
     float eps;
+    const int *rope_pos;      /* [rows], NULL: rows turn by the position that they sit at */
 } qk_paged_append_args;
 int qk_paged_append_launch(const qk_paged_append_args *a, hipStream_t s);
 
@@ -513,7 +514,11 @@ typedef struct {
     int rows2;                /* prompts: blocks of 64 rows instead of 128 */
     int nsplit, chunk;        /* keys per split, unless a sequence is longer than nsplit of them */
     float *part_o, *part_ml;  /* nsplit > 1 */
+    int window, sinks;        /* window > 0: positions p - window + 1 .. p and 0 .. sinks - 1 of those up to p */
+    const uint32_t *tree;     /* [rows][tree_words]: drafts that a row sees besides the past, a bit each; NULL: causal */
+    int tree_words;           /* even, at most QK_TREE_WORDS */
 } qk_paged_attn_args;
+#define QK_TREE_WORDS 8
 #define QK_PAGED_MAX_SPLIT 64
 /* splits and keys per split for sequences of up to max_len positions */
 void qk_paged_decode_plan(int n_seqs, int heads, int kv_heads, int cache_bf16, int max_len, int *nsplit, int *chunk);
