@@ -584,6 +584,67 @@ int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_pa
                                   int dtype, int heads, float scale, const uint64_t *tree, int words, void *ws,
                                   size_t ws_bytes, hipStream_t s);
 
+/* ---- sequences that continue others ------------------------------------- */
+
+/* The next page table of a program whose sequences continue others (beams, branches), grow, end
+ * and begin.  Row s of the new table (n_out rows of kv->table_stride ids; n_out at most 1024)
+ * continues row parent[s] of kv->table (kv->n_seqs rows, kv_len positions each): it
+ * names the pages of that row's positions and then pages for new_rows[s] more (n: the
+ * length kv_len[parent[s]]; entries behind are dropped; len_out[s] = n + new_rows[s], what
+ * append and attention take as kv_len).  A parent outside [0, kv->n_seqs) (-1) is an
+ * empty sequence; parent NULL: row s continues row s (n_out == kv->n_seqs); new_rows NULL: none.
+ *   Pages are shared where rows continue the same positions.  A last page with free slots, which
+ * the new rows would write, is not: of the rows that have it as their last the last one keeps it
+ * (unless a row has it for positions behind, or `outside` names it), the others with new rows
+ * take a fresh page, and copies[s] = {page, fresh page, 0, slots} says what has to be copied
+ * (qwen_hip_paged_copy; {-1, -1, 0, 0}: nothing; copies [n_out][4], 16-byte aligned).
+ *   Fresh pages are those that no entry of the new table names and outside (bytes [n_pages],
+ * not 0: a page that the program holds besides; NULL: none) does not, lowest first, to the rows
+ * in order.  So a page is free as soon as no row names it, and the old table means nothing any
+ * more.  *missing (device) is how many pages there were not, or the table's rows had no
+ * room for (at most 2^31 - 1): their entries are -1, and a last page that could not be copied is lost to its row.
+ *   The same inputs give the same tables.  kv->k, kv->v may be NULL.  table_out and
+ * len_out do not overlap the table and kv_len.  The workspace is 0 bytes up to 2^19 pages.
+ * No rows: nothing to launch, *missing stays. */
+size_t qwen_hip_paged_fork_ws_bytes(const qwen_hip_paged_kv *kv, int n_out);
+int qwen_hip_paged_fork(const qwen_hip_paged_kv *kv, const int *kv_len, const int *parent, const int *new_rows,
+                        const unsigned char *outside, int n_out, int *table_out, int *len_out, int *copies, int *missing,
+                        void *ws, size_t ws_bytes, hipStream_t s);
+
+/* Copies of pages in n_layers layers at once (layers: a HOST array of 1 .. 64 caches of one shape): for
+ * each of copies[n_copies][4] = {from, to, first, slots} the keys and values of slots first ..
+ * first + slots - 1 of page `from`, to the same slots of page `to`, of all kv heads.
+ * One that names a page or slots that are none copies nothing.  A page that is written is
+ * no other copy's source or destination. */
+int qwen_hip_paged_copy(const qwen_hip_paged_kv *layers, int n_layers, const int *copies, int n_copies, hipStream_t s);
+
+/* The drafts of a tree that were accepted move up behind the past, in n_layers layers at once (as
+ * above; the layers share one table): sequence s's drafts are its last rows (batch, as for
+ * attention), path[s] (rows path_stride entries apart) names n_path[s] of them, ascending
+ * (draft 0 .. n - 1), and the i-th goes to position kv_len - n + i.  The list ends before an
+ * entry that is no draft or not above the one before it.  len_out[s] is the length with what was
+ * accepted (the sequence's positions behind it are free); it does not overlap kv_len.  A draft
+ * or a place without a page is left out of the moves.  The pages that are written belong
+ * to one sequence. */
+int qwen_hip_paged_compact(const qwen_hip_paged_kv *layers, int n_layers, const qwen_hip_paged_batch *batch, int *len_out,
+                           const int *path, long path_stride, const int *n_path, hipStream_t s);
+
+/* The n_out best continuations of each sequence's beams: candidates are the tokens of its `beams` rows
+ * of logits ([seqs * beams][vocab] of `dtype`, QWEN_HIP_ST_F32 or _BF16, rows row_stride entries
+ * apart), each with score[row] + logit - log(sum of e^logit over the row); by falling score, equal
+ * ones by row and token.  The k-th of sequence q goes to place q * n_out + k of parent (its row,
+ * as qwen_hip_paged_fork takes it), token and score_out (fp32).  A beam at its end
+ * (ended[row] in 0 .. vocab - 1; ended may be NULL) has one candidate: that token, with its
+ * score as it is.  Logits that are no number count as -infinity, +infinity as the largest fp32 number;
+ * what has the score -infinity is no candidate, nor has a beam one whose score is not finite.
+ * Places without a candidate get -1, -1, -infinity.  Scores are held and compared in 64 bits
+ * (exponentials in fp32).  beams and n_out up to 64, vocab up to 2^20, seqs * beams up to
+ * 2^16.  The same inputs give the same choice. */
+size_t qwen_hip_beam_select_ws_bytes(int seqs, int beams, int vocab, int n_out);
+int qwen_hip_beam_select(int *parent, int *token, float *score_out, const void *logits, int dtype, long row_stride,
+                         int seqs, int beams, int vocab, const float *score, const int *ended, int n_out, void *ws,
+                         size_t ws_bytes, hipStream_t s);
+
 /* One token per row of logits [rows][vocab] (rows row_stride entries apart), as
  * given by the row's parameters (device arrays [rows], each may be NULL: off):
  *   temperature  logits are divided by it; 0, negative or NaN: the largest logit

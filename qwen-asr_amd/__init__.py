@@ -144,6 +144,12 @@ SIGNATURES = [
     ("qwen_hip_paged_attention_window", _i, [_vp] * 4 + [_i, _i, _f, _i, _i, _vp, C.c_size_t, _vp]),
     ("qwen_hip_paged_attention_tree_ws_bytes", C.c_size_t, [_vp, _vp, _i]),
     ("qwen_hip_paged_attention_tree", _i, [_vp] * 4 + [_i, _i, _f, _vp, _i, _vp, C.c_size_t, _vp]),
+    ("qwen_hip_paged_fork_ws_bytes", C.c_size_t, [_vp, _i]),
+    ("qwen_hip_paged_fork", _i, [_vp] * 5 + [_i] + [_vp] * 5 + [C.c_size_t, _vp]),
+    ("qwen_hip_paged_copy", _i, [_vp, _i, _vp, _i, _vp]),
+    ("qwen_hip_paged_compact", _i, [_vp, _i, _vp, _vp, _vp, C.c_long, _vp, _vp]),
+    ("qwen_hip_beam_select_ws_bytes", C.c_size_t, [_i, _i, _i, _i]),
+    ("qwen_hip_beam_select", _i, [_vp] * 4 + [_i, C.c_long, _i, _i, _i, _vp, _vp, _i, _vp, C.c_size_t, _vp]),
     ("qwen_hip_sample_ws_bytes", C.c_size_t, [_i, _i]),
     ("qwen_hip_sample", _i, [_vp, _vp, C.c_long, _i, _i] + [_vp] * 6 + [C.c_size_t, _vp]),
     ("qwen_synth_key", _u64, [_u64, _u64]),

@@ -41,6 +41,10 @@ void qk_set_err(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
         return QWEN_HIP_EINVAL;                                                 \
     } while (0)
 
+/* the paged cache and the batch, checked, in the kernels' form (paged.c) */
+int qk_paged_view(const char *op, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *b, int heads, int dtype,
+                  qk_paged *p);
+
 static inline int qk_aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
 #endif

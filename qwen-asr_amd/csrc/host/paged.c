@@ -19,8 +19,8 @@
 static int is_dtype(int t) { return t == QWEN_HIP_ST_F32 || t == QWEN_HIP_ST_BF16; }
 
 /* the cache and the batch, checked, in the kernels' form */
-static int paged_view(const char *op, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *b, int heads,
-                      int dtype, qk_paged *p) {
+int qk_paged_view(const char *op, const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *b, int heads, int dtype,
+                  qk_paged *p) {
     if (!kv || !b) QK_REFUSE("%s: no cache or no batch", op);
     if (!is_dtype(kv->dtype) || !is_dtype(dtype))
         QK_REFUSE("%s: types are QWEN_HIP_ST_F32 or QWEN_HIP_ST_BF16 (rows %d, cache %d)", op, dtype, kv->dtype);
@@ -64,7 +64,7 @@ static int append(const char *op, const qwen_hip_paged_kv *kv, const qwen_hip_pa
                   int heads, const float *q_norm, const float *k_norm, float eps, const float *cos_vals,
                   const float *sin_vals, int n_pos, hipStream_t s) {
     qk_paged_append_args a = {0};
-    const int rc = paged_view(op, kv, batch, heads, dtype, &a.pg);
+    const int rc = qk_paged_view(op, kv, batch, heads, dtype, &a.pg);
     if (rc) return rc;
     const int unit = dtype == QWEN_HIP_ST_F32 ? 4 : 8;
     if (q_stride < (long)heads * QWEN_HIP_HEAD_DIM || kv_stride < (long)kv->kv_heads * QWEN_HIP_HEAD_DIM ||
@@ -161,7 +161,7 @@ static int by_matrix(const qk_paged *p, int drafts, int heads) {
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
     int rows2, nsplit, chunk;
-    if (paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
+    if (qk_paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
     const int matrix = by_matrix(&p, 0, heads);
     return attention_plan(&p, matrix, heads, batch->max_len, 0, 0, &rows2, &nsplit, &chunk);
 }
@@ -173,7 +173,7 @@ static int attention(const char *op, int kind, const qk_paged_attn_args *mask, c
                      const qwen_hip_paged_batch *batch, void *out, const void *q, int dtype, int heads, float scale,
                      void *ws, size_t ws_bytes, hipStream_t s) {
     qk_paged_attn_args a = *mask;
-    const int rc = paged_view(op, kv, batch, heads, dtype, &a.pg);
+    const int rc = qk_paged_view(op, kv, batch, heads, dtype, &a.pg);
     if (rc) return rc;
     if (kind == PACKED && !batch->row_start) QK_REFUSE("%s: no row_start", op);
     if (kind == TOKENS && batch->row_start) QK_REFUSE("%s: one row per sequence: row_start has to be NULL", op);
@@ -223,7 +223,7 @@ size_t qwen_hip_paged_attention_window_ws_bytes(const qwen_hip_paged_kv *kv, con
     qk_paged p;
     int rows2, nsplit, chunk;
     if (window <= 0 || sinks < 0 ||
-        paged_view("paged_attention_window_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p))
+        qk_paged_view("paged_attention_window_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p))
         return 0;
     return attention_plan(&p, by_matrix(&p, 0, heads), heads, batch->max_len, window, first_positions(sinks), &rows2,
                           &nsplit, &chunk);
@@ -241,7 +241,7 @@ int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_
 size_t qwen_hip_paged_attention_tree_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
     int rows2, nsplit, chunk;
-    if (paged_view("paged_attention_tree_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
+    if (qk_paged_view("paged_attention_tree_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
     return attention_plan(&p, 1, heads, batch->max_len, 0, 0, &rows2, &nsplit, &chunk);
 }
 

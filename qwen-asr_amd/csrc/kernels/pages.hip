@@ -1,0 +1,309 @@
+// pages.hip - the pages of a paged KV cache as a program's sequences change: page tables of
+// sequences that continue others, pages for their next rows, copies of pages that two of
+// them would write (in all layers), and accepted drafts that move up behind the past.
+//
+// Whole numbers and copies of bits: the results are exact.
+#include "paged.h"
+
+#include <limits.h>
+
+typedef uint32_t pages_u32x4 __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// paged_fork: row s of the new table continues row p = parent[s] of the old one.
+//
+//   keep     entries 0 .. ceil(len / P) - 1 of row p, len = kv_len[p], P positions a page
+//   held     a page is held where an entry of the new table or the program (`outside`) names it
+//   tail     the last kept page, where len % P > 0: new rows go to its free slots.  If the row has new
+//            rows and another one holds the page as well, the row takes a copy; of the rows that have it
+//            as their tail the last keeps it, unless a row holds it for positions past it
+//   fresh    entries up to ceil((len + new) / P) and tails that are copied or no page: the pages that are
+//            not held, lowest first, by row and entry
+//
+// Nothing is counted from call to call: what is held follows from the new table, so
+// a page that no row names is free again.
+//
+// One block: the work is a few thousand table entries (64 rows of 24 pages) between barriers, and what is
+// held is a bit a page, in LDS up to FK_LDS_PAGES pages, in the workspace beyond.
+// ---------------------------------------------------------------------------
+#define FK_THREADS 1024
+#define FK_WAVES (FK_THREADS / 64)
+
+// exclusive sum over the block's threads and the sum of all; part: FK_WAVES + 1 ints
+__device__ __forceinline__ int fk_scan(int v, int *part, int &all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int up = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(up, d, 64);
+        if (lane >= d) up += o;
+    }
+    __syncthreads();                                  // part is free again
+    if (lane == 63) part[wave] = up;
+    __syncthreads();
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < FK_WAVES; i++) {
+        const int p = part[i];
+        before += i < wave ? p : 0;
+        sum += p;
+    }
+    all = sum;
+    return before + up - v;
+}
+
+struct FkRow {
+    int first, count;                                 // entries that get fresh pages: first .. first + count - 1
+    int tail;                                         // page that is copied to the first of them, -1: none
+    int part;                                         // its slots
+};
+
+template <int LDS_WORDS>
+__global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
+    __shared__ unsigned bits[LDS_WORDS > 0 ? 2 * LDS_WORDS : 1];
+    __shared__ int tails[QK_PAGED_FORK_ROWS], offs[QK_PAGED_FORK_ROWS + 1], part[FK_WAVES];
+    __shared__ FkRow rows[QK_PAGED_FORK_ROWS];
+    __shared__ unsigned long long over;               // pages that the table has no room for
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int words = (a.n_pages + 31) >> 5;
+    unsigned *const held = LDS_WORDS > 0 ? bits : a.ws, *const whole = held + words;
+    // in the workspace the bits are set and read past the first cache, which atomics do not go through
+    auto get = [&](const unsigned *w) {
+        if constexpr (LDS_WORDS > 0) return *w;
+        else return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    auto set = [&](unsigned *w, int id) { atomicOr(w + (id >> 5), 1u << (id & 31)); };
+    for (int i = tid; i < 2 * words; i += FK_THREADS) {
+        if constexpr (LDS_WORDS > 0) held[i] = 0u;
+        else __hip_atomic_store(held + i, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if constexpr (LDS_WORDS == 0) __threadfence();
+
+    if (tid == 0) over = 0;
+
+    // a thread a row: how much of it is kept
+    const int P = 1 << a.page_shift;
+    const bool on = tid < a.n_out;
+    int p = -1, len = 0, fresh_rows = 0;
+    if (on) {
+        p = a.parent ? a.parent[tid] : tid;
+        p = (unsigned)p < (unsigned)a.n_in ? p : -1;
+        len = p >= 0 ? max(a.kv_len[p], 0) : 0;
+        fresh_rows = a.new_rows ? max(a.new_rows[tid], 0) : 0;
+    }
+    const int kept = (int)min(((long)len + P - 1) >> a.page_shift, (long)a.stride);
+    const int whole_pages = min(len >> a.page_shift, a.stride), slots = len & (P - 1);
+    if (on) {
+        tails[tid] = p;
+        rows[tid] = {whole_pages, kept, 0, 0};
+        const long end = (long)len + fresh_rows;
+        a.len_out[tid] = (int)min(end, (long)INT_MAX);
+        *reinterpret_cast<int4 *>(a.copies + 4 * tid) = make_int4(-1, -1, 0, 0);
+    }
+    __syncthreads();
+    // a wave a row: its entries, and which pages they hold
+    for (int s = wave; s < a.n_out; s += FK_WAVES) {
+        const int from = tails[s], n_whole = rows[s].first, n = rows[s].count;
+        const int *const in = a.table + (size_t)max(from, 0) * a.stride;
+        int *const out = a.table_out + (size_t)s * a.stride;
+        for (int e = lane; e < a.stride; e += 64) {
+            int id = e < n ? in[e] : -1;
+            id = (unsigned)id < (unsigned)a.n_pages ? id : -1;
+            out[e] = id;
+            if (id >= 0) {
+                set(held, id);
+                if (e < n_whole) set(whole, id);
+            }
+        }
+    }
+    if (a.outside) {
+        for (int i = tid; i < a.n_pages; i += FK_THREADS)
+            if (a.outside[i]) {
+                set(held, i);
+                set(whole, i);
+            }
+    }
+    if constexpr (LDS_WORDS == 0) __threadfence();
+    __syncthreads();
+    const int at = whole_pages;                       // the tail's entry, where it is in the table
+    const bool has_tail = on && slots > 0 && at < a.stride;
+    const int tail = has_tail ? a.table_out[(size_t)tid * a.stride + at] : -1;
+    if (on) tails[tid] = tail;
+    __syncthreads();
+    bool copied = false;
+    if (tail >= 0 && fresh_rows > 0) {
+        copied = get(whole + (tail >> 5)) >> (tail & 31) & 1u;
+        for (int j = tid + 1; j < a.n_out && !copied; j++) copied = tails[j] == tail;
+    }
+    FkRow r = {kept, 0, -1, 0};
+    if (on) {
+        const long need = ((long)len + fresh_rows + P - 1) >> a.page_shift;
+        if (has_tail && fresh_rows > 0 && (copied || tail < 0)) r.first = at;
+        r.count = fresh_rows > 0 ? max((int)min(need, (long)a.stride) - r.first, 0) : 0;
+        const long room = max((long)a.stride, ((long)len + P - 1) >> a.page_shift);
+        if (fresh_rows > 0 && need > room) atomicAdd(&over, (unsigned long long)(need - room));
+        if (copied) {
+            r.tail = tail;
+            r.part = slots;
+            a.table_out[(size_t)tid * a.stride + at] = -1;
+        }
+        rows[tid] = r;
+    }
+    int total;
+    const int off = fk_scan(r.count, part, total);
+    if (on) offs[tid] = off;
+    // free pages of this thread's words, in order
+    const int per = (words + FK_THREADS - 1) / FK_THREADS, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    auto free_bits = [&](int w) {
+        const unsigned f = ~get(held + w);
+        return w == words - 1 && (a.n_pages & 31) ? f & ((1u << (a.n_pages & 31)) - 1) : f;
+    };
+    int mine = 0, all;
+    for (int w = w0; w < w1; w++) mine += __popc(free_bits(w));
+    int rank = fk_scan(mine, part, all);
+    if (tid == 0) *a.missing = (int)min((long)over + max(total - all, 0), (long)INT_MAX);
+    for (int w = w0; w < w1 && rank < total; w++) {
+        for (unsigned f = free_bits(w); f && rank < total; f &= f - 1, rank++) {
+            const int id = 32 * w + __builtin_ctz(f);
+            int lo = 0, hi = a.n_out;                 // the last row whose fresh pages begin at rank or before
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (offs[mid] <= rank) lo = mid;
+                else hi = mid;
+            }
+            const FkRow x = rows[lo];
+            a.table_out[(size_t)lo * a.stride + x.first + (rank - offs[lo])] = id;
+            if (x.tail >= 0 && rank == offs[lo])
+                *reinterpret_cast<int4 *>(a.copies + 4 * lo) = make_int4(x.tail, id, 0, x.part);
+        }
+    }
+}
+
+#define FK_SMALL (1 << 16)                            // pages: 16 KB of bits
+#define FK_LDS_PAGES (1 << 19)
+
+extern "C" size_t qk_paged_fork_ws_bytes(int n_pages) {
+    return n_pages > FK_LDS_PAGES ? 2 * sizeof(unsigned) * (((size_t)n_pages + 31) / 32) : 0;
+}
+
+extern "C" int qk_paged_fork_launch(const qk_paged_fork_args *a, hipStream_t s) {
+    if (a->n_pages <= FK_SMALL) paged_fork<FK_SMALL / 32><<<1, FK_THREADS, 0, s>>>(*a);
+    else if (a->n_pages <= FK_LDS_PAGES) paged_fork<FK_LDS_PAGES / 32><<<1, FK_THREADS, 0, s>>>(*a);
+    else paged_fork<0><<<1, FK_THREADS, 0, s>>>(*a);
+    return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
+}
+
+// ---------------------------------------------------------------------------
+// paged_copy: slots first .. first + slots - 1 of a page to the same slots of another, keys and values
+// of all kv heads and layers.  Block (copy, layer and K or V, share of the page's 16-byte pieces).
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void paged_copy(qk_paged_layers L, const int *copies) {
+    const int4 c = *reinterpret_cast<const int4 *>(copies + 4 * (size_t)blockIdx.x);
+    if ((unsigned)c.x >= (unsigned)L.n_pages || (unsigned)c.y >= (unsigned)L.n_pages || c.x == c.y) return;
+    if (c.z < 0 || c.w <= 0 || c.z > (1 << L.page_shift) - c.w) return;
+    unsigned char *const base = (unsigned char *)(blockIdx.y & 1 ? L.v[blockIdx.y >> 1] : L.k[blockIdx.y >> 1]);
+    const int row = L.row_bytes / 16;                 // pieces of a row
+    const size_t head = (size_t)L.row_bytes << L.page_shift, page = head * L.kv_heads;
+    const unsigned char *const from = base + c.x * page + (size_t)c.z * L.row_bytes;
+    unsigned char *const to = base + c.y * page + (size_t)c.z * L.row_bytes;
+    const long piece = (long)c.w * row, n = piece * L.kv_heads;      // of a kv head, in all
+    const long step = 256L * gridDim.z;
+    for (long i0 = 256L * blockIdx.z + threadIdx.x; i0 < n; i0 += 4 * step) {
+        pages_u32x4 v[4];
+        size_t at[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const long i = min(i0 + j * step, n - 1), h = n >> 31 ? i / piece : (long)((unsigned)i / (unsigned)piece);
+            at[j] = h * head + 16 * (size_t)(i - h * piece);
+            v[j] = *reinterpret_cast<const pages_u32x4 *>(from + at[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i0 + j * step < n) *reinterpret_cast<pages_u32x4 *>(to + at[j]) = v[j];
+    }
+}
+
+extern "C" int qk_paged_copy_launch(const qk_paged_layers *L, const int *copies, int n, hipStream_t s) {
+    if (n > 0xffffff) return QWEN_HIP_EINVAL;         // a launch has fewer than 2^32 threads along an axis
+    // about 4096 blocks, none of less than 1024 pieces of a whole page
+    const long pieces = ((long)L->row_bytes / 16 * L->kv_heads) << L->page_shift, pairs = 2L * L->n_layers * n;
+    long z = (4096 + pairs - 1) / pairs, most = (pieces + 1023) / 1024;
+    z = z < most ? z : most;
+    paged_copy<<<dim3((unsigned)n, 2 * L->n_layers, (unsigned)z), 256, 0, s>>>(*L, copies);
+    return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
+}
+
+// ---------------------------------------------------------------------------
+// paged_compact: of a sequence's n drafts (positions past .. past + n - 1) those of `path`, ascending, move to
+// past, past + 1, ..  A thread owns 16 bytes of a row for all of them, in order and CP_ROWS at a time, loads
+// before stores: draft path[i] >= i has not been written over when it is read.
+// ---------------------------------------------------------------------------
+#define CP_ROWS 8
+#define CP_PART 256                                   // accepted drafts at a time
+
+__global__ __launch_bounds__(256) void paged_compact(qk_paged_layers L, qk_paged pg, int *len_out, const int *path,
+                                                     long path_stride, const int *n_path) {
+    __shared__ int from[CP_PART], to[CP_PART], bad;
+    const int s = blockIdx.x, tid = threadIdx.x;
+    int n = 1;
+    if (pg.row_start) {
+        const int a = min(max(pg.row_start[s], 0), pg.rows), b = min(max(pg.row_start[s + 1], 0), pg.rows);
+        n = max(b - a, 0);
+    }
+    const long past = (long)pg_len(pg, s) - n;
+    const int want = (int)min((long)max(n_path[s], 0), min((long)n, path_stride));
+    path += s * path_stride;
+    unsigned char *const base = (unsigned char *)(blockIdx.y & 1 ? L.v[blockIdx.y >> 1] : L.k[blockIdx.y >> 1]);
+    const int row = L.row_bytes / 16, col = (int)(256 * blockIdx.z + tid), h = col / row;
+    const bool on = h < L.kv_heads;
+    unsigned char *const mine = base + (((size_t)min(h, L.kv_heads - 1) << L.page_shift) * L.row_bytes) + 16 * (col % row);
+    // a row of the cache (of kv head 0) by its position, -1: none.  The host has seen that rows fit an int.
+    auto place = [&](long p) {
+        if (p < 0 || p >= pg.capacity) return -1;
+        const int id = pg_page(pg, s, (int)p);
+        return id < 0 ? -1 : id * (L.kv_heads << L.page_shift) + (int)(p & ((1 << L.page_shift) - 1));
+    };
+    int count = 0;                                    // accepted so far
+    for (int i0 = 0; i0 < want; i0 += CP_PART) {
+        const int m = min(want - i0, CP_PART);
+        __syncthreads();                              // the last part is read
+        if (tid == 0) bad = m;
+        __syncthreads();
+        if (tid < m) {
+            const int i = i0 + tid, d = path[i], before = i > 0 ? path[i - 1] : -1;
+            // the list ends at an entry that is no draft, or none behind the one before
+            if (d <= before || d >= n) atomicMin(&bad, tid);
+            const bool stays = d == i || d < 0 || d >= n;
+            from[tid] = stays ? -1 : place(past + d);
+            to[tid] = stays ? -1 : place(past + i);
+        }
+        __syncthreads();
+        const int good = bad;
+        for (int j0 = 0; j0 < good; j0 += CP_ROWS) {
+            pages_u32x4 v[CP_ROWS];
+            int t[CP_ROWS];                           // the same for the block
+#pragma unroll
+            for (int j = 0; j < CP_ROWS; j++) {
+                const int k = min(j0 + j, CP_PART - 1), f = __builtin_amdgcn_readfirstlane(from[k]);
+                t[j] = f >= 0 && j0 + j < good ? __builtin_amdgcn_readfirstlane(to[k]) : -1;
+                // what does not move is read at the pages' start, where it does no harm
+                v[j] = *reinterpret_cast<const pages_u32x4 *>(mine + (size_t)max(t[j] < 0 ? -1 : f, 0) * L.row_bytes);
+            }
+#pragma unroll
+            for (int j = 0; j < CP_ROWS; j++)
+                if (on && t[j] >= 0) *reinterpret_cast<pages_u32x4 *>(mine + (size_t)t[j] * L.row_bytes) = v[j];
+        }
+        count += good;
+        if (good < m) break;
+    }
+    if (blockIdx.y == 0 && blockIdx.z == 0 && tid == 0) len_out[s] = (int)max(past + count, 0L);
+}
+
+extern "C" int qk_paged_compact_launch(const qk_paged_layers *L, const qk_paged *pg, int *len_out, const int *path,
+                                       long path_stride, const int *n_path, hipStream_t s) {
+    const int cols = L->row_bytes / 16 * L->kv_heads;
+    if ((long)cols > 0xffffL * 256 || pg->n_seqs > 0xffffff) return QWEN_HIP_EINVAL;
+    paged_compact<<<dim3((unsigned)pg->n_seqs, 2 * L->n_layers, (cols + 255) / 256), 256, 0, s>>>(*L, *pg, len_out, path,
+                                                                                                path_stride, n_path);
+    return hipGetLastError() == hipSuccess ? 0 : QWEN_HIP_EDEVICE;
+}

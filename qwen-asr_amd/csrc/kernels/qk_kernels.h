@@ -529,6 +529,46 @@ int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s);
 /* joins the partials into out */
 int qk_paged_merge_launch(const qk_paged_attn_args *a, hipStream_t s);
 
+/* ---- pages of sequences that change ------------------------------------- */
+#define QK_PAGED_MAX_LAYERS 64
+#define QK_PAGED_FORK_ROWS 1024
+typedef struct {
+    const int *table, *kv_len;           /* [n_in][stride], [n_in] */
+    const int *parent, *new_rows;        /* [n_out], NULL: itself, none */
+    const unsigned char *outside;        /* [n_pages], NULL: none */
+    int *table_out, *len_out, *copies;   /* [n_out][stride], [n_out], [n_out][4] */
+    int *missing;
+    int n_in, n_out, stride, page_shift, n_pages;
+    unsigned *ws;
+} qk_paged_fork_args;
+size_t qk_paged_fork_ws_bytes(int n_pages);
+int qk_paged_fork_launch(const qk_paged_fork_args *a, hipStream_t s);
+
+/* the pages of several layers of one shape (a kernel argument: by value) */
+typedef struct {
+    void *k[QK_PAGED_MAX_LAYERS], *v[QK_PAGED_MAX_LAYERS];
+    int n_layers, n_pages, page_shift, kv_heads, row_bytes;
+} qk_paged_layers;
+int qk_paged_copy_launch(const qk_paged_layers *L, const int *copies, int n, hipStream_t s);
+int qk_paged_compact_launch(const qk_paged_layers *L, const qk_paged *pg, int *len_out, const int *path,
+                            long path_stride, const int *n_path, hipStream_t s);
+
+/* ---- beam selection ------------------------------------------------------ */
+#define QK_BEAM_MAX 64                   /* beams of a sequence, and places */
+typedef struct {
+    int *parent, *token;
+    float *score_out;
+    const void *logits;
+    int bf16;
+    long row_stride;
+    int seqs, beams, vocab, n_out;
+    const float *score;
+    const int *ended;                    /* NULL: none */
+    void *ws;
+} qk_beam_args;
+size_t qk_beam_ws_bytes(int seqs, int beams, int vocab, int n_out);
+int qk_beam_launch(const qk_beam_args *a, hipStream_t s);
+
 /* ---- drawing tokens ----------------------------------------------------- */
 typedef struct {
     int *tokens;
