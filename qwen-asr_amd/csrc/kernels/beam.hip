@@ -5,44 +5,53 @@
 //
 // by falling score, equal ones by (b, i).  One pass over the logits:
 //
-//   beam_rows    block (share of a row): its maximum and sum of exponentials, and its n largest entries
-//                in order.  Only entries from a threshold on are looked at: the n-th largest of the 64 lanes'
-//                maxima of a wave is no larger than the n-th largest entry, so it is a lower
-//                bound; in each of the four waves at most n lanes reach the largest such
-//                bound, so at most 4 n VPT entries do (as a rule about 2 n).
-//   beam_select  block (sequence): each beam's logarithm from its shares, and the n best of all shares'
-//                lists, by a threshold of the same kind.
+//   beam_rows    block (share of a row): its maximum and sum of exponentials, and its entries from a threshold
+//                on that n of them reach: with the threads in n groups or more, the least of the
+//                groups' maxima, which about 3 n do (of a share that leaves groups empty: the n-th
+//                largest of a wave's threads').  Where more than a list holds do, by equal values
+//                (forbidden entries of the type's lowest value), indexes enter a bound: of the threads' largest
+//                entries by value and index, the n-th in each wave, the largest of these; at most n
+//                threads of each wave reach it, and 4 n VPT entries.  More than 4 n (32) of them are brought in order
+//                and the first n kept.
+//   beam_select  block (sequence): each beam's logarithm from its shares; a bound from the shares' largest
+//                entries, the entries of the shares that reach it, and the n best of these.
 //
-// Exponentials: (x - M) log2(e) in 64 bits, its whole part into the exponent, v_exp_f32 (1 ulp) of the rest;
-// sums, logarithms and scores in 64 bits, in an order that does not depend on the run.
-// Entries are compared as whole numbers (the value's order in the upper half, the index below, the lower
-// one first), so equal ones are in order and every choice is unique.
+// Exponentials: log2(e) x in two fp32 terms, its whole part into the exponent, v_exp_f32 (1 ulp) of the rest, where the
+// share's maximum lies within 30 of 0 (no x is subtracted from then, so nothing is rounded before); otherwise of
+// x - M in 64 bits.  Pairs are added in fp32, everything else, logarithms and scores, in 64 bits, in an order that
+// does not depend on the run or on the rows' alignment: equal beams have equal scores.  Entries are
+// compared as whole numbers (the value's order in the upper half, the index below, the lower one
+// first), so equal ones are in order and every choice is unique.
 #include "common.h"
 #include "qk_kernels.h"
 #include "qwen_asr_hip.h"
 
+#include <limits.h>
 #include <math.h>
 
 #define BM_THREADS 256
 #define BM_WAVES 4
-#define BM_LIST 2048                  // entries from the threshold on: 4 n VPT at most
+#define BM_PART 512                   // entries from a threshold on of a wave: n VPT at most by one of value and index
 #define BM_LOG2E 1.4426950408889634
 
 typedef unsigned long long bm_u64;
 
-struct BmShare {                      // of a row: maximum (-inf: no entry), sum of e^(x - maximum)
-    double sum;
-    float max, pad;
+struct BmShare {                      // of a row
+    double sum;                       // of e^(x - ref)
+    float ref;
+    int count;                        // entries listed
+    bm_u64 best;                      // the largest entry; without an index (0 in its place) where it is not known; 0: none
 };
 
-// what is no number is no entry, +inf the largest number
-__device__ __forceinline__ float bm_clean(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f) + 0.0f; }
+// what is no number is no entry (the middle of three is the least one then), +inf the largest number
+__device__ __forceinline__ float bm_clean(float x) { return __builtin_amdgcn_fmed3f(x, -INFINITY, 3.402823466e38f); }
 
-// the order of entries: larger first, then the lower index; 0 is none
-__device__ __forceinline__ bm_u64 bm_key(float x, unsigned i) {
-    const unsigned u = __float_as_uint(x);
-    return (bm_u64)(u ^ ((unsigned)((int)u >> 31) | 0x80000000u)) << 32 | (0xffffffffu - i);
+// the order of values (-0 is 0), and of entries: larger first, then the lower index; 0 is none
+__device__ __forceinline__ unsigned bm_rank(float x) {
+    const unsigned u = __float_as_uint(x + 0.0f);
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ bm_u64 bm_key(float x, unsigned i) { return (bm_u64)bm_rank(x) << 32 | (0xffffffffu - i); }
 __device__ __forceinline__ float bm_value(bm_u64 key) {
     const unsigned u = (unsigned)(key >> 32);
     return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u);
@@ -57,11 +66,20 @@ __device__ __forceinline__ double bm_double(bm_u64 u) {
     return __longlong_as_double((long long)(u >> 63 ? u ^ 1ull << 63 : ~u));
 }
 
-// 2^t, t <= 0 or so
+// 2^t, -300 <= t < 127
 __device__ __forceinline__ float bm_exp2(double t) {
     const double magic = 6755399441055744.0, z = t + magic;      // 1.5 2^52: t's whole part in the low word
     const float f = (float)(t - (z - magic));
     return __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)(unsigned)(bm_u64)__double_as_longlong(z));
+}
+
+// e^x for |x| of tens, e^-80 below (nothing beside a largest one of e^-30): y + r = x log2(e), y's whole part z by
+// adding 1.5 2^23, into the exponent's place
+__device__ __forceinline__ float bm_exp(float x) {
+    const float magic = 12582912.0f, L = 1.44269504e+00f, L2 = 1.92596299e-08f;
+    x = fmaxf(x, -80.0f);
+    const float y = x * L, z = y + magic, r = fmaf(x, L2, fmaf(x, L, -y));
+    return __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f((y - (z - magic)) + r)) + (__float_as_uint(z) << 23));
 }
 
 __device__ __forceinline__ double bm_sum(double v) {             // of a wave, the same in every lane
@@ -87,39 +105,46 @@ __device__ __forceinline__ K bm_bound(K key, int n) {
 struct BmRows {
     const void *logits;
     long stride;
-    int vocab, n, shares;
+    int vocab, n, shares, width;   // entries of a share: a multiple of 8, BM_THREADS VPT at most
     const float *score;
     const int *ended;
     BmShare *share;                   // [rows][shares]
-    bm_u64 *list;                     // [rows][shares][n]
+    bm_u64 *list;                     // [rows][shares][bm_slots(n)]
+    bool late;                        // idle rows are found out behind the loads
 };
+
+// entries that a share lists at most: a power of two
+__host__ __device__ __forceinline__ int bm_slots_log(int n) { return n <= 8 ? 5 : n <= 16 ? 6 : n <= 32 ? 7 : 8; }
 
 // a beam that takes no part with its logits: one at its end, one without a score
 __device__ __forceinline__ bool bm_idle(const float *score, const int *ended, int row, int vocab) {
     const float s = score[row];
-    return !(fabsf(s) <= 3.402823466e38f) || (ended && (unsigned)ended[row] < (unsigned)vocab);
+    const int e = ended ? ended[row] : -1;
+    return !(fabsf(s) <= 3.402823466e38f) || (unsigned)e < (unsigned)vocab;
 }
 
 template <typename T, int VPT>
 __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     constexpr int V = 16 / sizeof(T), NV = VPT / V;              // entries of a load, loads
-    __shared__ float wmax[BM_WAVES];
-    __shared__ bm_u64 wbound[BM_WAVES], list[BM_LIST];
+    __shared__ float wmax[BM_WAVES], wleast[BM_WAVES];
+    __shared__ __attribute__((aligned(16))) bm_u64 list[BM_WAVES * BM_PART];
+    __shared__ bm_u64 wkey[BM_WAVES];
     __shared__ double wsum[BM_WAVES];
-    __shared__ int count;
+    __shared__ int count[BM_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int share = blockIdx.y, row = blockIdx.x;
     const T *const x0 = (const T *)a.logits + (size_t)row * a.stride;
-    if (bm_idle(a.score, a.ended, row, a.vocab)) return;
-    if (tid == 0) count = 0;
+    if (!a.late && bm_idle(a.score, a.ended, row, a.vocab)) return;
     // Shares and threads by index, whatever the row's alignment: equal rows have equal sums.  (Loads of 16 bytes
     // need no more alignment than the type's.)
-    auto index = [&](int j) { return share * BM_THREADS * VPT + (j * BM_THREADS + tid) * V; };
+    const int end = min((share + 1) * a.width, a.vocab);
+    auto index = [&](int j) { return share * a.width + (j * BM_THREADS + tid) * V; };
     float x[VPT];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        const int i = index(j);
-        if (i + V <= a.vocab) {
+        // The planes before the share's end have no condition on a lane: behind one, loads would wait for each other.
+        const int i = index(j), plane = share * a.width + j * BM_THREADS * V;
+        if (plane + BM_THREADS * V <= end) {
             unsigned u[4];
             __builtin_memcpy(u, x0 + i, 16);
 #pragma unroll
@@ -129,67 +154,144 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                float v = -INFINITY;
-                if (i + k < a.vocab) {
-                    if constexpr (V == 4) v = x0[i + k];
-                    else v = bf16_to_f32(x0[i + k]);
+            for (int k = 0; k < V; k++) x[V * j + k] = -INFINITY;
+            if (i + V <= end) {
+                unsigned u[4];
+                __builtin_memcpy(u, x0 + i, 16);
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    if constexpr (V == 4) x[V * j + k] = __uint_as_float(u[k]);
+                    else x[V * j + k] = k % 2 ? bf16_hi(u[k / 2]) : bf16_lo(u[k / 2]);
                 }
-                x[V * j + k] = v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    if (i + k < end) {
+                        if constexpr (V == 4) x[V * j + k] = x0[i + k];
+                        else x[V * j + k] = bf16_to_f32(x0[i + k]);
+                    }
             }
         }
     }
-    // the thread's largest entry (indexes rise with j and k: the first of equal ones stays)
+    if (a.late && bm_idle(a.score, a.ended, row, a.vocab)) return;
     float mx = -INFINITY;
-    int mi = 0;
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
         x[j] = bm_clean(x[j]);
-        if (x[j] > mx) {
-            mx = x[j];
-            mi = j;
-        }
+        mx = fmaxf(mx, x[j]);
     }
-    const bm_u64 top = mx > -INFINITY ? bm_key(mx, index(mi / V) + mi % V) : 0;
-    const float wm = wave_max(mx);
-    const bm_u64 bound = bm_bound<bm_u64, 64>(top, a.n);
+    // the least of the groups' maxima: 4, 8, 16, 32 or 64 groups of the block's threads
+    float g = mx, all = mx;
+    if (a.n > 4) {
+        g = group_max<4>(g);
+        if (a.n <= 32) g = group_max<8>(g);
+        if (a.n <= 16) g = group_max<16>(g);
+        if (a.n <= 8) g = group_max<32>(g);
+        all = wave_max(g);
+        g = -wave_max(-g);
+    } else {
+        g = all = wave_max(g);
+    }
     if (lane == 0) {
-        wmax[wave] = wm;
-        wbound[wave] = bound;
+        wmax[wave] = all;
+        wleast[wave] = g;
     }
     __syncthreads();
     const float M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    bm_u64 T0 = wbound[0];
+    float T0 = fminf(fminf(wleast[0], wleast[1]), fminf(wleast[2], wleast[3]));
+    if (T0 == -INFINITY) {
+        // groups without entries (the row's last share): the n-th largest of a wave's threads instead
+        const unsigned t = bm_bound<unsigned, 32>(mx > -INFINITY ? bm_rank(mx) : 0u, a.n);
+        if (lane == 0) wkey[wave] = t;
+        __syncthreads();
+        const bm_u64 most = max(max(wkey[0], wkey[1]), max(wkey[2], wkey[3]));
+        if (most) T0 = bm_value(most << 32);
+    }
+    T0 = fmaxf(T0, -3.402823466e38f);                 // what is -inf is no entry
+    // the wave's entries from there on, into its part of the list
+    bm_u64 *const part = list + BM_PART * wave;
+    int n_part = 0;
 #pragma unroll
-    for (int w = 1; w < BM_WAVES; w++) T0 = wbound[w] > T0 ? wbound[w] : T0;
+    for (int j = 0; j < VPT; j++) {
+        const bool in = x[j] >= T0;
+        const bm_u64 m = __ballot(in);
+        if (m) {
+            const int to = n_part + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0u));
+            if (in && to < BM_PART) part[to] = bm_key(x[j], index(j / V) + j % V);
+            n_part += __popcll(m);
+        }
+    }
+    if (lane == 0) count[wave] = n_part;
     double sum = 0.0;
-    if (M > -INFINITY) {
-        // differences in 64 bits; of what is far below nothing is left
+    const bool plain = fabsf(M) <= 30.0f;             // relative to 0, not to M
+    if (plain) {
+        float e[2];
+#pragma unroll
+        for (int j = 0; j < VPT; j++) {
+            e[j % 2] = bm_exp(x[j]);
+            if (j % 2) sum += (double)(e[0] + e[1]);
+        }
+    } else if (M > -INFINITY) {
 #pragma unroll
         for (int j = 0; j < VPT; j++) sum += (double)bm_exp2(fmax(((double)x[j] - (double)M) * BM_LOG2E, -300.0));
     }
     sum = bm_sum(sum);
     if (lane == 0) wsum[wave] = sum;
-    if (top >= T0 && top > 0) {
+    __syncthreads();
+    if (max(max(count[0], count[1]), max(count[2], count[3])) > BM_PART) {
+        // the thread's first largest entry
+        bm_u64 top = 0;
 #pragma unroll
         for (int j = 0; j < VPT; j++) {
             const bm_u64 key = bm_key(x[j], index(j / V) + j % V);
-            if (x[j] > -INFINITY && key >= T0) list[atomicAdd(&count, 1)] = key;
+            if (x[j] > -INFINITY && key > top) top = key;
         }
+        const bm_u64 t = bm_bound<bm_u64, 64>(top, a.n);
+        if (lane == 0) wkey[wave] = t;
+        __syncthreads();                              // every thread has seen the counts
+        bm_u64 T1 = wkey[0];
+#pragma unroll
+        for (int w = 1; w < BM_WAVES; w++) T1 = wkey[w] > T1 ? wkey[w] : T1;
+        n_part = 0;
+#pragma unroll
+        for (int j = 0; j < VPT; j++) {
+            const bm_u64 key = bm_key(x[j], index(j / V) + j % V);
+            const bool in = x[j] > -INFINITY && key >= T1;
+            const bm_u64 m = __ballot(in);
+            if (in) part[n_part + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0u))] = key;
+            n_part += __popcll(m);
+        }
+        if (lane == 0) count[wave] = n_part;
+        __syncthreads();
     }
-    __syncthreads();
+    int before = 0, some = 0;
+#pragma unroll
+    for (int w = 0; w < BM_WAVES; w++) {
+        before += w < wave ? count[w] : 0;
+        some += count[w];
+    }
     const size_t at = (size_t)row * a.shares + share;
-    if (tid == 0) a.share[at] = {(wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), M, 0.0f};
-    // places by counting
-    const int c = count;
-    bm_u64 *const out = a.list + at * a.n;
-    for (int i = tid; i < c; i += BM_THREADS) {
-        const bm_u64 key = list[i];
-        int rank = 0;
-        for (int j = 0; j < c; j++) rank += list[j] > key;
-        if (rank < a.n) out[rank] = key;
+    const int slots = bm_slots_log(a.n);
+    bm_u64 *const out = a.list + (at << slots);
+    BmShare result = {(wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), plain ? 0.0f : M, some, M > -INFINITY ? bm_key(M, 0xffffffffu) : 0};
+    if (some <= 1 << slots) {
+        for (int i = lane; i < n_part; i += 64) out[before + i] = part[i];
+    } else {
+        // places by counting
+        result.count = a.n;
+        for (int i = lane; i < n_part; i += 64) {
+            const bm_u64 key = part[i];
+            int rank = 0;
+#pragma unroll
+            for (int w = 0; w < BM_WAVES; w++)
+                for (int j = 0; j < count[w]; j++) rank += list[BM_PART * w + j] > key;
+            if (rank < a.n) out[rank] = key;
+            if (rank == 0) wkey[0] = key;
+        }
+        __syncthreads();
+        result.best = wkey[0];
     }
-    for (int i = c + tid; i < a.n; i += BM_THREADS) out[i] = 0;
+    if (tid == 0) a.share[at] = result;
 }
 
 // ---------------------------------------------------------------------------
@@ -197,8 +299,11 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
 // token, the lower first).
 // ---------------------------------------------------------------------------
 #define BS_THREADS 1024
-#define BS_WAVES 16
-#define BS_LIST 2048
+#define BS_WAVES (BS_THREADS / 64)
+#define BS_LIST 4096
+#define BS_COUNTED 256                // shares whose n-th largest is found by counting
+#define BS_RANKED 128                 // candidates that are ranked as they are
+#define BS_ACTIVE 2048                // shares whose entries are looked at
 
 struct BsKey {
     bm_u64 score;                     // 0: none
@@ -212,41 +317,50 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     __shared__ double base[QK_BEAM_MAX];                         // score - log(sum); NaN: no candidates by logits
     __shared__ float most[QK_BEAM_MAX];                          // the largest logit
     __shared__ BsKey bounds[BS_WAVES], list[BS_LIST];
-    __shared__ int count;
+    __shared__ int counts[3][8], count, n_active, active[BS_ACTIVE], entries[BS_ACTIVE], rank[BS_LIST];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = blockIdx.x, n = a.n_out;
-    const int row0 = q * a.beams;
+    const int row0 = q * a.beams, cols = a.beams * shares, slots = bm_slots_log(n);
+    share += (size_t)row0 * shares;
+    lists += (size_t)row0 * shares << slots;
+    const BmShare first = share[min(tid, cols - 1)];             // of what idle beams left nothing is looked at
     for (int b = wave; b < a.beams; b += BS_WAVES) {
+        const BmShare *const s = share + (size_t)b * shares;
+        const BmShare mx = s[min(lane, shares - 1)];
+        const float score = a.score[row0 + b];
+        const int end = a.ended ? a.ended[row0 + b] : -1;
         double v = NAN;
-        if (!bm_idle(a.score, a.ended, row0 + b, a.vocab)) {
-            const BmShare *const s = share + (size_t)(row0 + b) * shares;
-            float M = -INFINITY;
-            for (int i = lane; i < shares; i += 64) M = fmaxf(M, s[i].max);
+        if (fabsf(score) <= 3.402823466e38f && (unsigned)end >= (unsigned)a.vocab) {
+            auto max_of = [](const BmShare &x) { return x.best ? bm_value(x.best) : -INFINITY; };
+            float M = max_of(mx);
+            for (int i = lane + 64; i < shares; i += 64) M = fmaxf(M, max_of(s[i]));
             M = wave_max(M);
-            double sum = 0.0;
-            for (int i = lane; i < shares; i += 64)
-                if (s[i].max > -INFINITY) sum += s[i].sum * exp((double)s[i].max - (double)M);
+            auto part = [&](const BmShare &x) {
+                return x.best ? x.sum * (double)bm_exp2(fmax(((double)x.ref - (double)M) * BM_LOG2E, -300.0)) : 0.0;
+            };
+            double sum = lane < shares ? part(mx) : 0.0;
+            for (int i = lane + 64; i < shares; i += 64) sum += part(s[i]);
             sum = bm_sum(sum);
-            if (M > -INFINITY) v = (double)a.score[row0 + b] - log(sum);
+            if (M > -INFINITY) v = (double)score - log(sum);
             if (lane == 0) most[b] = M;
         }
         if (lane == 0) base[b] = v;
     }
-    if (tid == 0) count = 0;
+    if (tid == 0) count = n_active = 0;
+    if (tid < 24) counts[tid / 8][tid % 8] = 0;
     __syncthreads();
-    const int per = shares * n, all = per * a.beams;
-    const bm_u64 *const mine = lists + (size_t)row0 * per;
-    // candidate i: an entry of a list, or behind those a beam at its end
-    auto candidate = [&](int i) {
+    auto key_of = [&](int b, bm_u64 e) {
+        const double s = base[b];
         BsKey k = {0, 0};
-        if (i < all) {
-            const int b = i / per;
-            const double s = base[b];
-            if (s == s) {                                        // otherwise its lists hold nothing
-                const bm_u64 e = mine[i];
-                if (e) k = {bm_order(s + ((double)bm_value(e) - (double)most[b])), 0xffffffffu - ((unsigned)b * a.vocab + bm_index(e))};
-            }
-        } else if (i < all + a.beams && a.ended) {
-            const int b = i - all;
+        if (s == s && e) {
+            k.score = bm_order(s + ((double)bm_value(e) - (double)most[b]));
+            k.at = (unsigned)e ? 0xffffffffu - ((unsigned)b * a.vocab + bm_index(e)) : 0u;
+        }
+        return k;
+    };
+    // beam b's candidate where it is at its end
+    auto end_of = [&](int b) {
+        BsKey k = {0, 0};
+        if (b < a.beams && a.ended) {
             const float s = a.score[row0 + b];
             const int t = a.ended[row0 + b];
             if ((unsigned)t < (unsigned)a.vocab && fabsf(s) <= 3.402823466e38f)
@@ -254,77 +368,193 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
         }
         return k;
     };
-    const int m = all + a.beams;
-    BsKey top = {0, 0};
-    for (int i = tid; i < m; i += BS_THREADS) {
-        const BsKey k = candidate(i);
+    auto best_of = [&](int i, const BmShare &s) { return key_of((int)((unsigned)i / (unsigned)shares), s.best); };
+    // a thread's largest candidate
+    BsKey top = end_of(tid);
+    if (tid < cols) {
+        const BsKey k = best_of(tid, first);
         if (k > top) top = k;
     }
-    // a bound as in beam_rows, and by the places where scores are equal
-    {
-        BsKey b = {bm_bound<bm_u64, 64>(top.score, n), 0};
-        const bool equal = top.score == b.score;
-        const int above = __popcll(__ballot(top.score > b.score));
-        if (b.score && above + __popcll(__ballot(equal)) > n) b.at = bm_bound<unsigned, 32>(equal ? top.at : 0u, n - above);
+    for (int i = tid + BS_THREADS; i < cols; i += BS_THREADS) {
+        const BsKey k = best_of(i, share[i]);
+        if (k > top) top = k;
+    }
+    // A bound that at least n of the block's keys reach, and at most `enough` where it can be: the bits of the n-th
+    // largest from the top, three at a time, until so few are left.  own(u): how many of the thread's keys reach u.
+    auto bound = [&](int enough, auto own) {
+        BsKey t = {0, 0};
+        for (int b = 96 - 3, turn = 0; b >= 0; b -= 3, turn = turn == 2 ? 0 : turn + 1) {
+            auto with = [&](unsigned k) {                        // t with k in the bits b .. b + 2
+                BsKey u = t;
+                if (b >= 32) u.score |= (bm_u64)k << (b - 32);
+                else {
+                    u.at |= k << b;
+                    if (b > 29) u.score |= k >> (32 - b);
+                }
+                return u;
+            };
+            int mine = 0;                                        // of lane k: the wave's keys that reach with(k)
+#pragma unroll
+            for (int k = 1; k < 8; k++) {
+                const int c = own(with(k));
+                if (lane == k) mine = c;
+            }
+            if (lane > 0 && lane < 8 && mine) atomicAdd(&counts[turn][lane], mine);
+            if (tid < 8) counts[turn == 2 ? 0 : turn + 1][tid] = 0;        // its last readers are two barriers back
+            __syncthreads();
+            int got = INT_MAX, most = 0;
+#pragma unroll
+            for (int k = 1; k < 8; k++) {
+                const int c = counts[turn][k];
+                if (c >= n) {
+                    most = k;
+                    got = c;
+                }
+            }
+            t = with(most);
+            if (got <= enough) break;
+        }
+        __syncthreads();
+        if (tid < 24) counts[tid / 8][tid % 8] = 0;
+        __syncthreads();
+        return t;
+    };
+    BsKey T0 = {0, 0};
+    // The same from the waves' n-th largest: cheaper, and looser where a wave's keys are not a sample of all.  Of a
+    // score's upper half; where more than n are equal in that, by the rest and the places.
+    auto wave_bound = [&](const BsKey &key) {
+        const unsigned high = (unsigned)(key.score >> 32);
+        const unsigned t = bm_bound<unsigned, 32>(high, n);
+        BsKey b = {(bm_u64)t << 32, 0};
+        const int above = __popcll(__ballot(high > t)), equal = __popcll(__ballot(high == t));
+        if (t && above < n && above + equal > n) {
+            const bm_u64 rest = bm_bound<bm_u64, 64>(high == t ? key.score << 32 | key.at : 0, n - above);
+            b = {(bm_u64)t << 32 | rest >> 32, (unsigned)rest};
+        }
         if (lane == 0) bounds[wave] = b;
+        __syncthreads();
+        BsKey most = bounds[0];
+#pragma unroll
+        for (int w = 1; w < BS_WAVES; w++)
+            if (bounds[w] > most) most = bounds[w];
+        return most;
+    };
+    // The keys of the block's threads that reach T0, to the list (in no order); how many
+    auto gather = [&](const BsKey &key) {
+        if (tid == 0) count = 0;
+        __syncthreads();
+        if (key.score && key >= T0) list[atomicAdd(&count, 1)] = key;
+        __syncthreads();
+        return count;
+    };
+    // The n-th largest of the threads', by counting, once the waves' bounds have left few enough: the first
+    // of these is loose (a beam's shares are in one or two waves, the best beam's may be fewer than n of a wave).
+    if (cols > BS_COUNTED) T0 = wave_bound(top);
+    int c0 = gather(top);
+    if (c0 > BS_COUNTED) {
+        const BsKey one = tid < c0 ? list[tid] : BsKey{0, 0};
+        T0 = wave_bound(one);
+        c0 = gather(one);
+    }
+    if (c0 > n && c0 <= BS_COUNTED) {
+        constexpr int PARTS = BS_THREADS / BS_COUNTED;
+        if (tid < BS_COUNTED) rank[tid] = 0;
+        __syncthreads();
+        const int i = tid % BS_COUNTED;
+        if (i < c0) {
+            const BsKey one = list[i];
+            int above = 0;
+            for (int j = tid / BS_COUNTED; j < c0; j += PARTS) above += list[j] > one || (j < i && list[j] >= one);
+            atomicAdd(rank + i, above);
+        }
+        __syncthreads();
+        if (tid < c0 && rank[tid] == n - 1) bounds[0] = list[tid];
+        __syncthreads();
+        T0 = bounds[0];
     }
     __syncthreads();
-    BsKey T0 = bounds[0];
-#pragma unroll
-    for (int w = 1; w < BS_WAVES; w++)
-        if (bounds[w] > T0) T0 = bounds[w];
+    if (tid == 0) count = 0;
+    for (int i = tid; i < cols; i += BS_THREADS) {
+        const BmShare s = i == tid ? first : share[i];
+        const BsKey k = best_of(i, s);
+        if (k.score && k.score >= T0.score) {
+            const int at = atomicAdd(&n_active, 1);
+            if (at < BS_ACTIVE) {
+                active[at] = i;
+                entries[at] = s.count;
+            }
+        }
+    }
+    __syncthreads();
+    // all candidates that may reach the bound: of the active shares (of all, where they are too many for a list), and ends
+    const bool every = n_active > BS_ACTIVE;
+    const long m = (long)(every ? cols : n_active) << slots;
+    auto each = [&](auto take) {
+        for (long i = tid; i < m; i += BS_THREADS) {
+            const int k = (int)(i >> slots), l = every ? k : active[k], slot = (int)i & ((1 << slots) - 1);
+            const int b = (int)((unsigned)l / (unsigned)shares);
+            if (base[b] == base[b] && slot < (every ? share[l].count : entries[k])) take(key_of(b, lists[((size_t)l << slots) + slot]));
+        }
+        take(end_of(tid));
+    };
     auto collect = [&]() {
-        for (int i = tid; i < m; i += BS_THREADS) {
-            const BsKey k = candidate(i);
+        each([&](const BsKey &k) {
             if (k.score && k >= T0) {
                 const int at = atomicAdd(&count, 1);
                 if (at < BS_LIST) list[at] = k;
             }
-        }
+        });
         __syncthreads();
     };
     collect();
     if (count > BS_LIST) {
-        // candidates beyond the list (many of one thread's are large): the bound's bits from the top, by
-        // counting all of them, until they fit
-        BsKey t = {0, 0};
-        for (int b = 95; b >= 0; b--) {
-            BsKey u = t;
-            if (b >= 32) u.score |= 1ull << (b - 32);
-            else u.at |= 1u << b;
-            __syncthreads();
-            if (tid == 0) count = 0;
-            __syncthreads();
+        // candidates beyond the list (many shares that reach the bound many times over)
+        T0 = bound(BS_LIST, [&](const BsKey &u) {
             int c = 0;
-            for (int i = tid; i < m; i += BS_THREADS) {
-                const BsKey k = candidate(i);
-                c += k.score && k >= u;
-            }
-            c = (int)wave_sum((float)c);
-            if (lane == 0) atomicAdd(&count, c);
-            __syncthreads();
-            const int got = count;
-            if (got >= n) t = u;
-            if (got >= n && got <= BS_LIST) break;
-        }
-        T0 = t;
-        __syncthreads();
+            each([&](const BsKey &k) { c += k.score && k >= u; });
+            return (int)wave_sum((float)c);
+        });
         if (tid == 0) count = 0;
         __syncthreads();
         collect();
     }
+    if (count > BS_RANKED) {
+        // a tighter bound from the list (in no order: a wave's part is a sample)
+        BsKey mine[BS_LIST / BS_THREADS], most = {0, 0};
+#pragma unroll
+        for (int j = 0; j < BS_LIST / BS_THREADS; j++) {
+            const int i = tid + BS_THREADS * j;
+            mine[j] = i < count ? list[i] : BsKey{0, 0};
+            if (mine[j] > most) most = mine[j];
+        }
+        T0 = wave_bound(most);
+        if (tid == 0) count = 0;                      // every thread has its part of the list
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < BS_LIST / BS_THREADS; j++)
+            if (mine[j].score && mine[j] >= T0) list[atomicAdd(&count, 1)] = mine[j];
+        __syncthreads();
+    }
     const int c = count;
     const size_t o = (size_t)q * n;
-    for (int i = tid; i < c; i += BS_THREADS) {
+    // places by counting, `parts` threads an entry
+    for (int i = tid; i < c; i += BS_THREADS) rank[i] = 0;
+    __syncthreads();
+    const int parts = c <= 64 ? BS_THREADS / 64 : c <= 256 ? BS_THREADS / 256 : 1, width = BS_THREADS / parts;
+    for (int i = tid % width; i < c; i += width) {
         const BsKey key = list[i];
-        int rank = 0;
-        for (int j = 0; j < c; j++) rank += list[j] > key;
-        if (rank < n) {
-            const unsigned place = 0xffffffffu - key.at;
-            a.parent[o + rank] = row0 + (int)(place / a.vocab);
-            a.token[o + rank] = (int)(place % a.vocab);
-            a.score_out[o + rank] = (float)bm_double(key.score);
-        }
+        int above = 0;
+        for (int j = tid / width; j < c; j += parts) above += list[j] > key;
+        atomicAdd(rank + i, above);
+    }
+    __syncthreads();
+    for (int i = tid; i < c; i += BS_THREADS) {
+        if (rank[i] >= n) continue;
+        const BsKey key = list[i];
+        const unsigned place = 0xffffffffu - key.at;
+        a.parent[o + rank[i]] = row0 + (int)(place / a.vocab);
+        a.token[o + rank[i]] = (int)(place % a.vocab);
+        a.score_out[o + rank[i]] = (float)bm_double(key.score);
     }
     for (int i = c + tid; i < n; i += BS_THREADS) {
         a.parent[o + i] = a.token[o + i] = -1;
@@ -343,7 +573,7 @@ static int row_shares(int vocab, int v) { return (vocab + BM_THREADS * v - 1) / 
 
 extern "C" size_t qk_beam_ws_bytes(int seqs, int beams, int vocab, int n_out) {
     const int rows = seqs * beams, shares = row_shares(vocab, vpt(rows, vocab, n_out));
-    return (size_t)rows * shares * (sizeof(BmShare) + sizeof(bm_u64) * n_out);
+    return (size_t)rows * shares * (sizeof(BmShare) + (sizeof(bm_u64) << bm_slots_log(n_out)));
 }
 
 template <typename T>
@@ -356,9 +586,13 @@ static void rows_launch(const BmRows &r, int rows, int v, hipStream_t s) {
 
 extern "C" int qk_beam_launch(const qk_beam_args *a, hipStream_t s) {
     const int rows = a->seqs * a->beams, v = vpt(rows, a->vocab, a->n_out), shares = row_shares(a->vocab, v);
+    // even shares: one of few entries would leave groups of threads with few or none
+    const int width = ((a->vocab + shares - 1) / shares + 7) / 8 * 8;
     BmShare *const share = (BmShare *)a->ws;
     bm_u64 *const lists = (bm_u64 *)(share + (size_t)rows * shares);
-    const BmRows r = {a->logits, a->row_stride, a->vocab, a->n_out, shares, a->score, a->ended, share, lists};
+    // few rows: a chain of loads less; many: the bytes of idle ones
+    const BmRows r = {a->logits, a->row_stride, a->vocab, a->n_out, shares, width, a->score, a->ended, share, lists,
+                      (long)rows * a->vocab < 4 << 20};
     if (a->bf16) rows_launch<uint16_t>(r, rows, v, s);
     else rows_launch<float>(r, rows, v, s);
     beam_select<<<(unsigned)a->seqs, BS_THREADS, 0, s>>>(*a, shares, share, lists);

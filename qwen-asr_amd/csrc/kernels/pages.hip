@@ -28,6 +28,7 @@ typedef uint32_t pages_u32x4 __attribute__((ext_vector_type(4)));
 // ---------------------------------------------------------------------------
 #define FK_THREADS 1024
 #define FK_WAVES (FK_THREADS / 64)
+#define FK_ROWS 4                                     // rows that a wave has on their way at once
 
 // exclusive sum over the block's threads and the sum of all; part: FK_WAVES + 1 ints
 __device__ __forceinline__ int fk_scan(int v, int *part, int &all) {
@@ -61,7 +62,8 @@ struct FkRow {
 template <int LDS_WORDS>
 __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     __shared__ unsigned bits[LDS_WORDS > 0 ? 2 * LDS_WORDS : 1];
-    __shared__ int tails[QK_PAGED_FORK_ROWS], offs[QK_PAGED_FORK_ROWS + 1], part[FK_WAVES];
+    __shared__ __attribute__((aligned(16))) int tails[QK_PAGED_FORK_ROWS];
+    __shared__ int offs[QK_PAGED_FORK_ROWS], ranks[FK_THREADS], part[FK_WAVES];
     __shared__ FkRow rows[QK_PAGED_FORK_ROWS];
     __shared__ unsigned long long over;               // pages that the table has no room for
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -102,17 +104,25 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     }
     __syncthreads();
     // a wave a row: its entries, and which pages they hold
-    for (int s = wave; s < a.n_out; s += FK_WAVES) {
-        const int from = tails[s], n_whole = rows[s].first, n = rows[s].count;
-        const int *const in = a.table + (size_t)max(from, 0) * a.stride;
-        int *const out = a.table_out + (size_t)s * a.stride;
+    for (int s0 = wave; s0 < a.n_out; s0 += FK_WAVES * FK_ROWS) {
         for (int e = lane; e < a.stride; e += 64) {
-            int id = e < n ? in[e] : -1;
-            id = (unsigned)id < (unsigned)a.n_pages ? id : -1;
-            out[e] = id;
-            if (id >= 0) {
-                set(held, id);
-                if (e < n_whole) set(whole, id);
+            int id[FK_ROWS], n_whole[FK_ROWS];
+#pragma unroll
+            for (int j = 0; j < FK_ROWS; j++) {
+                const int s = min(s0 + FK_WAVES * j, a.n_out - 1), from = tails[s];
+                n_whole[j] = rows[s].first;
+                id[j] = e < rows[s].count ? a.table[(size_t)max(from, 0) * a.stride + e] : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < FK_ROWS; j++) {
+                const int s = s0 + FK_WAVES * j;
+                if (s >= a.n_out) break;
+                id[j] = (unsigned)id[j] < (unsigned)a.n_pages ? id[j] : -1;
+                a.table_out[(size_t)s * a.stride + e] = id[j];
+                if (id[j] >= 0) {
+                    set(held, id[j]);
+                    if (e < n_whole[j]) set(whole, id[j]);
+                }
             }
         }
     }
@@ -128,12 +138,17 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     const int at = whole_pages;                       // the tail's entry, where it is in the table
     const bool has_tail = on && slots > 0 && at < a.stride;
     const int tail = has_tail ? a.table_out[(size_t)tid * a.stride + at] : -1;
-    if (on) tails[tid] = tail;
+    tails[tid] = tail;                                // -1 behind the last row
     __syncthreads();
     bool copied = false;
     if (tail >= 0 && fresh_rows > 0) {
         copied = get(whole + (tail >> 5)) >> (tail & 31) & 1u;
-        for (int j = tid + 1; j < a.n_out && !copied; j++) copied = tails[j] == tail;
+#pragma unroll 4
+        for (int j = tid & ~3; j < a.n_out; j += 4) {
+            const int4 t = *reinterpret_cast<const int4 *>(tails + j);
+            copied = copied || (t.x == tail && j > tid) || (t.y == tail && j + 1 > tid) || (t.z == tail && j + 2 > tid) ||
+                     (t.w == tail && j + 3 > tid);
+        }
     }
     FkRow r = {kept, 0, -1, 0};
     if (on) {
@@ -160,22 +175,39 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     };
     int mine = 0, all;
     for (int w = w0; w < w1; w++) mine += __popc(free_bits(w));
-    int rank = fk_scan(mine, part, all);
+    ranks[tid] = fk_scan(mine, part, all);
     if (tid == 0) *a.missing = (int)min((long)over + max(total - all, 0), (long)INT_MAX);
-    for (int w = w0; w < w1 && rank < total; w++) {
-        for (unsigned f = free_bits(w); f && rank < total; f &= f - 1, rank++) {
-            const int id = 32 * w + __builtin_ctz(f);
-            int lo = 0, hi = a.n_out;                 // the last row whose fresh pages begin at rank or before
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (offs[mid] <= rank) lo = mid;
-                else hi = mid;
-            }
-            const FkRow x = rows[lo];
-            a.table_out[(size_t)lo * a.stride + x.first + (rank - offs[lo])] = id;
-            if (x.tail >= 0 && rank == offs[lo])
-                *reinterpret_cast<int4 *>(a.copies + 4 * lo) = make_int4(x.tail, id, 0, x.part);
+    __syncthreads();
+    // the last of n ascending numbers that is at most x (the first is 0)
+    auto last_upto = [](const int *v, int n, int x) {
+        int lo = 0;
+        for (int step = 1 << (31 - __builtin_clz(n)); step > 0; step >>= 1)
+            if (lo + step < n && v[lo + step] <= x) lo += step;
+        return lo;
+    };
+    // a thread a fresh page: the row that takes it, and which it is
+    for (int rank = tid; rank < min(total, all); rank += FK_THREADS) {
+        const int s = last_upto(offs, a.n_out, rank), t = last_upto(ranks, FK_THREADS, rank);
+        int k = rank - ranks[t], w = t * per;
+        unsigned f = free_bits(w);
+        while (k >= __popc(f)) {
+            k -= __popc(f);
+            f = free_bits(++w);
         }
+        int bit = 0;                                  // the k-th of its bits
+#pragma unroll
+        for (int half = 16; half > 0; half >>= 1) {
+            const int c = __popc(f & ((1u << half) - 1));
+            if (k >= c) {
+                k -= c;
+                f >>= half;
+                bit += half;
+            }
+        }
+        const FkRow x = rows[s];
+        a.table_out[(size_t)s * a.stride + x.first + (rank - offs[s])] = 32 * w + bit;
+        if (x.tail >= 0 && rank == offs[s])
+            *reinterpret_cast<int4 *>(a.copies + 4 * s) = make_int4(x.tail, 32 * w + bit, 0, x.part);
     }
 }
 
