@@ -138,41 +138,47 @@ static int tokens_by_matrix(int cache_bf16, int group) { return cache_bf16 && gr
  * < 2 R T: for prompts 2 x 128 x 384, for single tokens 2 x 8 x 2048 (fewer heads a block: as many).
  * Times 520 bytes, that is below QWEN_HIP_PAGED_ATTENTION_WS_MAX for any batch.
  */
-static size_t attention_plan(const qk_paged *p, int matrix, int heads, int max_len, int window, int sinks, int *rows2,
-                             int *nsplit, int *chunk) {
+enum { ALL, WINDOW, TREE };
+typedef struct {
+    int kind, window, sinks;
+} seen_keys;
+
+static size_t attention_plan(const qk_paged *p, seen_keys seen, int matrix, int heads, int max_len, int *rows2, int *nsplit,
+                             int *chunk) {
     if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;
-    if (window) {
+    if (seen.kind == WINDOW) {
         /* what a block walks at most, about: the window and the first positions, and of packed rows as many
          * positions more as a block has rows, and tiles that are seen in part */
-        const long most = (long)window + sinks + (matrix ? 128 * p->kv_heads / heads + 62 : 0);
+        const long most = (long)seen.window + seen.sinks + (matrix ? 128 * p->kv_heads / heads + 62 : 0);
         if (most < max_len) max_len = (int)most;
     }
     *rows2 = 0;
-    if (matrix) *rows2 = qk_paged_prefill_plan(p, heads, max_len, nsplit, chunk);
-    else qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
+    if (!matrix) qk_paged_decode_plan(p->n_seqs, heads, p->kv_heads, p->cache_bf16, max_len, nsplit, chunk);
+    else if (seen.kind == ALL) *rows2 = qk_paged_prefill_plan(p, heads, max_len, nsplit, chunk);
+    else *rows2 = qk_paged_masked_plan(p, seen.kind == TREE, heads, max_len, nsplit, chunk);
     if (*nsplit == 1) return 0;
     return (size_t)p->rows * heads * *nsplit * (QWEN_HIP_HEAD_DIM + 2) * sizeof(float);
 }
 
-static int by_matrix(const qk_paged *p, int drafts, int heads) {
-    return drafts || p->row_start || tokens_by_matrix(p->cache_bf16, heads / p->kv_heads);
+static int by_matrix(const qk_paged *p, seen_keys seen, int heads) {
+    return seen.kind == TREE || p->row_start || tokens_by_matrix(p->cache_bf16, heads / p->kv_heads);
 }
 
 size_t qwen_hip_paged_attention_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
     int rows2, nsplit, chunk;
     if (qk_paged_view("paged_attention_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
-    const int matrix = by_matrix(&p, 0, heads);
-    return attention_plan(&p, matrix, heads, batch->max_len, 0, 0, &rows2, &nsplit, &chunk);
+    const seen_keys all = {ALL, 0, 0};
+    return attention_plan(&p, all, by_matrix(&p, all, heads), heads, batch->max_len, &rows2, &nsplit, &chunk);
 }
 
-/* kind: single tokens, packed rows, either, a tree's drafts (those by a.window and a.tree of `mask`) */
-enum { TOKENS, PACKED, EITHER, DRAFTS };
+/* rows: single tokens, packed ones, or either */
+enum { TOKENS, PACKED, EITHER };
 
-static int attention(const char *op, int kind, const qk_paged_attn_args *mask, const qwen_hip_paged_kv *kv,
+static int attention(const char *op, int kind, seen_keys seen, const uint64_t *tree, int words, const qwen_hip_paged_kv *kv,
                      const qwen_hip_paged_batch *batch, void *out, const void *q, int dtype, int heads, float scale,
                      void *ws, size_t ws_bytes, hipStream_t s) {
-    qk_paged_attn_args a = *mask;
+    qk_paged_attn_args a = {0};
     const int rc = qk_paged_view(op, kv, batch, heads, dtype, &a.pg);
     if (rc) return rc;
     if (kind == PACKED && !batch->row_start) QK_REFUSE("%s: no row_start", op);
@@ -183,9 +189,9 @@ static int attention(const char *op, int kind, const qk_paged_attn_args *mask, c
     if (!out || !q) QK_REFUSE("%s: a pointer of the rows is NULL", op);
     if (!qk_aligned16(out) || !qk_aligned16(q)) QK_REFUSE("%s: the rows are not 16-byte aligned", op);
     if (out == q) QK_REFUSE("%s: out cannot be q", op);
-    if (kind == DRAFTS && !a.tree) QK_REFUSE("%s: no tree", op);
-    const int matrix = by_matrix(&a.pg, kind == DRAFTS, heads);
-    const size_t need = attention_plan(&a.pg, matrix, heads, batch->max_len, a.window, a.sinks, &a.rows2, &a.nsplit, &a.chunk);
+    if (seen.kind == TREE && !tree) QK_REFUSE("%s: no tree", op);
+    const int matrix = by_matrix(&a.pg, seen, heads);
+    const size_t need = attention_plan(&a.pg, seen, matrix, heads, batch->max_len, &a.rows2, &a.nsplit, &a.chunk);
     if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);
     a.out = out;
@@ -193,6 +199,11 @@ static int attention(const char *op, int kind, const qk_paged_attn_args *mask, c
     a.act_bf16 = dtype == QWEN_HIP_ST_BF16;
     a.heads = heads;
     a.scale = scale;
+    a.window = seen.window;
+    a.sinks = seen.sinks;
+    /* little-endian: bit i of a row is bit i % 32 of its 32-bit word i / 32 */
+    a.tree = (const uint32_t *)tree;
+    a.tree_words = 2 * words;
     a.part_o = (float *)ws;
     a.part_ml = need ? a.part_o + (size_t)a.pg.rows * heads * a.nsplit * QWEN_HIP_HEAD_DIM : NULL;
     if (matrix) QK_TRY(qk_paged_prefill_launch(&a, s));
@@ -204,15 +215,15 @@ static int attention(const char *op, int kind, const qk_paged_attn_args *mask, c
 int qwen_hip_paged_attention_decode(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
                                     const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
                                     hipStream_t s) {
-    const qk_paged_attn_args all = {0};
-    return attention("paged_attention_decode", TOKENS, &all, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+    const seen_keys all = {ALL, 0, 0};
+    return attention("paged_attention_decode", TOKENS, all, NULL, 0, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
 }
 
 int qwen_hip_paged_attention_prefill(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
                                      const void *q, int dtype, int heads, float scale, void *ws, size_t ws_bytes,
                                      hipStream_t s) {
-    const qk_paged_attn_args all = {0};
-    return attention("paged_attention_prefill", PACKED, &all, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+    const seen_keys all = {ALL, 0, 0};
+    return attention("paged_attention_prefill", PACKED, all, NULL, 0, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
 }
 
 /* a window of more positions than a length can name, and more first positions than a table holds, are as good as those */
@@ -225,8 +236,8 @@ size_t qwen_hip_paged_attention_window_ws_bytes(const qwen_hip_paged_kv *kv, con
     if (window <= 0 || sinks < 0 ||
         qk_paged_view("paged_attention_window_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p))
         return 0;
-    return attention_plan(&p, by_matrix(&p, 0, heads), heads, batch->max_len, window, first_positions(sinks), &rows2,
-                          &nsplit, &chunk);
+    const seen_keys seen = {WINDOW, window, first_positions(sinks)};
+    return attention_plan(&p, seen, by_matrix(&p, seen, heads), heads, batch->max_len, &rows2, &nsplit, &chunk);
 }
 
 int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
@@ -234,15 +245,16 @@ int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_
                                     size_t ws_bytes, hipStream_t s) {
     static const char op[] = "paged_attention_window";
     if (window <= 0 || sinks < 0) QK_REFUSE("%s: a window of %d positions, %d first ones", op, window, sinks);
-    const qk_paged_attn_args a = {.window = window, .sinks = first_positions(sinks)};
-    return attention(op, EITHER, &a, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+    const seen_keys seen = {WINDOW, window, first_positions(sinks)};
+    return attention(op, EITHER, seen, NULL, 0, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
 }
 
 size_t qwen_hip_paged_attention_tree_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads) {
     qk_paged p;
     int rows2, nsplit, chunk;
     if (qk_paged_view("paged_attention_tree_ws_bytes", kv, batch, heads, QWEN_HIP_ST_F32, &p) || no_call(&p)) return 0;
-    return attention_plan(&p, 1, heads, batch->max_len, 0, 0, &rows2, &nsplit, &chunk);
+    const seen_keys seen = {TREE, 0, 0};
+    return attention_plan(&p, seen, 1, heads, batch->max_len, &rows2, &nsplit, &chunk);
 }
 
 int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out, const void *q,
@@ -251,7 +263,6 @@ int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_pa
     static const char op[] = "paged_attention_tree";
     if (words <= 0 || words > QK_TREE_WORDS / 2) QK_REFUSE("%s: %d words of bits a row (1 .. %d)", op, words, QK_TREE_WORDS / 2);
     if ((uintptr_t)tree % 8) QK_REFUSE("%s: the tree is not 8-byte aligned", op);
-    /* little-endian: bit i of a row is bit i % 32 of its 32-bit word i / 32 */
-    const qk_paged_attn_args a = {.tree = (const uint32_t *)tree, .tree_words = 2 * words};
-    return attention(op, DRAFTS, &a, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
+    const seen_keys seen = {TREE, 0, 0};
+    return attention(op, EITHER, seen, tree, words, kv, batch, out, q, dtype, heads, scale, ws, ws_bytes, s);
 }

@@ -233,11 +233,26 @@ __device__ __forceinline__ int pp_begin(const qk_paged &pg, int i) {
 // that take longest start first.  For more sequences, by sequence from the last: tiles of
 // sequence s take the slots from start_s G / ROWS + s on (ceil(n G / ROWS) of them never pass the
 // next sequence's first).
+//
+// FLAT: b counts through the tiles that there are, once for each split, so blocks without a tile come
+// behind all others.  They go out in order, in turn over parts of the card: between others, they would have these
+// wait (one sequence of 64 drafts behind 8000 positions, 24 splits: 37 us, 25 so; a split beside its next one
+// instead gives some parts all the full ones: 24 sequences, 60 and 85).
 struct PpTile {
     int s, f0, r0, n, len;
 };
-template <int ROWS>
-__device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int slots, PpTile &o) {
+template <int ROWS, bool FLAT>
+__device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int slots, int nsplit, PpTile &o, int &split) {
+    auto flat = [&](int tiles) {
+        if constexpr (FLAT) {
+            if (tiles == 0) return false;
+            split = nsplit == 1 ? 0 : __builtin_amdgcn_readfirstlane(b / tiles);
+            b -= split * tiles;
+            return split < nsplit && b < tiles;
+        } else {
+            return true;
+        }
+    };
     const int lane = threadIdx.x & 63;
     auto begin = [&](int i) { return pp_begin(pg, i); };
     auto take = [&](int s) {
@@ -247,6 +262,7 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
         o.len = pg_len(pg, s);
     };
     if (pg.n_seqs > 64) {
+        if (!flat(slots)) return false;
         const int slot = slots - 1 - b;
         auto first_slot = [&](int i) { return begin(i) * G / ROWS + i; };
         const int s = __builtin_amdgcn_readfirstlane(pg_search<64>(pg.n_seqs, slot, first_slot));
@@ -257,6 +273,7 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
     }
     if (pg.n_seqs == 1) {
         take(0);
+        if (!flat((o.n * G + ROWS - 1) / ROWS)) return false;
         o.f0 = ((o.n * G + ROWS - 1) / ROWS - 1 - b) * ROWS;
         return o.f0 >= 0;
     }
@@ -270,7 +287,8 @@ __device__ __forceinline__ bool pp_tile(const qk_paged &pg, int G, int b, int sl
         return (int)min(max((want + ROWS - 1) / ROWS - 1, 0L), (long)tiles);
     };
     auto sum_at = [&](int t) { return (int)wave_sum((float)(tiles - first_at(t))); };
-    if (b >= sum_at(0)) return false;
+    const int tiles_all = sum_at(0);
+    if (!flat(tiles_all) || b >= tiles_all) return false;
     int lo = 0, hi = (int)wave_max(on && n > 0 ? (float)((off + n + ROWS) / 128 + 2) : 0.0f);
     while (hi - lo > 1) {                        // sum_at(lo) > b >= sum_at(hi)
         const int mid = (lo + hi) >> 1;
@@ -317,7 +335,9 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
     const int ql = lane & 31, hl = lane >> 5;
     const int G = a.heads / pg.kv_heads, kvh = blockIdx.x % pg.kv_heads;
     PpTile tile;
-    if (!pp_tile<ROWS>(pg, G, (int)(blockIdx.x / pg.kv_heads), slots, tile)) return;      // block-uniform, as the next
+    int split = (int)blockIdx.y;
+    if (!pp_tile<ROWS, MASK != PP_CAUSAL>(pg, G, (int)(blockIdx.x / pg.kv_heads), slots, a.nsplit, tile, split)) return;      // block-uniform, as the next
+    if constexpr (MASK != PP_CAUSAL) split = __builtin_amdgcn_readfirstlane(split);
     const int s = __builtin_amdgcn_readfirstlane(tile.s), f0 = __builtin_amdgcn_readfirstlane(tile.f0),
               r0 = __builtin_amdgcn_readfirstlane(tile.r0), n = __builtin_amdgcn_readfirstlane(tile.n),
               len = __builtin_amdgcn_readfirstlane(tile.len);
@@ -337,7 +357,7 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         else return v;
     };
     const int need = (int)(((long)kend + a.nsplit - 1) / a.nsplit);
-    const int chunk = max(a.chunk, (need + PP_KT - 1) / PP_KT * PP_KT), split = blockIdx.y;
+    const int chunk = max(a.chunk, (need + PP_KT - 1) / PP_KT * PP_KT);
     const int k0s = (int)min((long)split * chunk, (long)kend), k1 = (int)min((long)k0s + chunk, (long)kend);
 
     // this lane's row
@@ -863,13 +883,43 @@ extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, 
     return rows2;
 }
 
+// Windows and trees of drafts.  Their blocks walk as many keys each (a window's) or as their sequence has (a
+// tree's), whose lengths differ; the host knows the mean of the sequences' rows, and takes each to have as many.  One
+// block of 128 rows a CU, two of 64 on bf16 pages, one on fp32 pages.
+//   rows   64 where a sequence has no more as a rule (8 x 32 drafts of 2 heads behind 250 to 2000, fp32 rows on bf16
+//          pages: 29 us, 31 with 128; 8 x 8 to 32 on fp32 pages: 38, 44).  Of a window also where its blocks are short
+//          (4 prompts of 500 to 2000 rows, bf16, 512 positions: 51 us, 54; but 1 of 8191 rows, 1024 positions: 134, 129;
+//          8 of 51 to 515, fp32 rows on bf16 pages, 1000 positions: 57, 51), which fp32 pages have no room for
+//   splits as many as the blocks, all of one length, find room for at once (4 x 100 to 700 rows, fp32, 512 positions:
+//          1 split, 180 blocks: 66 us; 2: 91; 1 x 64 drafts, bf16, behind 8000: 256 blocks 25, 336 34); of a tree whose
+//          blocks are many unsplit half as many more, as the long sequences would be waited for (24 x 21 to 64 drafts, bf16, behind 170 to 4000: 192 blocks 84 us, 384 60, 576 78; 4 x 100 to 200 of 4 heads
+//          behind 1500 to 6000: 160 blocks 122, 320 82, 480 107)
+extern "C" int qk_paged_masked_plan(const qk_paged *p, int tree, int heads, int max_len, int *nsplit, int *chunk) {
+    const long f = (long)p->rows * (heads / p->kv_heads), mean = (f + p->n_seqs - 1) / p->n_seqs;
+    const int fits = (f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 1024 : 384;
+    const int rows2 = p->page_shift >= 4 && (mean <= PP_ROWS(2) || (!tree && p->cache_bf16 && max_len <= fits));
+    const int rows = PP_ROWS(rows2 ? 2 : 4);
+    const long blocks = (mean + rows - 1) / rows * p->n_seqs * p->kv_heads;
+    long n = (rows2 ? 320 : tree && blocks >= 128 ? 384 : 256) / blocks;
+    n = n < 1 ? 1 : n > QK_PAGED_MAX_SPLIT ? QK_PAGED_MAX_SPLIT : n;
+    long c = ((max_len + n - 1) / n + 63) / 64 * 64;
+    c = c < 64 ? 64 : c;
+    // one block where that saves the join's launch, as above
+    if (p->cache_bf16 && max_len <= 128) c = 128;
+    n = (max_len + c - 1) / c;
+    *nsplit = n < 1 ? 1 : (int)n;
+    *chunk = (int)c;
+    return rows2;
+}
+
 template <typename T, typename C, int WR, int MASK>
 static int prefill_launch(const qk_paged_attn_args *a, hipStream_t s) {
     const qk_paged &pg = a->pg;
     const long slots = (long)pg.rows * (a->heads / pg.kv_heads) / PP_ROWS(WR) + pg.n_seqs;
     // a launch has fewer than 2^32 threads along an axis
-    if (slots * pg.kv_heads > 0xffffffffL / PP_THREADS(WR)) return QWEN_HIP_EINVAL;
-    const dim3 grid((unsigned)(slots * pg.kv_heads), (unsigned)a->nsplit);
+    const long row = slots * pg.kv_heads * (MASK == PP_CAUSAL ? 1 : a->nsplit);
+    if (row > 0xffffffffL / PP_THREADS(WR)) return QWEN_HIP_EINVAL;
+    const dim3 grid((unsigned)row, MASK == PP_CAUSAL ? (unsigned)a->nsplit : 1u);
     // the plan takes 64 rows for pages of 16 positions and more
     constexpr bool SOME_SMALL = WR == 4;
     if (SOME_SMALL && (1 << pg.page_shift) < PP_KT / WR)

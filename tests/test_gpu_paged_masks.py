@@ -79,13 +79,19 @@ def test_window_any_max_len(qa, gpu, max_len, packed):
 @pytest.mark.parametrize("act,cache", TYPES)
 @pytest.mark.parametrize("packed", [False, True])
 def test_window_of_everything(qa, gpu, act, cache, packed):
-    """a window of all positions, or all of them as first ones, is attention without one: the same bits"""
+    """a window of all positions, or all of them as first ones, is attention without one: the same bits for
+    single tokens; packed rows may be split otherwise, so both are within the tolerance of the definition"""
     new = [5, 100, 64, 2] if packed else None
     p = Paged(123, [300, 100, 64, 40], new=new, group=2, kv_heads=2, page=16, act=act, cache=cache).gpu(qa)
     want = p.attention(qa, SCALE)
     big = 2 ** 31 - 1
+    tol = M.reference(p, SCALE, M.window_sees(big, 0), packed)[1]
     for win, sinks in ((big, 0), (big, big), (300, 0), (1, big)):
-        assert T.equal(M.window(qa, p, SCALE, win, sinks), want), (win, sinks)
+        got = M.window(qa, p, SCALE, win, sinks)
+        if packed:
+            assert bool(((got.double() - want.double()).abs().cpu() <= 2 * tol).all()), (win, sinks)
+        else:
+            assert T.equal(got, want), (win, sinks)
 
 
 @pytest.mark.parametrize("packed", [False, True])
