@@ -300,6 +300,7 @@ __global__ __launch_bounds__(256) void paged_merge(qk_paged_attn_args a) {
         l = x.y;
         m = l == 0.0f ? -INFINITY : x.x;
     }
+    if (__builtin_amdgcn_readfirstlane(__float_as_int(l)) == __float_as_int(QK_PAGED_DONE)) return;      // the wave's, and all waves of the row
     const float M = wave_max(m);
     // a maximum that is no number passes fmaxf by: its sum is none either
     const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - pg_ref(M));

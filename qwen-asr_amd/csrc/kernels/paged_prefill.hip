@@ -825,7 +825,10 @@ __global__ __launch_bounds__(PP_THREADS(WR), sizeof(C) == 4 && WR == 2 ? 1 : 2) 
         o[d][r + 3] = fmaf(v.w, c1, o[d][r + 3] * c0);
     }
     if (!on) return;
-    if (a.nsplit == 1) {
+    // a window's or a tree's row whose keys are all in the first split is done here, and the join leaves it out
+    const bool whole = a.nsplit == 1 || (MASK != PP_CAUSAL && split == 0 && k1 == kend);
+    if (whole) {
+        if (MASK != PP_CAUSAL && a.nsplit > 1 && hl == 0) a.part_ml[2 * orow * a.nsplit + 1] = QK_PAGED_DONE;
         // 0 only where no key was seen: the largest p is at least 2^-8
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         T *dst = (T *)a.out + orow * PG_HD + 4 * hl;

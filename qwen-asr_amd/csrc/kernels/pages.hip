@@ -97,32 +97,35 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     const int whole_pages = min(len >> a.page_shift, a.stride), slots = len & (P - 1);
     if (on) {
         tails[tid] = p;
+        offs[tid] = -1;                               // the tail, once its wave has read it
         rows[tid] = {whole_pages, kept, 0, 0};
         const long end = (long)len + fresh_rows;
         a.len_out[tid] = (int)min(end, (long)INT_MAX);
         *reinterpret_cast<int4 *>(a.copies + 4 * tid) = make_int4(-1, -1, 0, 0);
     }
     __syncthreads();
-    // a wave a row: its entries, and which pages they hold
-    for (int s0 = wave; s0 < a.n_out; s0 += FK_WAVES * FK_ROWS) {
+    // a wave FK_ROWS rows beside each other: their entries, and which pages they hold.  What the row before has said already
+    // (beams share their first pages) is not said again: bits of one word are set one after the other.
+    for (int s0 = wave * FK_ROWS; s0 < a.n_out; s0 += FK_WAVES * FK_ROWS) {
         for (int e = lane; e < a.stride; e += 64) {
-            int id[FK_ROWS], n_whole[FK_ROWS];
+            int id[FK_ROWS];
+            bool in_whole[FK_ROWS];
 #pragma unroll
             for (int j = 0; j < FK_ROWS; j++) {
-                const int s = min(s0 + FK_WAVES * j, a.n_out - 1), from = tails[s];
-                n_whole[j] = rows[s].first;
+                const int s = min(s0 + j, a.n_out - 1), from = tails[s];
+                in_whole[j] = e < rows[s].first;
                 id[j] = e < rows[s].count ? a.table[(size_t)max(from, 0) * a.stride + e] : -1;
             }
 #pragma unroll
             for (int j = 0; j < FK_ROWS; j++) {
-                const int s = s0 + FK_WAVES * j;
-                if (s >= a.n_out) break;
+                if (s0 + j >= a.n_out) break;
                 id[j] = (unsigned)id[j] < (unsigned)a.n_pages ? id[j] : -1;
-                a.table_out[(size_t)s * a.stride + e] = id[j];
-                if (id[j] >= 0) {
-                    set(held, id[j]);
-                    if (e < n_whole[j]) set(whole, id[j]);
-                }
+                a.table_out[(size_t)(s0 + j) * a.stride + e] = id[j];
+                if (id[j] < 0) continue;
+                if (!in_whole[j]) offs[s0 + j] = id[j];          // the entry behind the whole pages
+                if (j > 0 && id[j] == id[j - 1] && in_whole[j] == in_whole[j - 1]) continue;
+                set(held, id[j]);
+                if (in_whole[j]) set(whole, id[j]);
             }
         }
     }
@@ -137,7 +140,7 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     __syncthreads();
     const int at = whole_pages;                       // the tail's entry, where it is in the table
     const bool has_tail = on && slots > 0 && at < a.stride;
-    const int tail = has_tail ? a.table_out[(size_t)tid * a.stride + at] : -1;
+    const int tail = has_tail ? offs[tid] : -1;
     tails[tid] = tail;                                // -1 behind the last row
     __syncthreads();
     bool copied = false;
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     };
     // a thread a fresh page: the row that takes it, and which it is
     for (int rank = tid; rank < min(total, all); rank += FK_THREADS) {
-        const int s = last_upto(offs, a.n_out, rank), t = last_upto(ranks, FK_THREADS, rank);
+        const int s = last_upto(offs, a.n_out, rank), t = last_upto(ranks, min(words, FK_THREADS), rank);
         int k = rank - ranks[t], w = t * per;
         unsigned f = free_bits(w);
         while (k >= __popc(f)) {

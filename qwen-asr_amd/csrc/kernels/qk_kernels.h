@@ -504,7 +504,8 @@ int qk_paged_append_launch(const qk_paged_append_args *a, hipStream_t s);
 
 /* Attention partials of split s of row r, head h: o[((r * heads + h) * nsplit + s) * 128 ..],
  * unnormalised, and ml[2 * (..)] = (maximum in base 2, sum); a split without keys has the sum 0
- * and no o. */
+ * and no o, and the first split of a row that is in `out` already has the sum QK_PAGED_DONE. */
+#define QK_PAGED_DONE -1.0f
 typedef struct {
     qk_paged pg;
     void *out;
