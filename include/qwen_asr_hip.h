@@ -594,9 +594,9 @@ int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_pa
  * append and attention take as kv_len).  A parent outside [0, kv->n_seqs) (-1) is an
  * empty sequence; parent NULL: row s continues row s (n_out == kv->n_seqs); new_rows NULL: none.
  *   Pages are shared where rows continue the same positions.  A last page with free slots, which
- * the new rows would write, is not: of the rows that have it as their last the last one keeps it
- * (unless a row has it for positions behind, or `outside` names it), the others with new rows
- * take a fresh page, and copies[s] = {page, fresh page, 0, slots} says what has to be copied
+ * the new rows would write, is not: of the rows that have it as their last the one with the most
+ * positions in it keeps it (of several the last; none where a row has it for positions behind, or
+ * `outside` names it), the others with new rows take a fresh page, and copies[s] = {page, fresh page, 0, slots} says what has to be copied
  * (qwen_hip_paged_copy; {-1, -1, 0, 0}: nothing; copies [n_out][4], 16-byte aligned).
  *   Fresh pages are those that no entry of the new table names and outside (bytes [n_pages],
  * not 0: a page that the program holds besides; NULL: none) does not, lowest first, to the rows
@@ -639,7 +639,7 @@ int qwen_hip_paged_compact(const qwen_hip_paged_kv *layers, int n_layers, const 
  * what has the score -infinity is no candidate, nor has a beam one whose score is not finite.
  * Places without a candidate get -1, -1, -infinity.  Scores are held and compared in 64 bits
  * (exponentials in fp32).  beams and n_out up to 64, vocab up to 2^20, seqs * beams up to
- * 2^16.  The same inputs give the same choice. */
+ * 2^16.  The outputs overlap neither score nor ended.  The same inputs give the same choice. */
 size_t qwen_hip_beam_select_ws_bytes(int seqs, int beams, int vocab, int n_out);
 int qwen_hip_beam_select(int *parent, int *token, float *score_out, const void *logits, int dtype, long row_stride,
                          int seqs, int beams, int vocab, const float *score, const int *ended, int n_out, void *ws,

@@ -7,10 +7,15 @@
  */
 #include "host_internal.h"
 
+#include <limits.h>
+
 #define BEAM_MAX_VOCAB (1 << 20)
 #define BEAM_MAX_ROWS (1 << 16)
 
-static int overlap(const int *a, size_t n, const int *b, size_t m) { return a && b && a < b + m && b < a + n; }
+/* n values at a and m at b, 4 bytes each */
+static int overlap(const void *a, size_t n, const void *b, size_t m) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + 4 * m && (uintptr_t)b < (uintptr_t)a + 4 * n;
+}
 
 /* the cache's shape, checked; its sequences as ones of a row each */
 static int shape(const char *op, const qwen_hip_paged_kv *kv, qk_paged *p) {
@@ -69,6 +74,7 @@ int qwen_hip_paged_fork(const qwen_hip_paged_kv *kv, const int *kv_len, const in
     if (!table_out || !len_out || !copies || !missing) QK_REFUSE("%s: an output is NULL", op);
     if (!qk_aligned16(copies)) QK_REFUSE("%s: copies is not 16-byte aligned", op);
     const size_t in = (size_t)p.n_seqs * p.table_stride, out = (size_t)n_out * p.table_stride;
+    if (out > INT_MAX) QK_REFUSE("%s: %d rows of %d page ids", op, n_out, p.table_stride);
     if (overlap(table_out, out, p.table, in) || overlap(len_out, n_out, kv_len, p.n_seqs))
         QK_REFUSE("%s: the new table or lengths overlap the old ones", op);
     const size_t need = qk_paged_fork_ws_bytes(p.n_pages);
@@ -134,6 +140,10 @@ int qwen_hip_beam_select(int *parent, int *token, float *score_out, const void *
     if (seqs == 0) return 0;
     if (!parent || !token || !score_out || !logits || !score) QK_REFUSE("%s: a pointer is NULL", op);
     if ((uintptr_t)logits % (dtype == QWEN_HIP_ST_F32 ? 4 : 2)) QK_REFUSE("%s: the logits are not aligned to their type", op);
+    const size_t rows = (size_t)seqs * beams, places = (size_t)seqs * n_out;
+    if (overlap(parent, places, score, rows) || overlap(parent, places, ended, rows) || overlap(token, places, score, rows) ||
+        overlap(token, places, ended, rows) || overlap(score_out, places, score, rows) || overlap(score_out, places, ended, rows))
+        QK_REFUSE("%s: an output overlaps score or ended", op);
     const size_t need = qk_beam_ws_bytes(seqs, beams, vocab, n_out);
     if (!ws || ws_bytes < need || !qk_aligned16(ws))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);

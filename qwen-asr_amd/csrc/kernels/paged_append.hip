@@ -6,6 +6,7 @@
 //   (x^[d], x^[d + 64]) -> (x^[d] c - x^[d + 64] s, x^[d + 64] c + x^[d] s),
 //   c, s = cos, sin[position][d], d = 0..63
 //
+// or, where the rows say by which position they turn (drafts of one depth alike, wherever they sit), of that one.
 // Everything in fp32, rounded once to the type it is stored in.  Bound by the
 // bytes it moves (rows in, queries and pages out) for many rows, by the chain
 // row -> sequence -> length -> page id -> store for one.

@@ -29,6 +29,9 @@
 //   24 sequences of 500 to 6001, all fp32, 1 head each: 81 us, 5.3 TB/s; 8 heads: 108 us,
 //     bound by the vector units
 // One short sequence is the time of two launches (11 us).
+//
+// Windows (WIN): the same over the positions that the row sees, the first ones and the window's, as if they were next
+// to each other (PgSeen).  64 sequences of 31 to 32769 positions, bf16, 2048 positions and 16 first ones: 52.5 us, 5.5 TB/s.
 #include "paged.h"
 
 // 16 bytes of a cached row as they lie in memory, widened at their use.  NT: rows that are

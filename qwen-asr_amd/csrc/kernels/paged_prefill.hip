@@ -4,7 +4,14 @@
 //
 //   o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s_j = scale log2(e) q . k_j,  m = max_j s_j
 //
-// on v_mfma_f32_32x32x16_bf16, with fp32 statistics and sums.
+// on v_mfma_f32_32x32x16_bf16, with fp32 statistics and sums.  Two more masks, a kernel each:
+//
+//   a window   j <= p and (j > p - window or j < sinks).  A block walks the tiles of the first positions and those
+//              from its first row's window on, as if they were next to each other (PgSeen); the bits of a
+//              tile that some row does not see in full are made of the row's two borders
+//   a tree     j < len - n, and draft d = j - (len - n) where bit d of the row's words is set.  The words lie in LDS
+//              behind a word of ones (the past) and before one of zeros, so the 32 bits of a tile are
+//              two reads and a shift, wherever the past ends
 //
 // Operands.  bf16 values go to the matrix cores as they are.  An fp32 value is
 // the sum of three bf16 terms, x = h + m + l: h is x rounded to nearest, m what is left
@@ -56,6 +63,11 @@
 //   the same on fp32 pages (six products for one; more than 64 rows a sequence: about 50 registers
 //     spill): 159 us; bf16 rows on fp32 pages (three for one): 82 us
 //   31 new rows behind 993, all fp32: 19.6 to 20.7 us, a chain of first loads and the join's launch
+//   windows: one prompt of 8191 rows, bf16, 1024 positions and 64 first ones: 129 to 134 us, 68 GFLOP, products (three for
+//     two) at 800 TFLOP/s: a block walks 18 turns, and begins and ends as long as 9 take; 8 pieces of 51 to 515 rows behind
+//     500 to 4000, fp32 rows on bf16 pages, 1000 positions: 51 us
+//   trees: 24 x 21 to 64 drafts behind 170 to 4000, bf16: 54 us and 6 for the join (216 MB, 45 us at a copy's rate): one
+//     block a CU, whose begin and end nothing covers; 16 drafts behind 529, fp32: 18.5 us
 //
 // Masked keys: a masked score is -inf before the maximum, but 0 times what the
 // cache holds is no number where that is infinite or none.  Such a V

@@ -29,7 +29,8 @@ def fork_reference(table, lens, parent, new, outside, page, n_pages):
     for s in range(n):
         if new[s] == 0:
             continue
-        copied = tails[s] >= 0 and (tails[s] in whole or tails[s] in tails[s + 1:])
+        more = any(tails[t] == tails[s] and (length[t] % page, t) > (length[s] % page, s) for t in range(n))
+        copied = tails[s] >= 0 and (tails[s] in whole or more)
         first = length[s] // page if inside[s] and (copied or tails[s] < 0) else kept[s]
         need = -(-(length[s] + new[s]) // page)
         missing += max(need - max(stride, -(-length[s] // page)), 0)

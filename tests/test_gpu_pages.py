@@ -56,13 +56,13 @@ def test_fork_beams(qa, gpu, page, seed):
 
 @pytest.mark.parametrize("held", [[], [0, 31, 32, 40], list(range(0, 96, 2))])
 def test_fork_rules(qa, gpu, held):
-    """who keeps a page: the last row that has it as its last; none where a row has it for positions behind or the
-    program holds it; a row without new rows leaves its own"""
+    """who keeps a page: the row with the most positions in it, of several the last; none where a row has it for positions
+    behind or the program holds it; a row without new rows leaves its own"""
     a, b, c = 40, 41, 42
-    table = [[a, b, -1, -1], [a, b, c, -1], [a, -1, -1, -1], [-1, b, -1, -1], [a, 96, 7, -1], [-1] * 4]
-    lens = [24, 40, 10, 20, 32, 0]
+    table = [[a, b, -1, -1], [a, b, c, -1], [a, -1, -1, -1], [-1, b, -1, -1], [a, 96, 7, -1], [-1] * 4, [a, -1, -1, -1]]
+    lens = [24, 40, 10, 20, 32, 0, 12]
     n = len(lens)
-    for parent in ([0, 0, 0], [0, 1, 0], [2, 2, 2, 0], [2, 2], [3, 3, 3], [1, 1, 0, 0, 2, 2, 3, 5, -1], [4, 4, 4], list(range(n)), None):
+    for parent in ([2, 6], [6, 2], [6, 2, 2], [2, 6, 6, 2], [0, 0, 0], [0, 1, 0], [2, 2, 2, 0], [2, 2], [3, 3, 3], [1, 1, 0, 0, 2, 2, 3, 5, -1], [4, 4, 4], list(range(n)), None):
         rows = n if parent is None else len(parent)
         for new in (None, [1] * rows, [0] * (rows - 1) + [5], [(9 * i) % 20 for i in range(rows)], [16] * rows):
             same_fork(qa, table, lens, parent, new, held, 16, 96)
@@ -124,32 +124,36 @@ def test_fork_from_no_table(qa, gpu):
     assert cp.tolist() == [[-1, -1, 0, 0]] * n and int(ms) == 0
 
 
-def test_fork_step_by_step(qa, gpu):
-    """beams over many steps: no page is ever two rows' to write, what a row's positions hold is what its ancestors wrote"""
-    rng, page, n_pages, stride = random.Random(5), 4, 80, 16
-    table, lens = [[-1] * stride], [0]
-    table, lens, _, miss = G.fork(qa, table, lens, [0], [6], [], page, n_pages)
-    assert miss == 0
-    store = {}                                             # (page, slot) -> what a row wrote
-    said = [[("prompt", i) for i in range(6)]]
-    for i in range(6):
-        store[table[0][i // page], i % page] = said[0][i]
-    for step in range(40):
-        n = rng.choice([1, 3, 6])
-        parent = [rng.randrange(len(table)) for _ in range(n)]
-        table, lens, copies, miss = same_fork(qa, table, lens, parent, [1] * n, [], page, n_pages)
+@pytest.mark.parametrize("waiting", [False, True])
+def test_fork_step_by_step(qa, gpu, waiting):
+    """beams over many steps: what a row's positions hold is what its ancestors wrote; `waiting`: some rows stand still for
+    steps (no new rows) while others of the same past go on, in any order"""
+    rng, page, n_pages, stride = random.Random(5), 4, 120, 16
+    for start in range(8 if waiting else 1):
+        table, lens = [[-1] * stride], [0]
+        table, lens, _, miss = G.fork(qa, table, lens, [0], [6], [], page, n_pages)
         assert miss == 0
-        for a, b, first, slots in copies:
-            for i in range(first, first + slots):
-                store[b, i] = store[a, i]
-        said = [said[p] + [(step, s)] for s, p in enumerate(parent)]
-        for s in range(n):
-            l = lens[s] - 1
-            store[table[s][l // page], l % page] = said[s][l]
-        for s in range(n):
-            assert [store[table[s][i // page], i % page] for i in range(lens[s])] == said[s], (step, s)
-        if lens[0] > 50:
-            break
+        store = {}                                         # (page, slot) -> what a row wrote
+        said = [[("prompt", i) for i in range(6)]]
+        for i in range(6):
+            store[table[0][i // page], i % page] = said[0][i]
+        for step in range(40):
+            n = rng.choice([1, 3, 6]) if not waiting else rng.choice([3, 6, 8])
+            parent = [rng.randrange(len(table)) for _ in range(n)]
+            new = [rng.choice([0, 0, 1, 2]) if waiting else 1 for _ in range(n)]
+            table, lens, copies, miss = same_fork(qa, table, lens, parent, new, [], page, n_pages)
+            assert miss == 0
+            for a, b, first, slots in copies:
+                for i in range(first, first + slots):
+                    store[b, i] = store[a, i]
+            said = [said[p] + [(step, s, i) for i in range(new[s])] for s, p in enumerate(parent)]
+            for s in range(n):
+                for i in range(lens[s] - new[s], lens[s]):
+                    store[table[s][i // page], i % page] = said[s][i]
+            for s in range(n):
+                assert [store[table[s][i // page], i % page] for i in range(lens[s])] == said[s], (start, step, s)
+            if max(lens) > 50:
+                break
 
 
 # ---------------------------------------------------------------------------

@@ -40,8 +40,8 @@ def compact(qa, kvd={}, bd={}, change=None, n_layers=2, **k):
 
 
 def beam(qa, **k):
-    d = dict(parent=P, token=P, score_out=P, logits=P, dtype=qa.ST_F32, row_stride=1000, seqs=2, beams=4, vocab=1000, score=P,
-             ended=P, n_out=8, ws=P, ws_bytes=1 << 40)
+    d = dict(parent=P, token=P, score_out=P, logits=P, dtype=qa.ST_F32, row_stride=1000, seqs=2, beams=4, vocab=1000, score=Q,
+             ended=Q + 0x10000, n_out=8, ws=P, ws_bytes=1 << 40)
     d.update(k)
     return qa.lib().qwen_hip_beam_select(*d.values(), None)
 
@@ -74,6 +74,7 @@ def test_fork_workspace(qa):
     assert need(1 << 19) == 0 and need(1 << 19, 1024) == 0
     n = need((1 << 19) + 1)
     assert n >= 2 * ((1 << 19) + 1) // 8
+    assert fork(qa, kvd=dict(table_stride=1 << 30)) == EINVAL and "page ids" in qa.last_error()
     assert need((1 << 19) + 1, 0) == need((1 << 19) + 1, 1025) == L.qwen_hip_paged_fork_ws_bytes(None, 1) == 0
     big = dict(n_pages=(1 << 19) + 1, page_size=1)
     for bad in (dict(ws=None, ws_bytes=n), dict(ws=Q, ws_bytes=n - 1), dict(ws=Q + 4, ws_bytes=n)):
@@ -120,7 +121,8 @@ def test_nothing_is_no_call(qa):
                                  dict(seqs=(1 << 14) + 1), dict(seqs=2 ** 31 - 1), dict(dtype=1), dict(dtype=-1), dict(row_stride=999),
                                  dict(row_stride=-1000), dict(parent=None), dict(token=None), dict(score_out=None),
                                  dict(logits=None), dict(score=None), dict(logits=P + 2), dict(ws=None), dict(ws=P + 4),
-                                 dict(ws_bytes=0)])
+                                 dict(ws_bytes=0), dict(score_out=Q - 8), dict(score_out=Q + 28), dict(parent=Q), dict(token=Q),
+                                 dict(parent=Q + 0x10000 - 60), dict(token=Q + 0x10000), dict(score_out=Q + 0x10000 + 31)])
 def test_beam_refused(qa, bad):
     assert beam(qa, **bad) == EINVAL
     assert "beam_select" in qa.last_error()
