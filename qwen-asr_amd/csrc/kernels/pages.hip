@@ -149,18 +149,25 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
     tails[tid] = tail;                                // -1 behind the last row
     parts[tid] = slots;
     __syncthreads();
-    bool copied = false;
-    if (tail >= 0 && fresh_rows > 0) {
-        copied = get(whole + (tail >> 5)) >> (tail & 31) & 1u;
-#pragma unroll 4
-        for (int j = 0; j < a.n_out; j += 4) {
+    // whether another row has more of the tail: `width` threads a part of the rows each
+    ranks[tid] = 0;
+    __syncthreads();
+    int width = 64;
+    while (width < a.n_out) width *= 2;
+    const int mine = tid & (width - 1), my_tail = tails[mine], my_part = parts[mine];
+    if (my_tail >= 0) {
+        bool found = false;
+        for (int j = 4 * (tid / width); j < a.n_out; j += 4 * (FK_THREADS / width)) {
             const int4 t = *reinterpret_cast<const int4 *>(tails + j), p = *reinterpret_cast<const int4 *>(parts + j);
             auto more = [&](int tail_j, int part_j, int i) {
-                return tail_j == tail && (part_j > slots || (part_j == slots && i > tid));
+                return tail_j == my_tail && (part_j > my_part || (part_j == my_part && i > mine));
             };
-            copied = copied || more(t.x, p.x, j) || more(t.y, p.y, j + 1) || more(t.z, p.z, j + 2) || more(t.w, p.w, j + 3);
+            found = found || more(t.x, p.x, j) || more(t.y, p.y, j + 1) || more(t.z, p.z, j + 2) || more(t.w, p.w, j + 3);
         }
+        if (found) ranks[mine] = 1;
     }
+    __syncthreads();
+    const bool copied = tail >= 0 && fresh_rows > 0 && (ranks[tid] || (get(whole + (tail >> 5)) >> (tail & 31) & 1u));
     FkRow r = {kept, 0, -1};
     if (on) {
         const long need = ((long)len + fresh_rows + P - 1) >> a.page_shift;
@@ -183,9 +190,9 @@ __global__ __launch_bounds__(FK_THREADS) void paged_fork(qk_paged_fork_args a) {
         const unsigned f = ~get(held + w);
         return w == words - 1 && (a.n_pages & 31) ? f & ((1u << (a.n_pages & 31)) - 1) : f;
     };
-    int mine = 0, all;
-    for (int w = w0; w < w1; w++) mine += __popc(free_bits(w));
-    ranks[tid] = fk_scan(mine, part, all);
+    int free_pages = 0, all;
+    for (int w = w0; w < w1; w++) free_pages += __popc(free_bits(w));
+    ranks[tid] = fk_scan(free_pages, part, all);
     if (tid == 0) *a.missing = (int)min((long)over + max(total - all, 0), (long)INT_MAX);
     __syncthreads();
     // the last of n ascending numbers that is at most x (the first is 0)
