@@ -5,7 +5,7 @@
 // Whole numbers and copies of bits: the results are exact.
 //
 // Measured (a device copy moves 4.8 to 5.1 TB/s): 64 beams of 131 to 701 positions, 28 layers, bf16, pages of 32: table
-// 9 us (a chain of loads and barriers in one block), copies of 31 half pages, 112 MB read and written, 25 to 33 us; 4 beams
+// 8 us (a chain of loads and barriers in one block), copies of 31 half pages, 112 MB read and written, 25 to 33 us; 4 beams
 // of 530, fp32: 5 and 3 us, less than the two calls take.  Accepted drafts of 1 and of 24 sequences, 28 layers: 9 us, a launch.
 #include "paged.h"
 
@@ -30,7 +30,7 @@ typedef uint32_t pages_u32x4 __attribute__((ext_vector_type(4)));
 //
 // One block: the work is a few thousand table entries (64 rows of 24 pages) between barriers, and what is
 // held is a bit a page, in LDS up to FK_LDS_PAGES pages, in the workspace beyond.  Rows are taken four at a time a wave, fresh
-// pages a thread each (a thread a word of bits, its free ones in turn: 19 us for 64 beams instead of 9).
+// pages a thread each (a thread a word of bits, its free ones in turn: 19 us for 64 beams instead of 8).
 // ---------------------------------------------------------------------------
 #define FK_THREADS 1024
 #define FK_WAVES (FK_THREADS / 64)
