@@ -308,6 +308,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
 #define BS_LIST 4096
 #define BS_COUNTED 256                // shares whose n-th largest is found by counting
 #define BS_RANKED 128                 // candidates that are ranked as they are
+#define BS_MANY 768
 #define BS_ACTIVE 2048                // shares whose entries are looked at
 
 struct BsKey {
@@ -532,7 +533,17 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
             mine[j] = i < count ? list[i] : BsKey{0, 0};
             if (mine[j] > most) most = mine[j];
         }
-        T0 = wave_bound(most);
+        // of many, whose ranks would take longer than a bound for all of them, few more than n
+        if (count > BS_MANY) {
+            T0 = bound(64 + n, [&](const BsKey &u) {
+                int c = 0;
+#pragma unroll
+                for (int j = 0; j < BS_LIST / BS_THREADS; j++) c += __popcll(__ballot(mine[j] >= u));
+                return c;
+            });
+        } else {
+            T0 = wave_bound(most);
+        }
         if (tid == 0) count = 0;                      // every thread has its part of the list
         __syncthreads();
 #pragma unroll

@@ -35,6 +35,22 @@ def test_beam_vocabulary(qa, gpu, dtype, seqs, beams, n_out):
     check_beam(beam(qa, x, score, None, n_out, seqs), x, score, None, seqs)
 
 
+@pytest.mark.parametrize("dtype,rows,seqs,n_out", [("f32", 3, 1, 64), ("bf16", 4, 2, 20), ("f32", 2, 2, 3)])
+def test_beam_largest_vocabulary(qa, gpu, dtype, rows, seqs, n_out):
+    x, score, _ = inputs(77, rows, 1 << 20, dtype)
+    check_beam(beam(qa, x, score, None, n_out, seqs), x, score, None, seqs)
+
+
+@pytest.mark.parametrize("n_out", [1, 7, 64])
+def test_beam_many_like_candidates(qa, gpu, n_out):
+    """thousands of candidates within a share's few: a list of them has to be cut more than once"""
+    g = T.Generator().manual_seed(78)
+    x = T.full((1, 5000), -30.0)
+    x[:, ::3] = T.randint(0, 3, (1, 1667), generator=g).float() * 1e-6
+    x = x.repeat(64, 1).cuda()                             # equal beams: which comes first is the definition's
+    check_beam(beam(qa, x, [-1.0] * 64, None, n_out, 1), x, [-1.0] * 64, None, 1)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("skew", [0, 1, 2, 3, 5, 7])
 @pytest.mark.parametrize("pad", [0, 1, 13])
