@@ -131,18 +131,19 @@ int qwen_hip_paged_append_at(const qwen_hip_paged_kv *kv, const qwen_hip_paged_b
  */
 static int tokens_by_matrix(int cache_bf16, int group) { return cache_bf16 && group > 4; }
 
-/*
- * splits of an attention call and the workspace it needs.  The plans split into at most
- * ceil(T / blocks) for a number T of blocks that they aim at, and not at all from T blocks on.  A
- * block has up to R rows of heads, so rows x heads x splits is at most R blocks (T + blocks - 1) / blocks
- * < 2 R T: for prompts 2 x 128 x 384, for single tokens 2 x 8 x 2048 (fewer heads a block: as many).
- * Times 520 bytes, that is below QWEN_HIP_PAGED_ATTENTION_WS_MAX for any batch.
- */
 enum { ALL, WINDOW, TREE };
 typedef struct {
     int kind, window, sinks;
 } seen_keys;
 
+/*
+ * splits of an attention call and the workspace it needs.  The plans split into at most
+ * ceil(T / blocks) for a number T of blocks that they aim at, and not at all from T blocks on.  A
+ * block has up to R rows of heads, so rows x heads x splits is at most R blocks (T + blocks - 1) / blocks
+ * < 2 R T: for prompts 2 x 128 x 384, for single tokens 2 x 8 x 2048 (fewer heads a block: as many).
+ * Of masks the splits are at most T / blocks: 128 x 512, and 64 x 768 with blocks of 64 rows.
+ * Times 520 bytes, that is below QWEN_HIP_PAGED_ATTENTION_WS_MAX for any batch.
+ */
 static size_t attention_plan(const qk_paged *p, seen_keys seen, int matrix, int heads, int max_len, int *rows2, int *nsplit,
                              int *chunk) {
     if (max_len == 0 || max_len > p->capacity) max_len = p->capacity;

@@ -64,8 +64,9 @@
 //     spill): 159 us; bf16 rows on fp32 pages (three for one): 82 us
 //   31 new rows behind 993, all fp32: 19.6 to 20.7 us, a chain of first loads and the join's launch
 //   windows: one prompt of 8191 rows, bf16, 1024 positions and 64 first ones: 129 to 134 us, 68 GFLOP, products (three for
-//     two) at 800 TFLOP/s: a block walks 18 turns, and begins and ends as long as 9 take; 8 pieces of 51 to 515 rows behind
-//     500 to 4000, fp32 rows on bf16 pages, 1000 positions: 51 us
+//     two) at 800 TFLOP/s: a block walks 17 to 18 turns, 0.46 of that time products, and begins and ends as long as 2 to 3
+//     take; 8 pieces of 51 to 515 rows behind 500 to 4000, fp32 rows on bf16 pages, 1000 positions: 51 us (begin and end: 4
+//     of 21 turns' time)
 //   trees: 24 x 21 to 64 drafts behind 170 to 4000, bf16: 54 us and 6 for the join (216 MB, 45 us at a copy's rate): one
 //     block a CU, whose begin and end nothing covers; 16 drafts behind 529, fp32: 18.5 us
 //
@@ -898,24 +899,52 @@ extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, 
     return rows2;
 }
 
-// Windows and trees of drafts.  Their blocks walk as many keys each (a window's) or as their sequence has (a
-// tree's), whose lengths differ; the host knows the mean of the sequences' rows, and takes each to have as many.  One
-// block of 128 rows a CU, two of 64 on bf16 pages, one on fp32 pages.
-//   rows   64 where a sequence has no more as a rule (8 x 32 drafts of 2 heads behind 250 to 2000, fp32 rows on bf16
-//          pages: 29 us, 31 with 128; 8 x 8 to 32 on fp32 pages: 38, 44).  Of a window also where its blocks are short
-//          (4 prompts of 500 to 2000 rows, bf16, 512 positions: 51 us, 54; but 1 of 8191 rows, 1024 positions: 134, 129;
-//          8 of 51 to 515, fp32 rows on bf16 pages, 1000 positions: 57, 51), which fp32 pages have no room for
-//   splits as many as the blocks, all of one length, find room for at once (4 x 100 to 700 rows, fp32, 512 positions:
-//          1 split, 180 blocks: 66 us; 2: 91; 1 x 64 drafts, bf16, behind 8000: 256 blocks 25, 336 34); of a tree whose
-//          blocks are many unsplit half as many more, as the long sequences would be waited for (24 x 21 to 64 drafts, bf16, behind 170 to 4000: 192 blocks 84 us, 384 60, 576 78; 4 x 100 to 200 of 4 heads
-//          behind 1500 to 6000: 160 blocks 122, 320 82, 480 107)
+// How many items of work (blocks by splits) the blocks of a call with a mask become, at most.  A CU has room for two of
+// 64 rows on bf16 pages, for one of any other.  A window's are of one length, so a second round of them costs as much as
+// the first; a tree's differ by sequence, the more sequences the more, and more items than there is room for at
+// once take less time than waiting for the longest.  8 kv heads; blocks unsplit, us by splits:
+//   tree, 64 rows, bf16 pages
+//          8 (1 sequence): 40: 16.4, 60: 16.9;  32: 10: 21, 15: 19;  48: 6: 30, 10: 28, 16: 35;  80: 4: 29, 6: 25, 9: 31
+//          128: 2: 37, 3: 29, 5: 27, 6: 32;  136: 2: 50, 4: 36, 7: 44;  192: 1: 56, 2: 38, 3: 31, 4: 38
+//          256: 1: 59, 2: 54, 3: 50;  384: 1: 77, 2: 68;  512: 1: 50, 2: 55
+//   tree, 64 rows, fp32 pages
+//          32: 4: 77, 8: 47, 10: 81;  48: 5: 55, 6: 47, 8: 60;  64: 3: 47, 4: 42, 5: 38, 6: 58;  96: 2: 109, 3: 79, 4: 88
+//          128: 2: 110, 3: 80, 4: 119;  160: 2: 110, 3: 138;  192: 1: 136, 2: 81, 3: 110;  240: 1: 137, 2: 98
+//          256: 1: 137, 2: 112;  320: 1: 138, 2: 150
+//   tree, 128 rows
+//          144: 2: 48, 3: 57;  160: 1: 122, 2: 82, 3: 107;  192: 1: 86, 2: 60, 3: 79;  240: 1: 77, 2: 73
+//          1 x 64 drafts, bf16, behind 8000: 256 items 25, 336 34
+//   window, 64 rows, bf16 pages
+//          32: 10: 22, 16: 21, 20: 22;  96: 3: 49, 4: 42, 5: 39;  128: 2: 50, 3: 47, 4: 46;  192: 1: 107, 2: 72;  240: 1: 48, 2: 52
+//   window, 64 rows, fp32 pages
+//          8 (1 sequence): 32: 28, 40: 25;  32: 6: 40, 8: 37, 10: 48;  48: 4: 52, 5: 45, 6: 62;  56: 4: 52, 5: 45, 6: 62
+//          64: 3: 63, 4: 52, 5: 74;  80: 2: 84, 3: 66, 4: 86;  96: 2: 148, 3: 109;  104: 2: 86, 3: 97;  160: 1: 144, 2: 151
+//   window, 128 rows
+//          180: 1: 66, 2: 91
+static long tree_items(long blocks, int rows2, int cache_bf16) {
+    if (rows2 && cache_bf16) return blocks < 16 ? 320 : blocks < 128 ? 480 : blocks < 256 ? 640 : 768;
+    if (blocks > 128) return blocks <= 256 ? 2 * blocks : blocks;
+    return blocks == 128 ? 384 : rows2 && blocks >= 48 ? 320 : 256;
+}
+
+static long window_items(long blocks, int rows2, int cache_bf16) {
+    if (rows2 && cache_bf16) return blocks <= 128 ? 512 : 448;
+    if (!rows2 || blocks > 128) return 256;
+    return blocks < 16 ? 320 : 256 + blocks / 2;          // as many splits as come nearest to 256
+}
+
+// Windows and trees of drafts.  The host knows the mean of the sequences' rows, and takes each to have as many.  Blocks
+// of 64 rows where a sequence has no more as a rule (8 x 32 drafts of 2 heads behind 250 to 2000, fp32 rows on bf16
+// pages: 29 us, 31 with 128; 8 x 8 to 32 on fp32 pages: 38, 44).  Of a window also where its blocks are short
+// (4 prompts of 500 to 2000 rows, bf16, 512 positions: 51 us, 54; but 1 of 8191 rows, 1024 positions: 134, 129;
+// 8 of 51 to 515, fp32 rows on bf16 pages, 1000 positions: 57, 51), which fp32 pages have no room for
 extern "C" int qk_paged_masked_plan(const qk_paged *p, int tree, int heads, int max_len, int *nsplit, int *chunk) {
     const long f = (long)p->rows * (heads / p->kv_heads), mean = (f + p->n_seqs - 1) / p->n_seqs;
     const int fits = (f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 1024 : 384;
     const int rows2 = p->page_shift >= 4 && (mean <= PP_ROWS(2) || (!tree && p->cache_bf16 && max_len <= fits));
     const int rows = PP_ROWS(rows2 ? 2 : 4);
     const long blocks = (mean + rows - 1) / rows * p->n_seqs * p->kv_heads;
-    long n = (rows2 ? 320 : tree && blocks >= 128 ? 384 : 256) / blocks;
+    long n = (tree ? tree_items(blocks, rows2, p->cache_bf16) : window_items(blocks, rows2, p->cache_bf16)) / blocks;
     n = n < 1 ? 1 : n > QK_PAGED_MAX_SPLIT ? QK_PAGED_MAX_SPLIT : n;
     long c = ((max_len + n - 1) / n + 63) / 64 * 64;
     c = c < 64 ? 64 : c;
