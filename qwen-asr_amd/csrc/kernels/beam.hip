@@ -37,6 +37,7 @@
 #define BM_THREADS 256
 #define BM_WAVES 4
 #define BM_PART 512                   // entries from a threshold on of a wave: n VPT at most by one of value and index
+#define BM_PAD 8
 #define BM_LOG2E 1.4426950408889634
 
 typedef unsigned long long bm_u64;
@@ -119,7 +120,7 @@ struct BmRows {
 };
 
 // entries that a share lists at most: a power of two
-__host__ __device__ __forceinline__ int bm_slots_log(int n) { return n <= 8 ? 5 : n <= 16 ? 6 : n <= 32 ? 7 : 8; }
+__host__ __device__ __forceinline__ int bm_slots_log(int n) { return n <= 8 ? 5 : n <= 32 ? 6 : 7; }
 
 // a beam that takes no part with its logits: one at its end, one without a score
 __device__ __forceinline__ bool bm_idle(const float *score, const int *ended, int row, int vocab) {
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     __shared__ __attribute__((aligned(16))) bm_u64 list[BM_WAVES * BM_PART];
     __shared__ bm_u64 wkey[BM_WAVES];
     __shared__ double wsum[BM_WAVES];
-    __shared__ int count[BM_WAVES];
+    __shared__ int count[BM_WAVES], steps[BM_THREADS], above[BM_WAVES], cut, kept, place;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int share = blockIdx.y, row = blockIdx.x;
     const T *const x0 = (const T *)a.logits + (size_t)row * a.stride;
@@ -216,6 +217,9 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     // the wave's entries from there on, into its part of the list
     bm_u64 *const part = list + BM_PART * wave;
     int n_part = 0;
+    auto pad = [&]() {                                // what is less than any entry, up to a multiple of BM_PAD
+        if (lane < BM_PAD && n_part + lane < BM_PART) part[n_part + lane] = 0;
+    };
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
         const bool in = x[j] >= T0;
@@ -227,6 +231,8 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
         }
     }
     if (lane == 0) count[wave] = n_part;
+    pad();
+    steps[tid] = 0;
     double sum = 0.0;
     const bool plain = fabsf(M) <= 30.0f;             // relative to 0, not to M
     if (plain) {
@@ -267,6 +273,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
             n_part += __popcll(m);
         }
         if (lane == 0) count[wave] = n_part;
+        pad();
         __syncthreads();
     }
     int before = 0, some = 0;
@@ -282,19 +289,54 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     if (some <= 1 << slots) {
         for (int i = lane; i < n_part; i += 64) out[before + i] = part[i];
     } else {
-        // places by counting
-        result.count = a.n;
-        for (int i = lane; i < n_part; i += 64) {
-            const bm_u64 key = part[i];
-            int rank = 0;
+        // Fewer, by their values' places among BM_THREADS steps of one width from the threshold (no lower than 64 from
+        // the largest) to the largest: those from the step on that n reach.
+        const float from = fmaxf(T0, M - 64.0f), scale = M > from ? (BM_THREADS - 1) / (M - from) : 0.0f;
+        auto step = [&](bm_u64 key) { return (int)fminf(fmaxf((bm_value(key) - from) * scale, 0.0f), BM_THREADS - 1.0f); };
+        for (int i = lane; i < n_part; i += 64) atomicAdd(steps + step(part[i]), 1);
+        if (tid == 0) place = 0;
+        __syncthreads();
+        const int here = steps[tid];
+        int upto = here;                              // of this step and those above it
 #pragma unroll
-            for (int w = 0; w < BM_WAVES; w++)
-                for (int j = 0; j < count[w]; j++) rank += list[BM_PART * w + j] > key;
-            if (rank < a.n) out[rank] = key;
-            if (rank == 0) wkey[0] = key;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_down(upto, d, 64);
+            if (lane + d < 64) upto += v;
+        }
+        if (lane == 0) above[wave] = upto;
+        __syncthreads();
+#pragma unroll
+        for (int w = 1; w < BM_WAVES; w++) upto += w > wave ? above[w] : 0;
+        if (upto >= a.n && upto - here < a.n) {       // one thread's: more than n are listed
+            cut = tid;
+            kept = upto;
         }
         __syncthreads();
-        result.best = wkey[0];
+        if (kept <= 1 << slots) {
+            result.count = kept;
+            for (int i = lane; i < n_part; i += 64)
+                if (step(part[i]) >= cut) out[atomicAdd(&place, 1)] = part[i];
+        } else {
+            // equal ones, or nearly: places by counting
+            result.count = a.n;
+            for (int i = lane; i < n_part; i += 64) {
+                const bm_u64 key = part[i];
+                int rank = 0;
+#pragma unroll
+                for (int w = 0; w < BM_WAVES; w++)
+                    for (int j = 0; j < count[w]; j += BM_PAD) { // loads side by side: one by one, each would be waited for
+                        bm_u64 e[BM_PAD];
+#pragma unroll
+                        for (int u = 0; u < BM_PAD; u++) e[u] = list[BM_PART * w + j + u];
+#pragma unroll
+                        for (int u = 0; u < BM_PAD; u++) rank += e[u] > key;
+                    }
+                if (rank < a.n) out[rank] = key;
+                if (rank == 0) wkey[0] = key;
+            }
+            __syncthreads();
+            result.best = wkey[0];
+        }
     }
     if (tid == 0) a.share[at] = result;
 }
@@ -322,8 +364,10 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
                                                           const bm_u64 *lists) {
     __shared__ double base[QK_BEAM_MAX];                         // score - log(sum); NaN: no candidates by logits
     __shared__ float most[QK_BEAM_MAX];                          // the largest logit
-    __shared__ BsKey bounds[BS_WAVES], list[BS_LIST];
-    __shared__ int counts[3][8], count, n_active, active[BS_ACTIVE], entries[BS_ACTIVE], rank[BS_LIST];
+    __shared__ BsKey list[BS_LIST], nth;
+    __shared__ int counts[3][8], count, n_active, active[BS_ACTIVE], entries[BS_ACTIVE], rank[BS_LIST], above[BS_WAVES], cut, kept;
+    __shared__ bm_u64 lows[BS_WAVES], highs[BS_WAVES], least;
+    int *const steps = rank;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = blockIdx.x, n = a.n_out;
     const int row0 = q * a.beams, cols = a.beams * shares, slots = bm_slots_log(n);
     share += (size_t)row0 * shares;
@@ -425,58 +469,92 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
         __syncthreads();
         return t;
     };
-    BsKey T0 = {0, 0};
-    // The same from the waves' n-th largest: cheaper, and looser where a wave's keys are not a sample of all.  Of a
-    // score's upper half; where more than n are equal in that, by the rest and the places.
-    auto wave_bound = [&](const BsKey &key) {
-        const unsigned high = (unsigned)(key.score >> 32);
-        const unsigned t = bm_bound<unsigned, 32>(high, n);
-        BsKey b = {(bm_u64)t << 32, 0};
-        const int above = __popcll(__ballot(high > t)), equal = __popcll(__ballot(high == t));
-        if (t && above < n && above + equal > n) {
-            const bm_u64 rest = bm_bound<bm_u64, 64>(high == t ? key.score << 32 | key.at : 0, n - above);
-            b = {(bm_u64)t << 32 | rest >> 32, (unsigned)rest};
-        }
-        if (lane == 0) bounds[wave] = b;
+    // Candidates by their scores' places among BS_THREADS steps of one width from `from` to the best: `cut` is the
+    // step from which on at least n of those counted are, `kept` how many.  count(add): the thread's.
+    double from = 0.0, scale = 0.0;
+    auto range = [&](bm_u64 lo, bm_u64 hi) {                     // steps from lo, no lower than e^-64 of the best
+        const double best = bm_double(hi);
+        from = lo ? fmax(bm_double(lo), best - 64.0) : best - 64.0;
+        scale = best > from ? (BS_THREADS - 1) / (best - from) : 0.0;
+    };
+    auto step = [&](const BsKey &k) { return (int)fmin(fmax((bm_double(k.score) - from) * scale, 0.0), BS_THREADS - 1.0); };
+    auto count_steps = [&](auto all) {
+        steps[tid] = 0;
+        if (tid == 0) cut = kept = 0;
         __syncthreads();
-        BsKey most = bounds[0];
+        all([&](const BsKey &k) { atomicAdd(steps + step(k), 1); });
+        __syncthreads();
+        const int here = steps[tid];
+        int upto = here;                                         // of this step and those above it
 #pragma unroll
-        for (int w = 1; w < BS_WAVES; w++)
-            if (bounds[w] > most) most = bounds[w];
-        return most;
-    };
-    // The keys of the block's threads that reach T0, to the list (in no order); how many
-    auto gather = [&](const BsKey &key) {
-        if (tid == 0) count = 0;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_down(upto, d, 64);
+            if (lane + d < 64) upto += v;
+        }
+        if (lane == 0) above[wave] = upto;
         __syncthreads();
-        if (key.score && key >= T0) list[atomicAdd(&count, 1)] = key;
+#pragma unroll
+        for (int w = 1; w < BS_WAVES; w++) upto += w > wave ? above[w] : 0;
+        if (upto >= n && upto - here < n) {                      // one thread's, or none's: fewer than n
+            cut = tid;
+            kept = upto;
+        }
         __syncthreads();
-        return count;
     };
-    // The n-th largest of the threads', by counting, once the waves' bounds have left few enough: the first
-    // of these is loose (a beam's shares are in one or two waves, the best beam's may be fewer than n of a wave).
-    if (cols > BS_COUNTED) T0 = wave_bound(top);
-    int c0 = gather(top);
-    if (c0 > BS_COUNTED) {
-        const BsKey one = tid < c0 ? list[tid] : BsKey{0, 0};
-        T0 = wave_bound(one);
-        c0 = gather(one);
-    }
-    if (c0 > n && c0 <= BS_COUNTED) {
+    // A bound that n of the threads' candidates reach, and few more: of few threads' the n-th largest, by counting
+    BsKey T0 = {0, 0};
+    bm_u64 best = top.score;
+    if (max(cols, a.beams) <= BS_COUNTED) {
         constexpr int PARTS = BS_THREADS / BS_COUNTED;
+        const int i = tid % BS_COUNTED, c = max(cols, a.beams);
+        if (tid < c) list[tid] = top;
         if (tid < BS_COUNTED) rank[tid] = 0;
         __syncthreads();
-        const int i = tid % BS_COUNTED;
-        if (i < c0) {
+        if (i < c) {
             const BsKey one = list[i];
-            int above = 0;
-            for (int j = tid / BS_COUNTED; j < c0; j += PARTS) above += list[j] > one || (j < i && list[j] >= one);
-            atomicAdd(rank + i, above);
+            int larger = 0;
+#pragma unroll 4
+            for (int j = tid / BS_COUNTED; j < c; j += PARTS) larger += list[j] > one || (j < i && list[j] >= one);
+            atomicAdd(rank + i, larger);
+        }
+        if (tid == 0) nth = BsKey{0, 0};
+        __syncthreads();
+        if (tid < c) {
+            if (rank[tid] == n - 1) nth = top;
+            if (rank[tid] == 0) highs[0] = top.score;
         }
         __syncthreads();
-        if (tid < c0 && rank[tid] == n - 1) bounds[0] = list[tid];
+        T0 = nth;
+        best = highs[0];
+    } else {
+        bm_u64 low = top.score ? top.score : ~0ull;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            best = max(best, __shfl_xor(best, d, 64));
+            low = min(low, __shfl_xor(low, d, 64));
+        }
+        if (lane == 0) {
+            highs[wave] = best;
+            lows[wave] = low;
+        }
+        if (tid == 0) least = ~0ull;
         __syncthreads();
-        T0 = bounds[0];
+#pragma unroll
+        for (int w = 0; w < BS_WAVES; w++) {
+            best = max(best, highs[w]);
+            low = min(low, lows[w]);
+        }
+        range(low, best);
+        count_steps([&](auto add) {
+            if (top.score) add(top);
+        });
+        if (kept > 64 + n) {                                     // equal ones, or nearly
+            T0 = bound(64 + n, [&](const BsKey &u) { return (int)__popcll(__ballot(top >= u)); });
+        } else if (kept) {
+            if (top.score && step(top) >= cut) atomicMin(&least, top.score);
+            __syncthreads();
+            T0.score = least;
+        }
     }
     __syncthreads();
     if (tid == 0) count = 0;
@@ -496,59 +574,87 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     const bool every = n_active > BS_ACTIVE;
     const long m = (long)(every ? cols : n_active) << slots;
     auto each = [&](auto take) {
-        for (long i = tid; i < m; i += BS_THREADS) {
-            const int k = (int)(i >> slots), l = every ? k : active[k], slot = (int)i & ((1 << slots) - 1);
-            const int b = (int)((unsigned)l / (unsigned)shares);
-            if (base[b] == base[b] && slot < (every ? share[l].count : entries[k])) take(key_of(b, lists[((size_t)l << slots) + slot]));
+        // four loads on their way at once, of what no share listed as well
+        for (long i0 = tid; i0 < m; i0 += 4 * BS_THREADS) {
+            bm_u64 e[4];
+            int l[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const long i = min(i0 + u * BS_THREADS, m - 1);
+                const int k = (int)(i >> slots), slot = (int)i & ((1 << slots) - 1);
+                l[u] = every ? k : active[k];
+                e[u] = lists[((size_t)l[u] << slots) + slot];
+                if (i0 + u * BS_THREADS >= m || slot >= (every ? share[l[u]].count : entries[k])) e[u] = 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int b = (int)((unsigned)l[u] / (unsigned)shares);
+                if (i0 + u * BS_THREADS < m) take(key_of(b, e[u]));
+            }
         }
         take(end_of(tid));
     };
-    auto collect = [&]() {
-        each([&](const BsKey &k) {
-            if (k.score && k >= T0) {
-                const int at = atomicAdd(&count, 1);
-                if (at < BS_LIST) list[at] = k;
-            }
-        });
-        __syncthreads();
-    };
-    collect();
+    auto hit = [&](const BsKey &k) { return k.score && k >= T0; };
+    each([&](const BsKey &k) {
+        if (hit(k)) {
+            const int at = atomicAdd(&count, 1);
+            if (at < BS_LIST) list[at] = k;
+        }
+    });
+    __syncthreads();
+    range(T0.score, best);
+    // fewer than n: all
+    auto from_cut = [&](const BsKey &k) { return hit(k) && step(k) >= cut; };
     if (count > BS_LIST) {
         // candidates beyond the list (many shares that reach the bound many times over)
-        T0 = bound(BS_LIST, [&](const BsKey &u) {
-            int c = 0;
-            each([&](const BsKey &k) { c += k.score && k >= u; });
-            return (int)wave_sum((float)c);
+        count_steps([&](auto add) {
+            each([&](const BsKey &k) {
+                if (hit(k)) add(k);
+            });
         });
+        if (kept > BS_LIST) {
+            T0 = bound(BS_LIST, [&](const BsKey &u) {
+                int c = 0;
+                each([&](const BsKey &k) { c += k.score && k >= u; });
+                return (int)wave_sum((float)c);
+            });
+            if (tid == 0) cut = 0;
+        }
         if (tid == 0) count = 0;
         __syncthreads();
-        collect();
+        each([&](const BsKey &k) {
+            if (from_cut(k)) list[atomicAdd(&count, 1)] = k;
+        });
+        __syncthreads();
+        range(T0.score, best);
     }
     if (count > BS_RANKED) {
-        // a tighter bound from the list (in no order: a wave's part is a sample)
-        BsKey mine[BS_LIST / BS_THREADS], most = {0, 0};
+        // fewer of the list
+        BsKey mine[BS_LIST / BS_THREADS];
 #pragma unroll
         for (int j = 0; j < BS_LIST / BS_THREADS; j++) {
             const int i = tid + BS_THREADS * j;
             mine[j] = i < count ? list[i] : BsKey{0, 0};
-            if (mine[j] > most) most = mine[j];
         }
-        // of many, whose ranks would take longer than a bound for all of them, few more than n
-        if (count > BS_MANY) {
+        count_steps([&](auto add) {
+#pragma unroll
+            for (int j = 0; j < BS_LIST / BS_THREADS; j++)
+                if (mine[j].score) add(mine[j]);
+        });
+        if (kept > BS_MANY) {                                    // equal ones, or nearly
             T0 = bound(64 + n, [&](const BsKey &u) {
                 int c = 0;
 #pragma unroll
                 for (int j = 0; j < BS_LIST / BS_THREADS; j++) c += __popcll(__ballot(mine[j] >= u));
                 return c;
             });
-        } else {
-            T0 = wave_bound(most);
+            if (tid == 0) cut = 0;
         }
-        if (tid == 0) count = 0;                      // every thread has its part of the list
+        if (tid == 0) count = 0;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < BS_LIST / BS_THREADS; j++)
-            if (mine[j].score && mine[j] >= T0) list[atomicAdd(&count, 1)] = mine[j];
+            if (from_cut(mine[j])) list[atomicAdd(&count, 1)] = mine[j];
         __syncthreads();
     }
     const int c = count;
@@ -560,6 +666,7 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     for (int i = tid % width; i < c; i += width) {
         const BsKey key = list[i];
         int above = 0;
+#pragma unroll 4
         for (int j = tid / width; j < c; j += parts) above += list[j] > key;
         atomicAdd(rank + i, above);
     }

@@ -153,6 +153,36 @@ def test_beam_far_scores(qa, gpu):
     assert set(parent[0, :6].tolist()) == {0, 2} and set(parent[0, 6:].tolist()) == {1, 3}
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("beams,n_out,vocab", [(64, 64, 151936), (40, 64, 20000), (33, 48, 3000), (30, 30, 5000)])
+def test_beam_more_candidates_than_a_list(qa, gpu, dtype, beams, n_out, vocab):
+    """many beams and places: of thousands of shares nearly all may reach what the best ones do"""
+    x, score, g = inputs(16, 2 * beams, vocab, dtype, 1.0)
+    score = [-1.0 - 1e-3 * i for i in range(2 * beams)]
+    ended = [i if i % 8 == 3 else -1 for i in range(2 * beams)]
+    check_beam(beam(qa, x, score, ended, n_out, 2), x, score, ended, 2)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("beams,n_out,vocab", [(4, 4, 151936), (12, 24, 30000), (40, 64, 20000), (64, 64, 5000)])
+@pytest.mark.parametrize("kind", ["one far above", "far below", "near each other", "steps"])
+def test_beam_ranges(qa, gpu, kind, dtype, beams, n_out, vocab):
+    """what the candidates' range is cut by: one far above all others, nearly all far below, nearly all equal, few values"""
+    x, score, g = inputs(17, beams, vocab, "f32", 1.0)
+    if kind == "one far above":
+        x[:, 7::5000] = 1e4
+        x[beams // 2:, 7::5000] = 0.0
+    elif kind == "far below":
+        x[:, T.randperm(vocab, generator=g)[:vocab - n_out // 2].cuda()] -= 1e4
+        score = [-1.0 if b % 3 else -5e4 for b in range(beams)]
+    elif kind == "near each other":
+        x = 5.0 + 1e-6 * x
+    else:
+        x = (x * 2).round() / 2
+    x = x.to(DT[dtype])
+    check_beam(beam(qa, x, score, None, n_out, 1), x, score, None, 1)
+
+
 def test_beam_many_rows(qa, gpu):
     x, score, _ = inputs(12, 4096, 300)
     check_beam(beam(qa, x, score, None, 2, 512), x, score, None, 512)
