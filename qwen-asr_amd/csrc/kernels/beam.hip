@@ -8,18 +8,21 @@
 //   beam_rows    block (share of a row): its maximum and sum of exponentials, and its entries from a threshold
 //                on that n of them reach: with the threads in n groups or more, the least of the
 //                groups' maxima, which about 3 n do (of a share that leaves groups empty: the n-th
-//                largest of a wave's threads').  Where more than a list holds do, by equal values
-//                (forbidden entries of the type's lowest value), indexes enter a bound: of the threads' largest
-//                entries by value and index, the n-th in each wave, the largest of these; at most n
-//                threads of each wave reach it, and 4 n VPT entries.  More than 4 n (32) of them are brought in order
-//                and the first n kept.
+//                largest of a wave's threads').  Of more than a list holds, 32 to 128 by n, those from the step of their
+//                range on that n reach; of equal ones (forbidden entries of the type's lowest value), and
+//                where too many are in one step, the n-th largest value by its bits, and the lowest indexes of that.
 //   beam_select  block (sequence): each beam's logarithm from its shares; a bound from the shares' largest
-//                entries, the entries of the shares that reach it, and the n best of these.
+//                entries (the n-th of them by counting; of many the waves' n-th largest, or the steps of their range), the entries of the shares that reach
+//                it, fewer of these by steps, and the n best.  What a step holds too many of is cut by the bits of
+//                score and place.
 //
-// Measured: 16 x 8 beams of 151936 fp32 entries, 16 places, one beam in eight at its end: 33 us, rows 24 (78 MB, 14 without
-// lists and exponentials: exponentials 3, entries to the lists and their order 6), choice 10 (a chain of loads, logarithms
-// and bounds in one block a sequence); 1 x 4 beams, 4 places: 4 and 7 us; 8 x 16 beams, 32 places: 52.
-// Exponentials of 64-bit differences took 3 us more, a bound by the n-th largest thread and every list in order 8.
+// Measured: 16 x 8 beams of 151936 fp32 entries, 16 places, one beam in eight at its end: 32 us, rows 23 (78 MB, 14 without
+// lists and exponentials: exponentials 3, entries to the lists 5), choice 10 (a chain of loads, logarithms
+// and bounds in one block a sequence); 1 x 4 beams, 4 places: 4 and 8 us; 8 x 16 beams, 32 places: 37; 2 x 32 beams, 64 places:
+// 37; 8 x 8 beams of equal logits, 16 places: 66.
+// Exponentials of 64-bit differences took 3 us more, a bound by the n-th largest thread and every list in order 8.  Lists brought
+// in order by counting, and a block's bounds by bits alone: 8 x 16 beams 52, 7 x 14 beams of 38397, 28 places 53 (22),
+// 2 x 32, 64 places 11.1 ms (a loose bound for the shares, thousands of candidates, 96 bits for all of them).
 //
 // Exponentials: log2(e) x in two fp32 terms, its whole part into the exponent, v_exp_f32 (1 ulp) of the rest, where the
 // share's maximum lies within 30 of 0 (no x is subtracted from then, so nothing is rounded before); otherwise of
@@ -36,8 +39,7 @@
 
 #define BM_THREADS 256
 #define BM_WAVES 4
-#define BM_PART 512                   // entries from a threshold on of a wave: n VPT at most by one of value and index
-#define BM_PAD 8
+#define BM_PART 512                   // entries from a threshold on of a wave
 #define BM_LOG2E 1.4426950408889634
 
 typedef unsigned long long bm_u64;
@@ -137,6 +139,7 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     __shared__ bm_u64 wkey[BM_WAVES];
     __shared__ double wsum[BM_WAVES];
     __shared__ int count[BM_WAVES], steps[BM_THREADS], above[BM_WAVES], cut, kept, place;
+    __shared__ bm_u64 first;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int share = blockIdx.y, row = blockIdx.x;
     const T *const x0 = (const T *)a.logits + (size_t)row * a.stride;
@@ -217,9 +220,6 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     // the wave's entries from there on, into its part of the list
     bm_u64 *const part = list + BM_PART * wave;
     int n_part = 0;
-    auto pad = [&]() {                                // what is less than any entry, up to a multiple of BM_PAD
-        if (lane < BM_PAD && n_part + lane < BM_PART) part[n_part + lane] = 0;
-    };
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
         const bool in = x[j] >= T0;
@@ -231,7 +231,6 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
         }
     }
     if (lane == 0) count[wave] = n_part;
-    pad();
     steps[tid] = 0;
     double sum = 0.0;
     const bool plain = fabsf(M) <= 30.0f;             // relative to 0, not to M
@@ -249,33 +248,6 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     sum = bm_sum(sum);
     if (lane == 0) wsum[wave] = sum;
     __syncthreads();
-    if (max(max(count[0], count[1]), max(count[2], count[3])) > BM_PART) {
-        // the thread's first largest entry
-        bm_u64 top = 0;
-#pragma unroll
-        for (int j = 0; j < VPT; j++) {
-            const bm_u64 key = bm_key(x[j], index(j / V) + j % V);
-            if (x[j] > -INFINITY && key > top) top = key;
-        }
-        const bm_u64 t = bm_bound<bm_u64, 64>(top, a.n);
-        if (lane == 0) wkey[wave] = t;
-        __syncthreads();                              // every thread has seen the counts
-        bm_u64 T1 = wkey[0];
-#pragma unroll
-        for (int w = 1; w < BM_WAVES; w++) T1 = wkey[w] > T1 ? wkey[w] : T1;
-        n_part = 0;
-#pragma unroll
-        for (int j = 0; j < VPT; j++) {
-            const bm_u64 key = bm_key(x[j], index(j / V) + j % V);
-            const bool in = x[j] > -INFINITY && key >= T1;
-            const bm_u64 m = __ballot(in);
-            if (in) part[n_part + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0u))] = key;
-            n_part += __popcll(m);
-        }
-        if (lane == 0) count[wave] = n_part;
-        pad();
-        __syncthreads();
-    }
     int before = 0, some = 0;
 #pragma unroll
     for (int w = 0; w < BM_WAVES; w++) {
@@ -286,9 +258,10 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
     const int slots = bm_slots_log(a.n);
     bm_u64 *const out = a.list + (at << slots);
     BmShare result = {(wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), plain ? 0.0f : M, some, M > -INFINITY ? bm_key(M, 0xffffffffu) : 0};
+    bool like = max(max(count[0], count[1]), max(count[2], count[3])) > BM_PART;
     if (some <= 1 << slots) {
         for (int i = lane; i < n_part; i += 64) out[before + i] = part[i];
-    } else {
+    } else if (!like) {
         // Fewer, by their values' places among BM_THREADS steps of one width from the threshold (no lower than 64 from
         // the largest) to the largest: those from the step on that n reach.
         const float from = fmaxf(T0, M - 64.0f), scale = M > from ? (BM_THREADS - 1) / (M - from) : 0.0f;
@@ -317,26 +290,73 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
             for (int i = lane; i < n_part; i += 64)
                 if (step(part[i]) >= cut) out[atomicAdd(&place, 1)] = part[i];
         } else {
-            // equal ones, or nearly: places by counting
-            result.count = a.n;
-            for (int i = lane; i < n_part; i += 64) {
-                const bm_u64 key = part[i];
-                int rank = 0;
-#pragma unroll
-                for (int w = 0; w < BM_WAVES; w++)
-                    for (int j = 0; j < count[w]; j += BM_PAD) { // loads side by side: one by one, each would be waited for
-                        bm_u64 e[BM_PAD];
-#pragma unroll
-                        for (int u = 0; u < BM_PAD; u++) e[u] = list[BM_PART * w + j + u];
-#pragma unroll
-                        for (int u = 0; u < BM_PAD; u++) rank += e[u] > key;
-                    }
-                if (rank < a.n) out[rank] = key;
-                if (rank == 0) wkey[0] = key;
-            }
-            __syncthreads();
-            result.best = wkey[0];
+            like = true;
         }
+    }
+    if (like) {
+        // Equal ones, or nearly: the n-th largest value v, its bits from the top; what is above it, and as many of v
+        // as are missing, the lowest indexes first.
+        unsigned r[VPT], v = 0;
+#pragma unroll
+        for (int j = 0; j < VPT; j++) r[j] = x[j] > -INFINITY ? bm_rank(x[j]) : 0u;
+        __syncthreads();                              // every thread is behind the steps
+        steps[tid] = 0;
+        if (tid == 0) {
+            place = 0;
+            first = 0;
+        }
+        __syncthreads();
+        for (int b = 31; b >= 0; b--) {
+            const unsigned u = v | 1u << b;
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < VPT; j++) c += __popcll(__ballot(r[j] >= u));
+            if (lane == 0 && c) atomicAdd(steps + b, c);
+            __syncthreads();
+            if (steps[b] >= a.n) v = u;
+        }
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < VPT; j++) c += __popcll(__ballot(r[j] > v));
+        if (lane == 0 && c) atomicAdd(steps + 32, c);
+        int *const equal = steps + 64;                // [NV][BM_WAVES]
+#pragma unroll
+        for (int p = 0; p < NV; p++) {
+            int e = 0;
+#pragma unroll
+            for (int k = 0; k < V; k++) e += __popcll(__ballot(r[V * p + k] == v));
+            if (lane == 0) equal[BM_WAVES * p + wave] = e;
+        }
+        __syncthreads();
+        const int missing = a.n - steps[32];
+        int below = 0;                                // of v with lower indexes: those of the planes before, ...
+#pragma unroll
+        for (int p = 0; p < NV; p++) {
+            int to = below;
+#pragma unroll
+            for (int w = 0; w < BM_WAVES; w++) {
+                to += w < wave ? equal[BM_WAVES * p + w] : 0;
+                below += equal[BM_WAVES * p + w];
+            }
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                const bm_u64 m = __ballot(r[V * p + k] == v);
+                to += (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0u));
+            }
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                const bool is = r[V * p + k] == v;
+                if (r[V * p + k] > v || (is && to < missing)) {
+                    const bm_u64 key = (bm_u64)r[V * p + k] << 32 | (0xffffffffu - (unsigned)(index(p) + k));
+                    out[atomicAdd(&place, 1)] = key;
+                    atomicMax(&first, key);
+                }
+                to += is;
+            }
+        }
+        __syncthreads();
+        result.count = a.n;
+        result.best = first;
     }
     if (tid == 0) a.share[at] = result;
 }
@@ -526,6 +546,23 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
         __syncthreads();
         T0 = nth;
         best = highs[0];
+    } else if (n <= 16) {
+        // of few places the waves' n-th largest do, by the scores' upper halves (4 beams, 4 places: 8.1 us, by steps 9.5)
+        const unsigned high = (unsigned)(top.score >> 32), t = bm_bound<unsigned, 32>(high, n);
+        unsigned most = high;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, d, 64));
+        if (lane == 0) {
+            highs[wave] = (bm_u64)most << 32 | 0xffffffffu;
+            lows[wave] = (bm_u64)t << 32;
+        }
+        __syncthreads();
+        best = 0;
+#pragma unroll
+        for (int w = 0; w < BS_WAVES; w++) {
+            best = max(best, highs[w]);
+            T0.score = max(T0.score, lows[w]);
+        }
     } else {
         bm_u64 low = top.score ? top.score : ~0ull;
 #pragma unroll
@@ -561,7 +598,8 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     for (int i = tid; i < cols; i += BS_THREADS) {
         const BmShare s = i == tid ? first : share[i];
         const BsKey k = best_of(i, s);
-        if (k.score && k.score >= T0.score) {
+        // (what is of no known index may be of any)
+        if (k.score > T0.score || (k.score && k.score == T0.score && (!k.at || k.at >= T0.at))) {
             const int at = atomicAdd(&n_active, 1);
             if (at < BS_ACTIVE) {
                 active[at] = i;
@@ -685,9 +723,9 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     }
 }
 
-// Entries a thread: few for few rows, whose shares have to fill the card, and for many places (BM_LIST).
+// Entries a thread: few for few rows, whose shares have to fill the card, and not too many for many places (8 x 20
+// beams, 40 places: 8 entries 54 us, 16 46, 32 44; 8 x 16, 32 places: 43, 37, 39; 2 x 5 of 300, 64 places: 16, 16, 18).
 static int vpt(int rows, int vocab, int n) {
-    if (n > 32) return 8;
     if (n > 16) return 16;
     return (long)rows * vocab < 4 << 20 ? 8 : 32;
 }
