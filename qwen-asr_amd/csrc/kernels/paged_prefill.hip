@@ -900,8 +900,8 @@ extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, 
 }
 
 // How many items of work (blocks by splits) the blocks of a call with a mask become, at most.  A CU has room for two of
-// 64 rows on bf16 pages, for one of any other.  A window's are of one length, so a second round of them costs as much as
-// the first; a tree's differ by sequence, the more sequences the more, and more items than there is room for at
+// 64 rows on bf16 pages, for one of any other.  A window's are of one length (even), so a second round of them costs as much as
+// the first; a tree's, or those of a window that few rows fill, differ, and more items than there is room for at
 // once take less time than waiting for the longest.  8 kv heads; blocks unsplit, us by splits:
 //   tree, 64 rows, bf16 pages
 //          8 (1 sequence): 40: 16.4, 60: 16.9;  32: 10: 21, 15: 19;  48: 6: 30, 10: 28, 16: 35;  80: 4: 29, 6: 25, 9: 31
@@ -914,6 +914,7 @@ extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, 
 //   tree, 128 rows
 //          144: 2: 48, 3: 57;  160: 1: 122, 2: 82, 3: 107;  192: 1: 86, 2: 60, 3: 79;  240: 1: 77, 2: 73
 //          1 x 64 drafts, bf16, behind 8000: 256 items 25, 336 34
+//   window of 1659 over 2 x 220 to 852 rows, fp32 (136): 1: 83, 2: 60, 3: 51
 //   window, 64 rows, bf16 pages
 //          32: 10: 22, 16: 21, 20: 22;  96: 3: 49, 4: 42, 5: 39;  128: 2: 50, 3: 47, 4: 46;  192: 1: 107, 2: 72;  240: 1: 48, 2: 52
 //   window, 64 rows, fp32 pages
@@ -921,13 +922,25 @@ extern "C" int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, 
 //          64: 3: 63, 4: 52, 5: 74;  80: 2: 84, 3: 66, 4: 86;  96: 2: 148, 3: 109;  104: 2: 86, 3: 97;  160: 1: 144, 2: 151
 //   window, 128 rows
 //          180: 1: 66, 2: 91
-static long tree_items(long blocks, int rows2, int cache_bf16) {
-    if (rows2 && cache_bf16) return blocks < 16 ? 320 : blocks < 128 ? 480 : blocks < 256 ? 640 : 768;
-    if (blocks > 128) return blocks <= 256 ? 2 * blocks : blocks;
-    return blocks == 128 ? 384 : rows2 && blocks >= 48 ? 320 : 256;
+//   short ones, whose begin and end, and the join's launch, cost more than splits give, by keys:
+//          192, 128 rows, bf16 pages: 360: 1: 19, 2: 33;  1060: 32, 39;  1560: 42, 43;  fp32 rows: 360: 27, 42;  1560: 60, 58
+//          192, 128 rows, fp32 pages: 360: 1: 52, 2: 68;  660: 76, 76;  1060: 112, 96;  64 rows: 100: 20, 33;  300: 32, 36;  600: 51, 47
+//          192, 64 rows, bf16 pages: 300: 1: 13, 3: 15;  600: 19, 18;  80, 128 rows: 160: 1: 13, 3: 19;  360: 17, 20;  660: 24, 22
+//          8, 64 rows, bf16 pages: 170: 1: 11, 3: 13;  270: 12, 13;  420: 13, 12;  32, fp32 rows: 170: 13, 14;  270: 16, 14
+static int unsplit_keys(long blocks, int rows2, int cache_bf16) {
+    if (!cache_bf16) return blocks > 128 ? 512 : 0;
+    if (blocks > 128 && !rows2) return 1500;
+    return blocks >= 64 ? 448 : 256;
 }
 
-static long window_items(long blocks, int rows2, int cache_bf16) {
+static long uneven_items(long blocks, int rows2, int cache_bf16, int keys) {
+    if (keys <= unsplit_keys(blocks, rows2, cache_bf16)) return blocks;
+    if (rows2 && cache_bf16) return blocks < 16 ? 320 : blocks < 128 ? 480 : blocks < 256 ? 640 : 768;
+    if (blocks > 128) return blocks <= 256 ? 2 * blocks : blocks;
+    return blocks == 128 ? 384 : rows2 && (blocks >= 48 || blocks < 16) ? 320 : 256;
+}
+
+static long even_items(long blocks, int rows2, int cache_bf16) {
     if (rows2 && cache_bf16) return blocks <= 128 ? 512 : 448;
     if (!rows2 || blocks > 128) return 256;
     return blocks < 16 ? 320 : 256 + blocks / 2;          // as many splits as come nearest to 256
@@ -938,13 +951,13 @@ static long window_items(long blocks, int rows2, int cache_bf16) {
 // pages: 29 us, 31 with 128; 8 x 8 to 32 on fp32 pages: 38, 44).  Of a window also where its blocks are short
 // (4 prompts of 500 to 2000 rows, bf16, 512 positions: 51 us, 54; but 1 of 8191 rows, 1024 positions: 134, 129;
 // 8 of 51 to 515, fp32 rows on bf16 pages, 1000 positions: 57, 51), which fp32 pages have no room for
-extern "C" int qk_paged_masked_plan(const qk_paged *p, int tree, int heads, int max_len, int *nsplit, int *chunk) {
+extern "C" int qk_paged_masked_plan(const qk_paged *p, int tree, int even, int heads, int max_len, int *nsplit, int *chunk) {
     const long f = (long)p->rows * (heads / p->kv_heads), mean = (f + p->n_seqs - 1) / p->n_seqs;
     const int fits = (f / PP_ROWS(2) + p->n_seqs) * p->kv_heads >= 320 ? 1024 : 384;
     const int rows2 = p->page_shift >= 4 && (mean <= PP_ROWS(2) || (!tree && p->cache_bf16 && max_len <= fits));
     const int rows = PP_ROWS(rows2 ? 2 : 4);
     const long blocks = (mean + rows - 1) / rows * p->n_seqs * p->kv_heads;
-    long n = (tree ? tree_items(blocks, rows2, p->cache_bf16) : window_items(blocks, rows2, p->cache_bf16)) / blocks;
+    long n = (even ? even_items(blocks, rows2, p->cache_bf16) : uneven_items(blocks, rows2, p->cache_bf16, max_len)) / blocks;
     n = n < 1 ? 1 : n > QK_PAGED_MAX_SPLIT ? QK_PAGED_MAX_SPLIT : n;
     long c = ((max_len + n - 1) / n + 63) / 64 * 64;
     c = c < 64 ? 64 : c;

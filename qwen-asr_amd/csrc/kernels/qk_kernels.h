@@ -525,8 +525,8 @@ typedef struct {
 void qk_paged_decode_plan(int n_seqs, int heads, int kv_heads, int cache_bf16, int max_len, int *nsplit, int *chunk);
 /* returns qk_paged_attn_args.rows2 */
 int qk_paged_prefill_plan(const qk_paged *p, int heads, int max_len, int *nsplit, int *chunk);
-/* the same of a window (max_len: what a block walks) or a tree of drafts */
-int qk_paged_masked_plan(const qk_paged *p, int tree, int heads, int max_len, int *nsplit, int *chunk);
+/* the same of a window (max_len: what a block walks) or a tree of drafts; even: most blocks walk as many keys */
+int qk_paged_masked_plan(const qk_paged *p, int tree, int even, int heads, int max_len, int *nsplit, int *chunk);
 int qk_paged_decode_launch(const qk_paged_attn_args *a, hipStream_t s);
 int qk_paged_prefill_launch(const qk_paged_attn_args *a, hipStream_t s);
 /* joins the partials into out */
