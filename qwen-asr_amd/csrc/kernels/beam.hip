@@ -12,8 +12,8 @@
 //                range on that n reach; of equal ones (forbidden entries of the type's lowest value), and
 //                where too many are in one step, the n-th largest value by its bits, and the lowest indexes of that.
 //   beam_select  block (sequence): each beam's logarithm from its shares; a bound from the shares' largest
-//                entries (the n-th of them by counting; of many the waves' n-th largest, or the steps of their range), the entries of the shares that reach
-//                it, fewer of these by steps, and the n best.  What a step holds too many of is cut by the bits of
+//                entries (the n-th of them by counting; of many the waves' n-th largest, or the steps of their
+//                range), the entries of the shares that reach it, fewer of these by steps, and the n best.  What a step holds too many of is cut by the bits of
 //                score and place.
 //
 // Measured: 16 x 8 beams of 151936 fp32 entries, 16 places, one beam in eight at its end: 32 us, rows 23 (78 MB, 14 without
