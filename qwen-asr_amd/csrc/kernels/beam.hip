@@ -51,8 +51,12 @@ struct BmShare {                      // of a row
     bm_u64 best;                      // the largest entry; without an index (0 in its place) where it is not known; 0: none
 };
 
-// what is no number is no entry (the middle of three is the least one then), +inf the largest number
-__device__ __forceinline__ float bm_clean(float x) { return __builtin_amdgcn_fmed3f(x, -INFINITY, 3.402823466e38f); }
+// What is no number is no entry, +inf the largest number.  Asked for outright: of a maximum, a minimum or a middle with
+// infinite constants the compiler leaves the minimum alone, which takes no number for the constant.  Largest by the bits:
+// as whole numbers the positive ones are in order, and all negative ones below them.
+__device__ __forceinline__ float bm_clean(float x) {
+    return __int_as_float(min(__float_as_int(x == x ? x : -INFINITY), 0x7f7fffff));
+}
 
 // the order of values (-0 is 0), and of entries: larger first, then the lower index; 0 is none
 __device__ __forceinline__ unsigned bm_rank(float x) {
