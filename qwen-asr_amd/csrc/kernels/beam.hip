@@ -85,13 +85,15 @@ __device__ __forceinline__ float bm_exp2(double t) {
     return __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)(unsigned)(bm_u64)__double_as_longlong(z));
 }
 
-// e^x for |x| of tens, e^-80 below (nothing beside a largest one of e^-30): y + r = x log2(e), y's whole part z by
-// adding 1.5 2^23, into the exponent's place
+// e^x for |x| of tens, e^-80 below (nothing beside a largest one of e^-30): x log2(e) less its whole part, that by adding
+// 1.5 2^23, into the exponent's place.  Every product is part of an fma of its own: a product that is used twice may be
+// taken unrounded in one of the places, and rounded in the other.  Off by v_exp_f32's 1 ulp, 2^-23, and what two fmas
+// round of a number up to 1/2, ln 2 2^-25.
 __device__ __forceinline__ float bm_exp(float x) {
     const float magic = 12582912.0f, L = 1.44269504e+00f, L2 = 1.92596299e-08f;
     x = fmaxf(x, -80.0f);
-    const float y = x * L, z = y + magic, r = fmaf(x, L2, fmaf(x, L, -y));
-    return __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f((y - (z - magic)) + r)) + (__float_as_uint(z) << 23));
+    const float z = fmaf(x, L, magic), f = fmaf(x, L2, fmaf(x, L, magic - z));
+    return __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(f)) + (__float_as_uint(z) << 23));
 }
 
 __device__ __forceinline__ double bm_sum(double v) {             // of a wave, the same in every lane
