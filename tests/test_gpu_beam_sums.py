@@ -36,3 +36,26 @@ def test_error_of_the_logarithm(qa, gpu, dtype, vocab, low, high):
     """an exponential: 2^-23 (v_exp_f32's 1 ulp) and ln 2 2^-25 (its argument up to 1/2, rounded twice); one of the share's
     reference the same; two are added in fp32: 2^-24.  Less than 3 x 2^-23 of the sum."""
     assert error(qa, dtype, vocab, low, high) <= 3 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("top", [40.0, -40.0, 300.0, 1e4])
+def test_shares_are_joined_exactly(qa, gpu, top):
+    """two entries far apart in the row: each is its share's reference, its sum 1, so that what joins them is all there is;
+    in 64 bits that is off by some 2^-50, and by what is written of a number below 2^-20 with 24 bits"""
+    rows, vocab = 96, 40000
+    below = T.linspace(0.0, 6.0, rows)
+    x = T.full((rows, vocab), -np.inf)
+    x[:, 0], x[:, vocab - 1] = top, top - below
+    d = x[:, vocab - 1].double() - top
+    lse = T.log1p(T.exp(d))
+    score = lse.float()
+    out = beam(qa, x.cuda(), score.tolist(), None, 1, rows)[2][:, 0].astype(np.float64)
+    assert float(np.abs(out - (score.double() - lse).numpy()).max()) <= 2.0 ** -44
+
+
+@TYPES
+@VOCAB
+@RANGES
+def test_error_of_the_sum(qa, gpu, dtype, vocab, low, high):
+    """an exponential: 2^-23 and ln 2 2^-25, as above; two are added in fp32: 2^-24.  Less than 2^-22 of the sum."""
+    assert error(qa, dtype, vocab, low, high) <= 1.25 * 2.0 ** -23 + (vocab > 1) * 2.0 ** -24
