@@ -632,13 +632,14 @@ int qwen_hip_paged_compact(const qwen_hip_paged_kv *layers, int n_layers, const 
 /* The n_out best continuations of each sequence's beams: candidates are the tokens of its `beams` rows
  * of logits ([seqs * beams][vocab] of `dtype`, QWEN_HIP_ST_F32 or _BF16, rows row_stride entries
  * apart), each with score[row] + logit - log(sum of e^logit over the row); by falling score, equal
- * ones by row and token.  The k-th of sequence q goes to place q * n_out + k of parent (its row,
- * as qwen_hip_paged_fork takes it), token and score_out (fp32).  A beam at its end
+ * ones by row, then by falling logit (scores that differ by less than 64 bits hold are equal: beside a
+ * score of -1e30 all of a row's), then by token.  The k-th of sequence q goes to place q * n_out + k of parent (its row,
+ * as qwen_hip_paged_fork takes it), token and score_out (fp32: -infinity where a score is below its numbers).  A beam at its end
  * (ended[row] in 0 .. vocab - 1; ended may be NULL) has one candidate: that token, with its
  * score as it is.  Logits that are no number count as -infinity, +infinity as the largest fp32 number;
  * what has the score -infinity is no candidate, nor has a beam one whose score is not finite.
- * Places without a candidate get -1, -1, -infinity.  Scores are held and compared in 64 bits
- * (exponentials in fp32).  beams and n_out up to 64, vocab up to 2^20, seqs * beams up to
+ * Places without a candidate get -1, -1, -infinity.  Scores are held and compared in 64 bits (exponentials
+ * in fp32: a row's logarithm is off by less than 2^-22).  beams and n_out up to 64, vocab up to 2^20, seqs * beams up to
  * 2^16.  The outputs overlap neither score nor ended.  The same inputs give the same choice. */
 size_t qwen_hip_beam_select_ws_bytes(int seqs, int beams, int vocab, int n_out);
 int qwen_hip_beam_select(int *parent, int *token, float *score_out, const void *logits, int dtype, long row_stride,

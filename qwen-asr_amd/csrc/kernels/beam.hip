@@ -3,7 +3,7 @@
 //
 //   score_b + x_i - M_b - log(sum_i e^(x_i - M_b)),   M_b = max_i x_i
 //
-// by falling score, equal ones by (b, i).  One pass over the logits:
+// by falling score, equal ones by b, then by falling x, then by i.  One pass over the logits:
 //
 //   beam_rows    block (share of a row): its maximum and sum of exponentials, and its entries from a threshold
 //                on that n of them reach: with the threads in n groups or more, the least of the
@@ -369,8 +369,9 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
 }
 
 // ---------------------------------------------------------------------------
-// A candidate is ordered by its score (64 bits), then by its place among the sequence's candidates (beam * vocab +
-// token, the lower first).
+// A candidate is ordered by its score (64 bits), then by beam (the lower first), logit and token (the lower first).  Scores
+// of one beam do not fall with the logit, so this is the order of the shares' lists, also where scores differ by
+// less than 64 bits hold (beside a score of -1e30, or of +inf as the largest number).
 // ---------------------------------------------------------------------------
 #define BS_THREADS 1024
 #define BS_WAVES (BS_THREADS / 64)
@@ -379,10 +380,12 @@ __global__ __launch_bounds__(BM_THREADS) void beam_rows(BmRows a) {
 #define BS_RANKED 128                 // candidates that are ranked as they are
 #define BS_MANY 768
 #define BS_ACTIVE 2048                // shares whose entries are looked at
+#define BS_AT 60                      // bits of BsKey.at, in threes
+#define BS_TOKEN ((1u << 20) - 1)
 
 struct BsKey {
     bm_u64 score;                     // 0: none
-    unsigned at;                      // 2^32 - 1 - place
+    bm_u64 at;                        // 63 - beam in 6 bits, the logit's order in 32, 2^20 - 1 - token in 20
     __device__ __forceinline__ bool operator>(const BsKey &o) const { return score > o.score || (score == o.score && at > o.at); }
     __device__ __forceinline__ bool operator>=(const BsKey &o) const { return !(o > *this); }
 };
@@ -425,12 +428,16 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     if (tid == 0) count = n_active = 0;
     if (tid < 24) counts[tid / 8][tid % 8] = 0;
     __syncthreads();
+    auto at_of = [](int b, unsigned order, unsigned token) {
+        return (bm_u64)(QK_BEAM_MAX - 1 - b) << 52 | (bm_u64)order << 20 | (BS_TOKEN - token);
+    };
+    // (what is of no known index has the last: as good as that at least)
     auto key_of = [&](int b, bm_u64 e) {
         const double s = base[b];
         BsKey k = {0, 0};
         if (s == s && e) {
             k.score = bm_order(s + ((double)bm_value(e) - (double)most[b]));
-            k.at = (unsigned)e ? 0xffffffffu - ((unsigned)b * a.vocab + bm_index(e)) : 0u;
+            k.at = at_of(b, (unsigned)(e >> 32), (unsigned)e ? bm_index(e) : BS_TOKEN);
         }
         return k;
     };
@@ -441,7 +448,7 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
             const float s = a.score[row0 + b];
             const int t = a.ended[row0 + b];
             if ((unsigned)t < (unsigned)a.vocab && fabsf(s) <= 3.402823466e38f)
-                k = {bm_order((double)s), 0xffffffffu - ((unsigned)b * a.vocab + t)};
+                k = {bm_order((double)s), at_of(b, 0u, (unsigned)t)};
         }
         return k;
     };
@@ -458,16 +465,15 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     }
     // A bound that at least n of the block's keys reach, and at most `enough` where it can be: the bits of the n-th
     // largest from the top, three at a time, until so few are left.  own(u): how many of the thread's keys reach u.
-    auto bound = [&](int enough, auto own) {
-        BsKey t = {0, 0};
-        for (int b = 96 - 3, turn = 0; b >= 0; b -= 3, turn = turn == 2 ? 0 : turn + 1) {
+    // Its score is one of low .. high, so it has the bits that these begin with.
+    auto bound = [&](int enough, bm_u64 low, bm_u64 high, auto own) {
+        const int open = low == high ? 0 : (66 - __clzll((long long)(low ^ high))) / 3 * 3;
+        BsKey t = {open < 64 ? high >> open << open : 0, 0};
+        for (int b = BS_AT + open - 3, turn = 0; b >= 0; b -= 3, turn = turn == 2 ? 0 : turn + 1) {
             auto with = [&](unsigned k) {                        // t with k in the bits b .. b + 2
                 BsKey u = t;
-                if (b >= 32) u.score |= (bm_u64)k << (b - 32);
-                else {
-                    u.at |= k << b;
-                    if (b > 29) u.score |= k >> (32 - b);
-                }
+                if (b >= BS_AT) u.score |= (bm_u64)k << (b - BS_AT);
+                else u.at |= (bm_u64)k << b;
                 return u;
             };
             int mine = 0;                                        // of lane k: the wave's keys that reach with(k)
@@ -593,7 +599,7 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
             if (top.score) add(top);
         });
         if (kept > 64 + n) {                                     // equal ones, or nearly
-            T0 = bound(64 + n, [&](const BsKey &u) { return (int)__popcll(__ballot(top >= u)); });
+            T0 = bound(64 + n, low, best, [&](const BsKey &u) { return (int)__popcll(__ballot(top >= u)); });
         } else if (kept) {
             if (top.score && step(top) >= cut) atomicMin(&least, top.score);
             __syncthreads();
@@ -606,7 +612,7 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
         const BmShare s = i == tid ? first : share[i];
         const BsKey k = best_of(i, s);
         // (what is of no known index may be of any)
-        if (k.score > T0.score || (k.score && k.score == T0.score && (!k.at || k.at >= T0.at))) {
+        if (k.score > T0.score || (k.score && k.score == T0.score && (k.at | BS_TOKEN) >= T0.at)) {
             const int at = atomicAdd(&n_active, 1);
             if (at < BS_ACTIVE) {
                 active[at] = i;
@@ -658,7 +664,7 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
             });
         });
         if (kept > BS_LIST) {
-            T0 = bound(BS_LIST, [&](const BsKey &u) {
+            T0 = bound(BS_LIST, T0.score, best, [&](const BsKey &u) {
                 int c = 0;
                 each([&](const BsKey &k) { c += k.score && k >= u; });
                 return (int)wave_sum((float)c);
@@ -687,7 +693,7 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
                 if (mine[j].score) add(mine[j]);
         });
         if (kept > BS_MANY) {                                    // equal ones, or nearly
-            T0 = bound(64 + n, [&](const BsKey &u) {
+            T0 = bound(64 + n, T0.score, best, [&](const BsKey &u) {
                 int c = 0;
 #pragma unroll
                 for (int j = 0; j < BS_LIST / BS_THREADS; j++) c += __popcll(__ballot(mine[j] >= u));
@@ -719,9 +725,8 @@ __global__ __launch_bounds__(BS_THREADS) void beam_select(qk_beam_args a, int sh
     for (int i = tid; i < c; i += BS_THREADS) {
         if (rank[i] >= n) continue;
         const BsKey key = list[i];
-        const unsigned place = 0xffffffffu - key.at;
-        a.parent[o + rank[i]] = row0 + (int)(place / a.vocab);
-        a.token[o + rank[i]] = (int)(place % a.vocab);
+        a.parent[o + rank[i]] = row0 + QK_BEAM_MAX - 1 - (int)(key.at >> 52);
+        a.token[o + rank[i]] = (int)(BS_TOKEN - ((unsigned)key.at & BS_TOKEN));
         a.score_out[o + rank[i]] = (float)bm_double(key.score);
     }
     for (int i = c + tid; i < n; i += BS_THREADS) {
