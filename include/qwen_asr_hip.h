@@ -603,8 +603,8 @@ int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_pa
  * in order.  So a page is free as soon as no row names it, and the old table means nothing any
  * more.  *missing (device) is how many pages there were not, or the table's rows had no
  * room for (at most 2^31 - 1): their entries are -1, and a last page that could not be copied is lost to its row.
- *   The same inputs give the same tables.  kv->k, kv->v may be NULL.  table_out and
- * len_out do not overlap the table and kv_len.  The workspace is 0 bytes up to 2^19 pages.
+ *   The same inputs give the same tables.  kv->k, kv->v may be NULL.  No output overlaps
+ * an input, but for len_out in the very place of parent or of new_rows.  The workspace is 0 bytes up to 2^19 pages.
  * No rows: nothing to launch, *missing stays. */
 size_t qwen_hip_paged_fork_ws_bytes(const qwen_hip_paged_kv *kv, int n_out);
 int qwen_hip_paged_fork(const qwen_hip_paged_kv *kv, const int *kv_len, const int *parent, const int *new_rows,
@@ -623,7 +623,7 @@ int qwen_hip_paged_copy(const qwen_hip_paged_kv *layers, int n_layers, const int
  * attention), path[s] (rows path_stride entries apart) names n_path[s] of them, ascending
  * (draft 0 .. n - 1), and the i-th goes to position kv_len - n + i.  The list ends before an
  * entry that is no draft or not above the one before it.  len_out[s] is the length with what was
- * accepted (the sequence's positions behind it are free); it does not overlap kv_len.  A draft
+ * accepted (the sequence's positions behind it are free); it overlaps no input.  A draft
  * or a place without a page is left out of the moves.  The pages that are written belong
  * to one sequence. */
 int qwen_hip_paged_compact(const qwen_hip_paged_kv *layers, int n_layers, const qwen_hip_paged_batch *batch, int *len_out,

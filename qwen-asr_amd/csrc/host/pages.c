@@ -12,10 +12,13 @@
 #define BEAM_MAX_VOCAB (1 << 20)
 #define BEAM_MAX_ROWS (1 << 16)
 
-/* n values at a and m at b, 4 bytes each */
-static int overlap(const void *a, size_t n, const void *b, size_t m) {
-    return a && b && (uintptr_t)a < (uintptr_t)b + 4 * m && (uintptr_t)b < (uintptr_t)a + 4 * n;
+/* n bytes at a and m at b */
+static int overlap_bytes(const void *a, size_t n, const void *b, size_t m) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
 }
+
+/* n values at a and m at b, 4 bytes each */
+static int overlap(const void *a, size_t n, const void *b, size_t m) { return overlap_bytes(a, 4 * n, b, 4 * m); }
 
 /* the cache's shape, checked; its sequences as ones of a row each */
 static int shape(const char *op, const qwen_hip_paged_kv *kv, qk_paged *p) {
@@ -80,6 +83,19 @@ int qwen_hip_paged_fork(const qwen_hip_paged_kv *kv, const int *kv_len, const in
     const size_t need = qk_paged_fork_ws_bytes(p.n_pages);
     if (need > 0 && (!ws || ws_bytes < need || !qk_aligned16(ws)))
         QK_REFUSE("%s: workspace of %zu bytes at %p (needs %zu, 16-byte aligned)", op, ws_bytes, ws, need);
+    /* what one thread writes another may read later; of lengths in the place of parents or new rows it is the same one */
+    const struct {
+        const void *at;
+        size_t n;
+    } outs[] = {{table_out, out}, {len_out, n_out}, {copies, 4 * (size_t)n_out}, {missing, 1}};
+    for (int i = 0; i < 4; i++) {
+        const int own = i == 1;
+        if (overlap_bytes(outs[i].at, 4 * outs[i].n, outside, p.n_pages) || overlap(outs[i].at, outs[i].n, p.table, in) ||
+            overlap(outs[i].at, outs[i].n, kv_len, p.n_seqs) ||
+            (!(own && outs[i].at == parent) && overlap(outs[i].at, outs[i].n, parent, n_out)) ||
+            (!(own && outs[i].at == new_rows) && overlap(outs[i].at, outs[i].n, new_rows, n_out)))
+            QK_REFUSE("%s: an output overlaps an input", op);
+    }
     const qk_paged_fork_args a = {.table = p.table, .kv_len = kv_len, .parent = parent, .new_rows = new_rows,
                                   .outside = outside, .table_out = table_out, .len_out = len_out, .copies = copies,
                                   .missing = missing, .n_in = p.n_seqs, .n_out = n_out, .stride = p.table_stride,
@@ -115,6 +131,11 @@ int qwen_hip_paged_compact(const qwen_hip_paged_kv *layers, int n_layers, const 
     if (p.n_seqs == 0) return 0;
     if (!p.table || !p.kv_len || !len_out || !path || !n_path) QK_REFUSE("%s: a pointer is NULL", op);
     if (overlap(len_out, p.n_seqs, p.kv_len, p.n_seqs)) QK_REFUSE("%s: the new lengths overlap the old ones", op);
+    /* every layer's blocks read what the first one's would write over */
+    if (overlap(len_out, p.n_seqs, n_path, p.n_seqs) || overlap(len_out, p.n_seqs, p.row_start, (size_t)p.n_seqs + 1) ||
+        overlap(len_out, p.n_seqs, p.table, (size_t)p.n_seqs * p.table_stride) ||
+        overlap(len_out, p.n_seqs, path, (size_t)(p.n_seqs - 1) * path_stride + (path_stride < p.rows ? path_stride : p.rows)))
+        QK_REFUSE("%s: the new lengths overlap an input", op);
     QK_TRY(qk_paged_compact_launch(&L, &p, len_out, path, path_stride, n_path, s));
     return 0;
 }
