@@ -1,5 +1,5 @@
-"""Logits that are no number: each such row is a sequence of one beam, so that what it gives is what is
-compared (tests/pages_util.py has the definition)."""
+"""Logits that are no number: each such row is a sequence of one beam, or the beam whose candidates come first,
+so that what it gives is what is compared (tests/pages_util.py has the definition)."""
 import math
 
 import pytest
@@ -75,3 +75,33 @@ def test_rows_of_no_numbers(qa, gpu, dtype, vocab, n_out):
             assert (parent[q] == -1).all() and (token[q] == -1).all() and (out[q] == -math.inf).all()
         assert all(t % 2 for t in token[1] if t >= 0)
         assert token[2, 0] == vocab - 1 and abs(out[2, 0] + 3.0) <= 2.0 ** -22 and (token[2, 1:] == -1).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("beams,n_out", [(2, 2), (8, 16), (40, 64)])
+def test_such_beams_among_others(qa, gpu, dtype, beams, n_out):
+    """the beam with entries that are no number is the best by far: its own candidates come first, then the others'"""
+    vocab = 5003
+    for k, bits in enumerate(NANS[dtype]):
+        x = normal(k, beams, vocab, dtype, 0.5)
+        score = [-30.0 - 0.01 * b for b in range(beams)]
+        b = beams // 2
+        score[b] = 0.0
+        score = T.tensor(score).tolist()                   # as the call takes them: in fp32
+        finite = [4, 1001, 1002, 4090, 5001]
+        keep = x[b, finite].clone()
+        put(x, b, slice(None), bits)
+        x[b, finite] = keep
+        x = x.cuda()
+        got = beam(qa, x, score, None, n_out, 1)
+        check_beam(got, x, score, None, 1)
+        n = min(n_out, 5)
+        assert (got[0][0, :n] == b).all() and set(got[1][0, :n].tolist()) <= set(finite)
+        assert (got[0][0, n:] != b).all()
+        # ... and one without a number at all has none of the places
+        y = x.cpu()
+        put(y, b, slice(None), bits)
+        y = y.cuda()
+        got = beam(qa, y, score, None, n_out, 1)
+        check_beam(got, y, score, None, 1)
+        assert (got[0] != b).all() and (got[0] >= 0).all()
