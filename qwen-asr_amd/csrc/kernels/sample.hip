@@ -89,8 +89,10 @@ struct SmY {
     int bin;                      // not falling with y
 };
 
-// Any l: what is -infinity or no number gets the last class, which weighs nothing.
+// Any l: what is -infinity or no number gets the last class, which weighs nothing.  y is the rounded product wherever it is
+// used: taken unrounded into a later difference, beside lo, what was rounded would count twice.
 __device__ __forceinline__ SmY sm_y(const SmPar &p, float l) {
+#pragma clang fp contract(off)
     // M - l and its rounding error
     const float d0 = p.M - l, bb = d0 - p.M, e0 = (p.M - (d0 - bb)) - (l + bb);
     const bool top = l == p.M;                   // also inf - inf
