@@ -567,7 +567,8 @@ int qwen_hip_paged_attention_prefill(const qwen_hip_paged_kv *kv, const qwen_hip
  * packed rows), but a row at position p sees only the positions p - window + 1 .. p and
  * the first `sinks` ones (0 .. sinks - 1, up to p).  window > 0, sinks >= 0.  Pages that hold
  * no position that a row sees are not read: their ids may be -1, so a stream that does
- * not end keeps a window's pages and the first ones. */
+ * not end keeps a window's pages and the first ones.  As exact as the two above: single tokens as
+ * _decode, packed rows as _prefill (of bf16 rows with probabilities, and fp32 values, to 2^-17). */
 size_t qwen_hip_paged_attention_window_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads,
                                                 int window, int sinks);
 int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out,
@@ -578,7 +579,9 @@ int qwen_hip_paged_attention_window(const qwen_hip_paged_kv *kv, const qwen_hip_
  * sequence's n sees the positions before its drafts (those below kv_len - n), and of the n drafts
  * the ones whose bit is set in its `words` 64-bit words (tree [rows][words], device, 8-byte
  * aligned; draft d is bit d % 64 of word d / 64; words 1 .. 4).  A tree's row has the bits of
- * itself and its ancestors; any other bits do as well, and a row that sees nothing gets 0. */
+ * itself and its ancestors; any other bits do as well, and a row that sees nothing gets 0.  As exact
+ * as _prefill, one row a sequence too: of bf16 rows with probabilities, and the values of an fp32 cache,
+ * to 2^-17. */
 size_t qwen_hip_paged_attention_tree_ws_bytes(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, int heads);
 int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_paged_batch *batch, void *out, const void *q,
                                   int dtype, int heads, float scale, const uint64_t *tree, int words, void *ws,
@@ -601,7 +604,7 @@ int qwen_hip_paged_attention_tree(const qwen_hip_paged_kv *kv, const qwen_hip_pa
  *   Fresh pages are those that no entry of the new table names and outside (bytes [n_pages],
  * not 0: a page that the program holds besides; NULL: none) does not, lowest first, to the rows
  * in order.  So a page is free as soon as no row names it, and the old table means nothing any
- * more.  *missing (device) is how many pages there were not, or the table's rows had no
+ * more.  A call reads and writes all of the table: its time grows with the rows' width.  *missing (device) is how many pages there were not, or the table's rows had no
  * room for (at most 2^31 - 1): their entries are -1, and a last page that could not be copied is lost to its row.
  *   The same inputs give the same tables.  kv->k, kv->v may be NULL.  No output overlaps
  * an input, but for len_out in the very place of parent or of new_rows.  The workspace is 0 bytes up to 2^19 pages.

@@ -16,10 +16,11 @@
 //                range), the entries of the shares that reach it, fewer of these by steps, and the n best.  What a step holds too many of is cut by the bits of
 //                score and place.
 //
-// Measured: 16 x 8 beams of 151936 fp32 entries, 16 places, one beam in eight at its end: 32 us, rows 23 (78 MB, 14 without
-// lists and exponentials: exponentials 3, entries to the lists 5), choice 10 (a chain of loads, logarithms
+// Measured: 16 x 8 beams of 151936 fp32 entries, 16 places, one beam in eight at its end: 31 us, rows 22 (78 MB, 14 without
+// lists and exponentials: exponentials 2 to 3, entries to the lists 5), choice 10 (a chain of loads, logarithms
 // and bounds in one block a sequence); 1 x 4 beams, 4 places: 4 and 8 us; 8 x 16 beams, 32 places: 37; 2 x 32 beams, 64 places:
-// 37; 8 x 8 beams of equal logits, 16 places: 66.
+// 37; 8 x 8 beams of equal logits, 16 places: 66; 1 x 64, 64 places: 257 (the bits of score, logit and place over all
+// lists in one block; from the first bit on, not the first that differs, 956).
 // Exponentials of 64-bit differences took 3 us more, a bound by the n-th largest thread and every list in order 8.  Lists brought
 // in order by counting, and a block's bounds by bits alone: 8 x 16 beams 52, 7 x 14 beams of 38397, 28 places 53 (22),
 // 2 x 32, 64 places 11.1 ms (a loose bound for the shares, thousands of candidates, 96 bits for all of them).

@@ -6,7 +6,10 @@
 //
 // Measured (a device copy moves 4.8 to 5.1 TB/s): 64 beams of 131 to 701 positions, 28 layers, bf16, pages of 32: table
 // 8 us (a chain of loads and barriers in one block), copies of 31 half pages, 112 MB read and written, 25 to 33 us; 4 beams
-// of 530, fp32: 5 and 3 us, less than the two calls take.  Accepted drafts of 1 and of 24 sequences, 28 layers: 9 us, a launch.
+// of 530, fp32: 5 and 3 us, less than the two calls take.  A wave takes four rows of the table, 64 entries of each at
+// a time, so wide tables of few rows are one wave's work: one row of 24 entries 5 us, of 1251 11, of 6251 39, of 62501
+// 350; 64 rows of 1251 22, of 6251 71; and 1024 rows of 24, each compared with all others, 132.  Accepted drafts of 1
+// and of 24 sequences, 28 layers: 9 us, a launch.
 #include "paged.h"
 
 #include <limits.h>
